@@ -76,6 +76,9 @@ int once_per_device(PerDeviceOnce& o, int dev, F&& init) {
 // run beside them size their grids for those SMs.
 int gemm_sm_reserve();
 
+// SMs of the current device that a persistent tensor-core launch may hold (all but the reserve).
+int gemm_usable_sms();
+
 // Router logits for few tokens on the CUDA cores (router.cu); dmoe_router_logits uses it when
 // T is small, where the tensor-core logits GEMM would run on one or two CTAs.
 bool logits_few_tokens_eligible(int T, int d, int E);
