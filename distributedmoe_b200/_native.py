@@ -8,6 +8,7 @@ sizes and the current CUDA stream; the kernels run inside the library.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -82,6 +83,21 @@ SIGNATURES = {
     "dmoe_grouped_gated_mlp_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int,
                                                   ctypes.c_int, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                   ctypes.c_int, _vp, _vp, _sz, _vp, ctypes.c_int, _vp]),
+    "dmoe_quantize_blocks_e4m3": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i64, ctypes.c_int, ctypes.c_int, _vp, _i64,
+                                                 _vp, _i64, _vp]),
+    "dmoe_grouped_matmul_fp8_blocks": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, ctypes.c_int, ctypes.c_int,
+                                                      ctypes.c_int, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                      ctypes.c_int, _vp, _i64, ctypes.c_int, _vp, _vp]),
+    "dmoe_grouped_mlp_fp8_blocks_workspace_size": (_sz, [ctypes.c_int, ctypes.c_int]),
+    "dmoe_grouped_gated_mlp_fp8_blocks": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                         ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp,
+                                                         ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                         ctypes.c_int, _vp, _vp, _sz, _vp, _vp]),
+    "dmoe_balance_loss_workspace_size": (_sz, []),
+    "dmoe_balance_loss": (ctypes.c_int, [_vp, ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                         ctypes.c_int, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "dmoe_balance_loss_backward": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                  ctypes.c_int, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp]),
     "dmoe_router_logits": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp,
                                           _vp]),
     "dmoe_grouped_gated_mlp": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
@@ -199,6 +215,26 @@ def _require_cuda(*ts: Optional[torch.Tensor]) -> torch.device:
             raise DMoEError("dmoe kernels take contiguous tensors")
         dev = t.device if dev is None else dev
     return dev
+
+
+def _one_device(*ts: Optional[torch.Tensor]) -> torch.device:
+    """The one CUDA device of these tensors."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise DMoEError("dmoe kernels take CUDA tensors only (no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise DMoEError(f"tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
+def _on(dev: torch.device):
+    """Make `dev` current for a launch (its streams belong to it)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 # ----------------------------------------------------------------------------- scratch
@@ -571,6 +607,267 @@ def grouped_gated_mlp_fp8(Xq: torch.Tensor, x_scale: torch.Tensor, experts: Fp8E
     del keep
     _check(rc, "dmoe_grouped_gated_mlp_fp8")
     tm.done()
+
+
+# ----------------------------------------------------------------------------- blocks of 128
+FP8_BLOCK = 128
+
+
+def _blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
+    """e4m3 codes of x and one fp32 scale for each block of block_rows x 128.
+
+    block_rows 1 (activations): x [..., cols], scale [..., ceil(cols / 128)]; block_rows 128
+    (weights): x [..., rows, cols], scale [..., ceil(rows / 128), ceil(cols / 128)].
+    scale = max(amax / 448, 2^-126), 1 for an all-zero block; codes = e4m3(x / scale), the quotient
+    rounded to fp32 first.  A value that is not finite becomes a NaN code and leaves the scale of
+    its block alone."""
+    dev = _require_cuda(x)
+    if block_rows not in (1, FP8_BLOCK):
+        raise DMoEError(f"block_rows={block_rows}: 1 or {FP8_BLOCK}")
+    if x.dim() < (1 if block_rows == 1 else 2) or x.shape[-1] == 0 or x.shape[-1] % 16:
+        raise DMoEError("x must be [..., cols] ([..., rows, cols] for 128 x 128 blocks) with cols a multiple of 16")
+    cols = x.shape[-1]
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    if block_rows == 1:
+        batch, rows = 1, x.numel() // cols
+        scale = torch.empty(*x.shape[:-1], _blocks(cols), dtype=torch.float32, device=dev)
+    else:
+        rows = x.shape[-2]
+        batch = x.numel() // (rows * cols) if rows else 0
+        scale = torch.empty(*x.shape[:-2], _blocks(rows), _blocks(cols), dtype=torch.float32, device=dev)
+    with _on(dev):
+        tm = _Timed("quantize_blocks_e4m3", _stream(dev), dev)
+        rc = lib().dmoe_quantize_blocks_e4m3(x.data_ptr(), dtype_code(x.dtype), batch, rows, cols, block_rows,
+                                             q.data_ptr(), cols, scale.data_ptr(), _blocks(cols), _stream(dev))
+        _check(rc, "dmoe_quantize_blocks_e4m3")
+        tm.done()
+    return q, scale
+
+
+def _check_weight_blocks(q: torch.Tensor, scale: torch.Tensor, what: str) -> None:
+    if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.float32:
+        raise DMoEError(f"{what} must be float8_e4m3fn with fp32 scales")
+    if q.dim() != 3 or scale.shape != (q.shape[0], _blocks(q.shape[1]), _blocks(q.shape[2])):
+        raise DMoEError(f"{what} must be [E, N, K] with scales [E, ceil(N / 128), ceil(K / 128)]")
+    if not (q.is_contiguous() and scale.is_contiguous()):
+        raise DMoEError("dmoe kernels take contiguous weights")
+
+
+def _check_row_blocks(xq: torch.Tensor, x_scale: torch.Tensor, K: int) -> Tuple[int, int]:
+    """Row strides (bytes, floats) of 2-D codes and scales of K columns; rows may be strided."""
+    if xq.dtype != torch.float8_e4m3fn or x_scale.dtype != torch.float32:
+        raise DMoEError("xq must be float8_e4m3fn with fp32 scales")
+    if xq.dim() != 2 or xq.shape[1] != K or x_scale.shape != (xq.shape[0], _blocks(K)):
+        raise DMoEError(f"xq must be [rows, {K}] with scales [rows, {_blocks(K)}]")
+    if (K > 1 and xq.stride(1) != 1) or (_blocks(K) > 1 and x_scale.stride(1) != 1):
+        raise DMoEError("the columns of xq and of its scales must be contiguous")
+    if xq.shape[0] < 2:
+        return K, _blocks(K)
+    return xq.stride(0), x_scale.stride(0)
+
+
+def _segments(seg_expert, seg_end, dev: torch.device):
+    """(expert pointer, end pointer, count, on device, what to keep alive) of a segment table."""
+    if isinstance(seg_expert, torch.Tensor) or isinstance(seg_end, torch.Tensor):
+        if not (isinstance(seg_expert, torch.Tensor) and isinstance(seg_end, torch.Tensor)):
+            raise DMoEError("a segment table is two int32 CUDA tensors or two sequences of numbers")
+        if seg_expert.dtype != torch.int32 or seg_end.dtype != torch.int32 or seg_expert.dim() != 1 \
+                or seg_expert.shape != seg_end.shape or not (seg_expert.is_contiguous() and seg_end.is_contiguous()):
+            raise DMoEError("a segment table on the device is two contiguous int32 tensors of one length")
+        if seg_expert.device != dev or seg_end.device != dev:
+            raise DMoEError(f"the segment table must be on {dev}")
+        return seg_expert.data_ptr(), seg_end.data_ptr(), seg_expert.numel(), 1, None
+    if len(seg_expert) != len(seg_end):
+        raise DMoEError("seg_expert and seg_end differ in length")
+    a1, a2 = _i32_array(seg_expert), _i32_array(seg_end)
+    return ctypes.addressof(a1), ctypes.addressof(a2), len(seg_expert), 0, (a1, a2)
+
+
+def grouped_matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
+                              seg_expert, seg_end, out: Optional[torch.Tensor] = None, *,
+                              out_dtype: Optional[torch.dtype] = None, rows_hint: int = 0) -> torch.Tensor:
+    """Rows of 8-bit activations times the transposed 8-bit weight of their segment.
+
+    xq [rows, K] with x_scale [rows, ceil(K / 128)] (:func:`quantize_blocks_e4m3`; rows may be
+    strided), w_q [E, N, K] with w_scale [E, ceil(N / 128), ceil(K / 128)]; segment i is rows
+    [seg_end[i-1], seg_end[i]) and uses weight seg_expert[i] (sequences of numbers, or int32 CUDA
+    tensors).  Returns `out` [rows, N] (rows may be strided), else a new tensor of out_dtype (bf16,
+    f16 or f32; bf16 if not said); rows outside the segments are not written.  rows_hint: rows
+    expected per segment where that is not rows / segments (a capacity-sized buffer); it only picks
+    the tile shape."""
+    dev = _one_device(xq, x_scale, w_q, w_scale, out)
+    _check_weight_blocks(w_q, w_scale, "w_q")
+    E, Nn, K = w_q.shape
+    x_ld, xs_ld = _check_row_blocks(xq, x_scale, K)
+    m = xq.shape[0]
+    if out is None:
+        out = torch.empty(m, Nn, dtype=out_dtype or torch.bfloat16, device=dev)
+    elif out.dim() != 2 or out.shape != (m, Nn) or (Nn > 1 and out.stride(1) != 1) or \
+            (out_dtype is not None and out.dtype != out_dtype):
+        raise DMoEError(f"out must be [{m}, {Nn}] with contiguous columns, in out_dtype where that is given")
+    y_ld = out.stride(0) if m > 1 else Nn
+    se, sn, n_seg, on_dev, keep = _segments(seg_expert, seg_end, dev)
+    with _on(dev):
+        tm = _Timed("grouped_matmul_fp8_blocks", _stream(dev), dev)
+        rc = lib().dmoe_grouped_matmul_fp8_blocks(xq.data_ptr(), x_ld, x_scale.data_ptr(), xs_ld, w_q.data_ptr(),
+                                                  w_scale.data_ptr(), E, Nn, K, se, sn, n_seg, on_dev, m,
+                                                  int(rows_hint), out.data_ptr(), y_ld, dtype_code(out.dtype),
+                                                  scratch.status(dev).data_ptr(), _stream(dev))
+        del keep
+        _check(rc, "dmoe_grouped_matmul_fp8_blocks")
+        tm.done()
+    return out
+
+
+def matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
+                      out: Optional[torch.Tensor] = None, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """xq [rows, K] times the transpose of w_q [N, K], both e4m3 with fp32 scales for each 1 x 128
+    and 128 x 128 block: :func:`grouped_matmul_fp8_blocks` with one segment."""
+    if w_q.dim() != 2 or w_scale.dim() != 2:
+        raise DMoEError("w_q must be [N, K] with scales [ceil(N / 128), ceil(K / 128)]")
+    return grouped_matmul_fp8_blocks(xq, x_scale, w_q.unsqueeze(0), w_scale.unsqueeze(0), (0,), (xq.shape[0],), out,
+                                     out_dtype=out_dtype)
+
+
+class Fp8BlockExperts:
+    """An expert stack whose three projections are e4m3 with one fp32 scale for each 128 x 128
+    block: quantised here from 16- or 32-bit stacks, or taken as a checkpoint holds them
+    (:meth:`from_quantized`)."""
+
+    def __init__(self, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> None:
+        self._set(*quantize_blocks_e4m3(w_gate.contiguous(), FP8_BLOCK),
+                  *quantize_blocks_e4m3(w_up.contiguous(), FP8_BLOCK),
+                  *quantize_blocks_e4m3(w_down.contiguous(), FP8_BLOCK))
+
+    @classmethod
+    def from_quantized(cls, wg_q: torch.Tensor, wg_scale: torch.Tensor, wu_q: torch.Tensor, wu_scale: torch.Tensor,
+                       wd_q: torch.Tensor, wd_scale: torch.Tensor) -> "Fp8BlockExperts":
+        """Codes [E, I, d] (gate, up) and [E, d, I] (down) with their scales."""
+        self = cls.__new__(cls)
+        self._set(wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale)
+        return self
+
+    def _set(self, wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale) -> None:
+        self.device = _one_device(wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale)
+        _check_weight_blocks(wg_q, wg_scale, "gate")
+        _check_weight_blocks(wu_q, wu_scale, "up")
+        _check_weight_blocks(wd_q, wd_scale, "down")
+        E, I, d = wg_q.shape
+        if wu_q.shape != (E, I, d) or wd_q.shape != (E, d, I):
+            raise DMoEError("expert stacks must be gate/up [E, I, d] and down [E, d, I]")
+        if d % 16 or I % 16:
+            raise DMoEError(f"8-bit experts need d % 16 == 0 and I % 16 == 0 (d={d}, I={I})")
+        self.wg_q, self.wg_scale, self.wu_q, self.wu_scale = wg_q, wg_scale, wu_q, wu_scale
+        self.wd_q, self.wd_scale = wd_q, wd_scale
+
+    @property
+    def shape(self):
+        return self.wg_q.shape
+
+
+def grouped_gated_mlp_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, experts: Fp8BlockExperts, seg_expert,
+                                 seg_end, act: int, Y: Optional[torch.Tensor] = None, *,
+                                 rows_hint: int = 0) -> torch.Tensor:
+    """Grouped expert MLP on e4m3 operands with block scales: h = act(x Wg^T) * (x Wu^T) quantised
+    1 x 128 in the epilogue, Y = h Wd^T in bf16.  xq [rows, d] with x_scale [rows, ceil(d / 128)]
+    (rows may be strided); segments and rows_hint as :func:`grouped_matmul_fp8_blocks`; rows outside
+    the segments are not written.  Returns Y [rows, d] (a new tensor if not given)."""
+    dev = _one_device(xq, x_scale, experts.wg_q, Y)
+    E, I, d = experts.wg_q.shape
+    x_ld, xs_ld = _check_row_blocks(xq, x_scale, d)
+    m = xq.shape[0]
+    if Y is None:
+        Y = torch.empty(m, d, dtype=torch.bfloat16, device=dev)
+    elif Y.dtype != torch.bfloat16 or Y.shape != (m, d) or not Y.is_contiguous():
+        raise DMoEError(f"Y must be a contiguous bf16 [{m}, {d}] tensor")
+    ws = torch.empty(lib().dmoe_grouped_mlp_fp8_blocks_workspace_size(m, I), dtype=torch.uint8, device=dev)
+    se, sn, n_seg, on_dev, keep = _segments(seg_expert, seg_end, dev)
+    with _on(dev):
+        tm = _Timed("grouped_gated_mlp_fp8_blocks", _stream(dev), dev)
+        rc = lib().dmoe_grouped_gated_mlp_fp8_blocks(
+            xq.data_ptr(), x_ld, x_scale.data_ptr(), xs_ld, experts.wg_q.data_ptr(), experts.wg_scale.data_ptr(),
+            experts.wu_q.data_ptr(), experts.wu_scale.data_ptr(), experts.wd_q.data_ptr(), experts.wd_scale.data_ptr(),
+            E, d, I, se, sn, n_seg, on_dev, m, int(rows_hint), int(act), Y.data_ptr(), ws.data_ptr(), ws.numel(),
+            scratch.status(dev).data_ptr(), _stream(dev))
+        del keep
+        _check(rc, "dmoe_grouped_gated_mlp_fp8_blocks")
+        tm.done()
+    return Y
+
+
+# ----------------------------------------------------------------------------- balance loss
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, idx, mode, seq_end, mask):
+        dev = logits.device
+        T, E = logits.shape
+        k = idx.shape[1]
+        S = 1 if seq_end is None else seq_end.numel()
+        counts = torch.empty(S * (E + 1) + 1, dtype=torch.int32, device=dev)
+        loss = torch.empty(2, dtype=torch.float32, device=dev)
+        ws = torch.empty(lib().dmoe_balance_loss_workspace_size(), dtype=torch.uint8, device=dev)
+        with _on(dev):
+            tm = _Timed("balance_loss", _stream(dev), dev)
+            rc = lib().dmoe_balance_loss(logits.data_ptr(), dtype_code(logits.dtype), idx.data_ptr(), T, E, k, mode,
+                                         _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), loss.data_ptr(),
+                                         ws.data_ptr(), ws.numel(), scratch.status(dev).data_ptr(), _stream(dev))
+            _check(rc, "dmoe_balance_loss")
+            tm.done()
+        ctx.save_for_backward(logits, seq_end, mask, counts)
+        ctx.args = (T, E, k, mode, S)
+        ctx.set_materialize_grads(False)
+        per_expert = counts[:S * E].view(S, E)
+        ctx.mark_non_differentiable(per_expert)
+        return loss[0], loss[1], per_expert
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_balance, g_z, _counts):
+        if g_balance is None and g_z is None:
+            return None, None, None, None, None
+        logits, seq_end, mask, counts = ctx.saved_tensors
+        T, E, k, mode, S = ctx.args
+        dev = logits.device
+        grad = torch.empty_like(logits)
+        with _on(dev):
+            tm = _Timed("balance_loss_backward", _stream(dev), dev)
+            rc = lib().dmoe_balance_loss_backward(logits.data_ptr(), dtype_code(logits.dtype), T, E, k, mode,
+                                                  _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), _ptr(g_balance),
+                                                  _ptr(g_z), grad.data_ptr(), _stream(dev))
+            _check(rc, "dmoe_balance_loss_backward")
+            tm.done()
+        return grad, None, None, None, None
+
+
+def balance_loss(logits: torch.Tensor, idx: torch.Tensor, *, mode: int = ROUTER_SOFTMAX,
+                 seq_end: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None
+                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Load-balance and z losses of router logits [T, E] and the selected experts idx [T, k] (as
+    :func:`router` returns both), with the selections of each expert: (balance, z, counts [S, E]).
+
+    p = softmax(logits), or sigmoid(logits) over its sum (ROUTER_SIGMOID_GROUP).  seq_end (int32
+    CUDA, ascending token ends) balances each of S sequences for itself; without it the batch is
+    one.  mask [T] (bool) leaves padding tokens out: their logits are not read and their gradients
+    are zero, as for tokens behind the last sequence.
+      balance = mean over non-empty s of sum_e (E counts[s,e] / (k n[s])) (sum_t p[t,e] / n[s])
+      z       = mean over counted tokens of logsumexp(logits)^2
+    Both are differentiable once with respect to the logits; the counts are constants.  As for any
+    autograd function, a backward pass is captured into a CUDA graph only once earlier eager graphs
+    of the same leaf are dropped (torch raises otherwise)."""
+    dev = _one_device(logits, idx, seq_end, mask)
+    _require_cuda(logits, idx, seq_end, mask)
+    if logits.dim() != 2 or idx.dim() != 2 or idx.shape[0] != logits.shape[0] or idx.dtype != torch.int64:
+        raise DMoEError("logits must be [T, E] and the selected experts int64 [T, k]")
+    dtype_code(logits.dtype)
+    if seq_end is not None and (seq_end.dtype != torch.int32 or seq_end.dim() != 1):
+        raise DMoEError("seq_end must be an int32 vector")
+    if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != logits.shape[:1]):
+        raise DMoEError("mask must be bool [T]")
+    return _BalanceLoss.apply(logits, idx, int(mode), seq_end, mask)
 
 
 def set_gemm_sm_reserve(sms: int) -> None:

@@ -1,0 +1,1183 @@
+// Products of e4m3 operands with one fp32 scale for each block of 128, on sm_100a tensor cores.
+//
+//   y[r, n] = sum_b xs[r, b] * ws[e, n / 128, b] * sum_{j in block b} xq[r, j] * wq[e, n, j]
+//
+// x has a scale for each row and 128 columns, the weights [E, N, K] one for each 128 x 128 block
+// (the layout of 8-bit checkpoints); rows come in segments, each with its stack entry e.  The
+// scales differ from one 128-wide step of the reduction to the next, so a tensor-core accumulator
+// may only span one step: each step's MMAs start a fresh TMEM accumulator, and the epilogue warps
+// read it back, multiply by the step's scales and add into fp32 registers while the tensor cores
+// work on the next step in another accumulator.
+//
+// Gated form (the gate/up half of an expert): h = act(x Wg^T) * (x Wu^T) leaves as e4m3 codes
+// with a scale for each row and 128 columns, made from the fp32 accumulators in the epilogue; it
+// is the input of the down product, which is the plain form.
+//
+// Two kernels:
+//   pair      256 rows x 256 weight rows on two SMs (tcgen05 cta_group::2): many rows a segment,
+//             bound by the tensor cores.
+//   few rows  128 weight rows as the MMA's M, 16..128 rows of x as its N, one SM: few rows a
+//             segment, bound by reading the weights; with few tiles the reduction is split over a
+//             cluster and joined through distributed shared memory, in the order of the ranks.
+#include <cuda_fp8.h>
+
+#include "dmoe_common.cuh"
+#include "tcgen05.cuh"
+
+namespace dmoe {
+namespace {
+
+constexpr int kBlk = 128;          // scale block; also bytes of one swizzle row of codes
+constexpr int kMaxSegs = 1024;     // device segment tables
+constexpr int kMaxHostSegs = 256;  // host tables travel in the launch parameters
+constexpr int kEpiWarps = 8;
+constexpr int kBlkThreads = 64 + 32 * kEpiWarps;  // TMA warp, MMA warp, epilogue warps
+
+struct BlkSegs {
+  int n_seg, m_rows, e_stack;
+  const int32_t* dev_expert;
+  const int32_t* dev_end;
+  int32_t expert[kMaxHostSegs];
+  int32_t end[kMaxHostSegs];
+};
+
+struct BlkArgs {
+  const float* xs;  // row scales: [row * xs_ld + kb]
+  int64_t xs_ld;
+  const float* ws0;  // [e][n_blk][k_blk] scales of the (gate) weights, and of the up weights
+  const float* ws1;
+  int n_out;      // valid output columns (weight rows)
+  int K;          // reduction length
+  int n_tiles_n;  // output column tiles
+  int n_blk, k_blk;
+  int act;
+  void* out;  // plain: rows of out_dtype; gated: e4m3 codes
+  int64_t ldo;
+  int out_dtype;
+  float* out_scale;  // gated: [row * os_ld + column block]
+  int64_t os_ld;
+  int32_t* status;
+  // plain only: store row r at scatter_base[code >> 27] + (code & 0x7ffffff) rows with
+  // code = scatter_map[r] (negative: not stored) instead of at row r of `out`; the bases may be
+  // other GPUs' memory.
+  int scatter;
+  const int32_t* scatter_map;
+  char* scatter_base[DMOE_EP_MAX_RANKS];
+};
+
+// Segment table in shared memory: rows [start, end) of stack entry `expert`, first row tile `tile`.
+struct SegTable {
+  int32_t* start;
+  int32_t* end;
+  int32_t* expert;
+  int32_t* tile;  // [n_seg + 1]
+};
+constexpr int kSegTableBytes = 4 * (kMaxSegs + 4) * 4;
+
+__device__ __forceinline__ SegTable seg_table_at(void* p) {
+  int32_t* b = reinterpret_cast<int32_t*>(p);
+  return SegTable{b, b + (kMaxSegs + 4), b + 2 * (kMaxSegs + 4), b + 3 * (kMaxSegs + 4)};
+}
+
+// One warp reads the table, 32 segments at a time: ends are clamped to [previous end, m_rows]
+// (reported in *status where that changes one), entries outside the stack are left out.
+__device__ void read_segments(const BlkSegs& segs, const SegTable& t, int tile_m, int32_t* status) {
+  const int lane = threadIdx.x & 31;
+  const int n = segs.n_seg;
+  int prev = 0, tiles = 0, bad = 0;
+  for (int base = 0; base < n; base += 32) {
+    const int i = base + lane;
+    int en = 0, e = -1;
+    if (i < n) {
+      en = segs.dev_end ? segs.dev_end[i] : segs.end[i];
+      e = segs.dev_expert ? segs.dev_expert[i] : segs.expert[i];
+    }
+    const int given = en;
+    en = min(max(en, 0), segs.m_rows);
+    if (i >= n) en = 0;
+    int top = en;  // running maximum of the ends up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, top, o);
+      if (lane >= o) top = max(top, v);
+    }
+    top = max(top, prev);
+    int first = __shfl_up_sync(0xffffffffu, top, 1);
+    if (lane == 0) first = prev;
+    if (i < n && given != top) bad = 1;
+    int len = i < n ? top - first : 0;
+    if (i < n && (e < 0 || e >= segs.e_stack)) {
+      bad = 1;
+      len = 0;
+      e = 0;
+    }
+    const int mine = (len + tile_m - 1) / tile_m;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (i < n) {
+      t.start[i] = first;
+      t.end[i] = first + len;
+      t.expert[i] = e;
+      t.tile[i] = tiles + sum - mine;
+    }
+    tiles += __shfl_sync(0xffffffffu, sum, 31);
+    prev = __shfl_sync(0xffffffffu, top, 31);
+  }
+  if (lane == 0) t.tile[n] = tiles;
+  if (__any_sync(0xffffffffu, bad) && lane == 0 && blockIdx.x == 0) atomicOr(status, DMOE_DEVERR_BAD_SEGMENT);
+}
+
+struct BlkTile {
+  int row0, row_end, expert, nt;
+};
+
+// Tiles go segment by segment, row tiles fastest: those in flight together share one expert's
+// weight rows, which come from memory once and then from L2.
+__device__ __forceinline__ BlkTile blk_tile(int tile, int n_tiles_n, int n_seg, int tile_m, const SegTable& t) {
+  int lo = 0, hi = n_seg - 1;  // last segment whose first tile is <= tile (skips empty segments)
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((int64_t)t.tile[mid] * n_tiles_n <= tile) lo = mid; else hi = mid - 1;
+  }
+  const int m_tiles = t.tile[lo + 1] - t.tile[lo];
+  const int local = tile - t.tile[lo] * n_tiles_n;
+  const int nt = local / m_tiles;
+  return BlkTile{t.start[lo] + (local - nt * m_tiles) * tile_m, t.end[lo], t.expert[lo], nt};
+}
+
+// acc += v * s on two lanes of packed fp32.
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t v0, uint32_t v1, uint64_t s2) {
+  asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(acc) : "r"(v0), "r"(v1), "l"(s2));
+}
+__device__ __forceinline__ uint64_t pack_f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f2(uint64_t v) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+
+// |v|, 0 for infinities and NaN, as an unsigned number (non-negative floats order as their bits).
+__device__ __forceinline__ uint32_t finite_abs_bits(float v) {
+  const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
+}
+
+// Scale of a block with this largest finite magnitude.
+__device__ __forceinline__ float block_scale(float amax) {
+  return amax > 0.f ? fmaxf(__fdiv_rn(amax, 448.f), 1.17549435e-38f) : 1.f;
+}
+
+// Four codes of h * inv; infinities become NaN codes (the conversion saturates them otherwise).
+__device__ __forceinline__ uint32_t codes4(const float* h, float inv) {
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = fabsf(h[i]) <= 3.402823466e38f ? h[i] * inv : __int_as_float(0x7fffffff);
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
+  return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+// Where row `row` of a plain product goes (nullptr: not stored).
+__device__ __forceinline__ char* blk_out_row(const BlkArgs& a, int row, int esz) {
+  if (!a.scatter) return reinterpret_cast<char*>(a.out) + (int64_t)row * a.ldo * esz;
+  const int32_t code = a.scatter_map[row];
+  if (code < 0) return nullptr;
+  char* base = a.scatter_base[(uint32_t)code >> 27];
+  return base == nullptr ? nullptr : base + (int64_t)(code & 0x7ffffff) * a.ldo * esz;
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]);
+template <>
+__device__ __forceinline__ void tmem_ld<32>(uint32_t taddr, uint32_t (&r)[32]) {
+  tmem_ld32(taddr, r);
+}
+template <>
+__device__ __forceinline__ void tmem_ld<16>(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : DMOE_R8(0), DMOE_R8(8)
+      : "r"(taddr)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void tmem_ld<8>(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : DMOE_R8(0)
+      : "r"(taddr)
+      : "memory");
+}
+
+// kind::f8f6f4, D fp32, A and B e4m3 (format 0), both K-major.
+__host__ __device__ constexpr uint32_t blk_idesc(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// mbar_wait without a call: the sums held in registers would be spilled around one.
+__device__ __forceinline__ bool wait_in_line(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
+                                             int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return false;
+    if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+      *abort_flag = 1;
+      atomicOr(status, code);
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void wait_or_report(uint64_t* bar, uint32_t parity, int32_t* status) {
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+      atomicOr(status, DMOE_DEVERR_TIMEOUT_TEARDOWN);
+      break;
+    }
+  }
+}
+
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// ------------------------------------------------------------------------------- pair kernel
+// A CTA pair computes 256 rows x 256 weight rows (gated: 128 gate and 128 up rows).  Each CTA
+// loads its 128 rows of x and its 128 weight rows (gated: CTA 0 the gate rows, CTA 1 the up rows);
+// its TMEM holds its 128 rows of x by all 256 columns, twice.  Eight epilogue warps: warp pairs
+// share a lane quadrant, each takes half of the columns (gated: 64 gate and the matching 64 up
+// columns), 128 fp32 sums a thread.  The sums need more registers than 65,536 / 384 threads: the
+// first warpgroup (TMA, MMA, segment table, one idle warp) hands its own to the other two.
+constexpr int kPM = 256, kPN = 256;
+constexpr int kPThreads = 128 + 32 * kEpiWarps;
+constexpr int kPRegsIssue = 56, kPRegsSums = 224;  // 128 * 56 + 256 * 224 = 384 * 168, the registers at launch
+constexpr int kPStages = 6;
+constexpr int kPOpBytes = 128 * kBlk;
+constexpr int kPStageBytes = 2 * kPOpBytes;
+constexpr int kPBarBytes = 256;
+constexpr int kPXchBytes = 2 * 2 * 128 * 4;
+constexpr int kPSmemBytes = 1024 + kPStages * kPStageBytes + kPBarBytes + kPXchBytes + kSegTableBytes;
+
+template <bool GATED>
+__global__ void __launch_bounds__(kPThreads, 1)
+    blk_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w0,
+                    const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ BlkSegs segs,
+                    const __grid_constant__ BlkArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPStages * kPStageBytes);
+  uint64_t* empty = full + kPStages;
+  uint64_t* accf = empty + kPStages;
+  uint64_t* acce = accf + 2;
+  uint64_t* fin = acce + 2;
+  uint64_t* bye = fin + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bye + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* xch = reinterpret_cast<uint32_t*>(smem + kPStages * kPStageBytes + kPBarBytes);
+  const SegTable tab = seg_table_at(smem + kPStages * kPStageBytes + kPBarBytes + kPXchBytes);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1;
+  const int n_pairs = gridDim.x >> 1;
+
+  if (warp == 2) read_segments(segs, tab, kPM, args.status);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&accf[a], 1);
+      mbar_init(&acce[a], 2 * kEpiWarps);
+    }
+    mbar_init(fin, 1);
+    mbar_init(bye, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 2 * kPN);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before any remote arrive or TMA signal
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total = tab.tile[segs.n_seg] * args.n_tiles_n;
+  const int nk = args.k_blk;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsIssue));
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      const uint32_t full_leader0 = map_to_cta(smem_u32(&full[0]), 0);
+      int stage = 0;
+      uint32_t ph = 0, armed = 0, armed_ph = 0;
+      bool ok = true;
+      for (int tile = pair; tile < total && ok; tile += n_pairs) {
+        const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, kPM, tab);
+        const int xrow = ti.row0 + (int)rank * 128;
+        const int wrow = GATED ? ti.nt * 128 : ti.nt * kPN + (int)rank * 128;
+        const CUtensorMap* tw = (GATED && rank == 1) ? &tm_w1 : &tm_w0;
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_wait(&empty[stage], ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sx = smem + stage * kPStageBytes;
+          const uint32_t fbar = full_leader0 + (uint32_t)(stage * sizeof(uint64_t));
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * kPStageBytes);
+          tma_load_2d_pair(sx, &tm_x, fbar, kb * kBlk, xrow);
+          tma_load_3d_pair(sx + kPOpBytes, tw, fbar, kb * kBlk, wrow, ti.expert);
+          armed |= 1u << stage;
+          armed_ph = (armed_ph & ~(1u << stage)) | (ph << stage);
+          if (++stage == kPStages) {
+            stage = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // The leader's full barriers count both CTAs' bytes: wait for every phase it armed.
+      if (leader)
+        for (int s = 0; s < kPStages; ++s)
+          if (armed >> s & 1u) wait_or_report(&full[s], armed_ph >> s & 1u, args.status);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (leader CTA)
+    if (leader && lane == 0) {
+      constexpr uint32_t idesc = blk_idesc(kPM, kPN);
+      int stage = 0, acc = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int tile = pair; tile < total && ok; tile += n_pairs) {
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_wait(&full[stage], ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA) ||
+              !mbar_wait(&acce[acc], acc_ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t xd = sdesc_sw128(smem_u32(smem + stage * kPStageBytes));
+          const uint64_t wd = sdesc_sw128(smem_u32(smem + stage * kPStageBytes + kPOpBytes));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // 32 codes of K per MMA; the first starts a fresh sum
+            umma_f16_pair<DMOE_E4M3>(tmem_base + (uint32_t)(acc * kPN), xd + 2 * k, wd + 2 * k, idesc, k != 0);
+          umma_commit_both(&empty[stage]);
+          umma_commit_both(&accf[acc]);
+          if (++stage == kPStages) {
+            stage = 0;
+            ph ^= 1u;
+          }
+          acc ^= 1;
+          if (acc == 0) acc_ph ^= 1u;
+        }
+      }
+      umma_commit_both(fin);
+    }
+    // Every MMA of the pair (issued by the leader) has completed once `fin` fires in this CTA.
+    if (lane == 0) wait_or_report(fin, 0, args.status);
+  }
+  } else {
+    // ------------------------------------------------------------------ epilogue (both CTAs)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPRegsSums));
+    const int q = warp & 3;               // TMEM lane quadrant this warp may access
+    const int half = (warp - 4) >> 2;     // its half of the columns
+    const uint32_t acce_leader0 = map_to_cta(smem_u32(&acce[0]), 0);
+    int acc = 0, flip = 0;
+    uint32_t acc_ph = 0;
+    bool ok = true;
+    for (int tile = pair; tile < total; tile += n_pairs, flip ^= 1) {
+      const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, kPM, tab);
+      const int row = ti.row0 + (int)rank * 128 + q * 32 + lane;
+      const bool valid = row < ti.row_end;
+      const float* xs = args.xs + (int64_t)(valid ? row : ti.row0) * args.xs_ld;
+      // Weight scales: gated, of this column block of both stacks; plain, of this half's block
+      // (the last tile's second half may lie past the last block: its sums are never stored).
+      const int nb = GATED ? ti.nt : min(ti.nt * 2 + half, args.n_blk - 1);
+      const int64_t wat = ((int64_t)ti.expert * args.n_blk + nb) * args.k_blk;
+      uint64_t sum[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) sum[i] = 0;
+      float x_next = __ldg(xs), w0_next = __ldg(args.ws0 + wat), w1_next = GATED ? __ldg(args.ws1 + wat) : 0.f;
+      for (int kb = 0; kb < nk && ok; ++kb) {
+        const float s0 = x_next * w0_next, s1 = GATED ? x_next * w1_next : s0;
+        if (kb + 1 < nk) {
+          x_next = __ldg(xs + kb + 1);
+          w0_next = __ldg(args.ws0 + wat + kb + 1);
+          if constexpr (GATED) w1_next = __ldg(args.ws1 + wat + kb + 1);
+        }
+        ok = wait_in_line(&accf[acc], acc_ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_EPILOGUE);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kPN);
+        const uint64_t s0p = pack_f2(s0, s0), s1p = pack_f2(s1, s1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int col = GATED ? (j < 2 ? half * 64 + j * 32 : 128 + half * 64 + (j - 2) * 32) : half * 128 + j * 32;
+          uint32_t v[32];
+          tmem_ld32(tbase + col, v);
+          if (j == 3) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acce_leader0 + (uint32_t)(acc * sizeof(uint64_t)));
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) fma2(sum[j * 16 + i], v[2 * i], v[2 * i + 1], j < 2 ? s0p : s1p);
+        }
+        acc ^= 1;
+        if (acc == 0) acc_ph ^= 1u;
+      }
+      // After a wait that ran out nothing is stored, but the warps that share a quadrant still meet.
+      if constexpr (GATED) {
+        float h[64];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 g = unpack_f2(sum[i]), u = unpack_f2(sum[32 + i]);
+          h[2 * i] = act_fn(g.x, args.act) * u.x;
+          h[2 * i + 1] = act_fn(g.y, args.act) * u.y;
+          top = max(top, max(finite_abs_bits(h[2 * i]), finite_abs_bits(h[2 * i + 1])));
+        }
+        // The row's other 64 columns are in the warp that shares this quadrant.
+        uint32_t* mine = xch + (flip * 2 + half) * 128 + q * 32 + lane;
+        uint32_t* other = xch + (flip * 2 + (half ^ 1)) * 128 + q * 32 + lane;
+        *mine = top;
+        named_sync(1 + q, 64);
+        top = max(top, *other);
+        const float s = block_scale(__uint_as_float(top));
+        const float inv = 1.f / s;
+        if (valid && ok) {
+          if (half == 0) args.out_scale[(int64_t)row * args.os_ld + ti.nt] = s;
+          const int col0 = ti.nt * 128 + half * 64;
+          uint8_t* dst = reinterpret_cast<uint8_t*>(args.out) + (int64_t)row * args.ldo + col0;
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (col0 + v * 16 < args.n_out)
+              *reinterpret_cast<uint4*>(dst + v * 16) = make_uint4(codes4(h + v * 16, inv), codes4(h + v * 16 + 4, inv),
+                                                                   codes4(h + v * 16 + 8, inv), codes4(h + v * 16 + 12, inv));
+        }
+      } else {
+        const int esz = args.out_dtype == DMOE_F32 ? 4 : 2;
+        const int col0 = ti.nt * kPN + half * 128;
+        char* dst = valid && ok ? blk_out_row(args, row, esz) : nullptr;
+        if (dst != nullptr) {
+          dst += (int64_t)col0 * esz;
+          if (args.out_dtype == DMOE_F32) {
+#pragma unroll
+            for (int v = 0; v < 32; ++v) {
+              const float2 a = unpack_f2(sum[2 * v]), b = unpack_f2(sum[2 * v + 1]);
+              if (col0 + v * 4 < args.n_out) *reinterpret_cast<float4*>(dst + v * 16) = make_float4(a.x, a.y, b.x, b.y);
+            }
+          } else {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 a = unpack_f2(sum[4 * v + i]);
+                pk[i] = args.out_dtype == DMOE_BF16 ? pack2<DMOE_BF16>(a.x, a.y) : pack2<DMOE_F16>(a.x, a.y);
+              }
+              if (col0 + v * 8 < args.n_out) *reinterpret_cast<uint4*>(dst + v * 16) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  if (args.scatter) __threadfence_system();  // scattered rows may live in other GPUs' memory
+  tc_fence_before();
+  __syncthreads();
+  // Exit handshake: tell the peer this CTA is done with the pair's shared state, then wait
+  // (bounded) until the peer says the same.
+  if (threadIdx.x == 0) {
+    mbar_arrive_cluster(map_to_cta(smem_u32(bye), rank ^ 1u));
+    wait_or_report(bye, 0, args.status);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * kPN);
+  }
+}
+
+// --------------------------------------------------------------------------- few-rows kernel
+// D[weight row, row of x]: M = 128 weight rows (gated: two MMAs, gate and up rows), N = NT rows
+// of x.  Eight epilogue warps: a thread holds one weight row and half of the tile's rows of x.
+// The scales differ by row of x here, that is by column of D: each warp multiplies its rows'
+// scales by the step's weight scale once (a lane a row) and reads them back from shared memory.
+template <bool GATED, int NT, bool SPLIT>
+struct Few {
+  static constexpr int kA = GATED ? 2 : 1;
+  static constexpr int kHalf = NT / 2;
+  static constexpr int kStageBytes = kA * 128 * kBlk + NT * kBlk;
+  static constexpr int kAccs = 512 / (kA * NT) >= 4 ? 4 : 2;  // TMEM accumulators (of kA x NT columns)
+  static constexpr int kTmemCols = kAccs * kA * NT < 32 ? 32 : kAccs * kA * NT;
+  static constexpr int kBarBytes = 512;
+  static constexpr int kScaleBytes = kEpiWarps * 2 * kA * kHalf * 4;
+  static constexpr int kTopBytes = 2 * 2 * 4 * kHalf * 4;
+  static constexpr int kRedBytes = SPLIT ? kA * NT * 128 * 4 : 0;
+  static constexpr int kFixed = 1024 + kBarBytes + kScaleBytes + kTopBytes + kRedBytes + kSegTableBytes;
+  static constexpr int kFit = (227 * 1024 - kFixed) / kStageBytes;
+  static constexpr int kStages = kFit > 12 ? 12 : kFit;
+  static constexpr int kSmemBytes = kFixed + kStages * kStageBytes;
+  static_assert(kStages >= 3 && kTmemCols <= 512, "few-rows tile does not fit");
+};
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <bool GATED, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kBlkThreads, 1)
+    blk_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w0,
+                   const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ BlkSegs segs,
+                   const __grid_constant__ BlkArgs args, int ranks) {
+  using F = Few<GATED, NT, SPLIT>;
+  constexpr int S = F::kStages, NA = F::kA, HN = F::kHalf, ACCS = F::kAccs;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* after = smem + S * F::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(after);
+  uint64_t* empty = full + S;
+  uint64_t* accf = empty + S;
+  uint64_t* acce = accf + ACCS;
+  uint64_t* fin = acce + ACCS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  after += F::kBarBytes;
+  float* red = reinterpret_cast<float*>(after);  // SPLIT: [NA][NT][128] partial sums
+  after += F::kRedBytes;
+  float* scales = reinterpret_cast<float*>(after);  // [warp][2][NA][HN]
+  after += F::kScaleBytes;
+  uint32_t* tops = reinterpret_cast<uint32_t*>(after);  // [2][half][HN][4 quadrants]
+  after += F::kTopBytes;
+  const SegTable tab = seg_table_at(after);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = SPLIT ? (int)cluster_ctarank() : 0;
+  const int group = SPLIT ? (int)blockIdx.x / ranks : (int)blockIdx.x;
+  const int n_groups = SPLIT ? (int)gridDim.x / ranks : (int)gridDim.x;
+
+  if (warp == 2) read_segments(segs, tab, NT, args.status);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < ACCS; ++a) {
+      mbar_init(&accf[a], 1);
+      mbar_init(&acce[a], kEpiWarps);
+    }
+    mbar_init(fin, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, F::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total = tab.tile[segs.n_seg] * args.n_tiles_n;
+  const int kb0 = SPLIT ? (int)((int64_t)args.k_blk * rank / ranks) : 0;
+  const int kb1 = SPLIT ? (int)((int64_t)args.k_blk * (rank + 1) / ranks) : args.k_blk;
+
+  // Every role walks the same tiles; with a split reduction all warps of the cluster's CTAs meet
+  // twice a tile (partial sums written; partial sums read).
+  int stage = 0, acc = 0, flip = 0;
+  uint32_t ph = 0, acc_ph = 0, armed = 0, armed_ph = 0;
+  bool ok = true;
+  const int q = warp & 3, half = (warp - 2) >> 2;
+  for (int tile = group; tile < total; tile += n_groups) {
+    const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, NT, tab);
+    uint64_t sum[NA][HN / 2];  // epilogue: pairs of rows of x
+    if (warp == 0) {
+      // ---------------------------------------------------------------- TMA producer
+      if (lane == 0 && ok) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&empty[stage], ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sw = smem + stage * F::kStageBytes;
+          mbar_arrive_expect_tx(&full[stage], F::kStageBytes);
+          tma_load_3d(sw, &tm_w0, &full[stage], kb * kBlk, ti.nt * 128, ti.expert);
+          if constexpr (GATED) tma_load_3d(sw + 128 * kBlk, &tm_w1, &full[stage], kb * kBlk, ti.nt * 128, ti.expert);
+          tma_load_2d(sw + NA * 128 * kBlk, &tm_x, &full[stage], kb * kBlk, ti.row0);
+          armed |= 1u << stage;
+          armed_ph = (armed_ph & ~(1u << stage)) | (ph << stage);
+          if (++stage == S) {
+            stage = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer
+      if (lane == 0 && ok) {
+        constexpr uint32_t idesc = blk_idesc(128, NT);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&full[stage], ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA) ||
+              !mbar_wait(&acce[acc], acc_ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sw = smem_u32(smem + stage * F::kStageBytes);
+          const uint64_t xd = sdesc_sw128(sw + NA * 128 * kBlk);
+#pragma unroll
+          for (int a = 0; a < NA; ++a) {
+            const uint64_t wd = sdesc_sw128(sw + a * 128 * kBlk);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // 32 codes of K per MMA; the first starts a fresh sum
+              umma_f16<DMOE_E4M3>(tmem_base + (uint32_t)((acc * NA + a) * NT), wd + 2 * k, xd + 2 * k, idesc, k != 0);
+          }
+          umma_commit(&empty[stage]);
+          umma_commit(&accf[acc]);
+          if (++stage == S) {
+            stage = 0;
+            ph ^= 1u;
+          }
+          if (++acc == ACCS) {
+            acc = 0;
+            acc_ph ^= 1u;
+          }
+        }
+      }
+    } else {
+      // ---------------------------------------------------------------- epilogue: scaled sums
+      constexpr int PL = (HN + 31) / 32;  // rows of x whose scales a lane fetches
+      float* sc = scales + (warp - 2) * 2 * NA * HN;
+      const int64_t wat = ((int64_t)ti.expert * args.n_blk + ti.nt) * args.k_blk;
+      const float* xs[PL];
+#pragma unroll
+      for (int p = 0; p < PL; ++p) {
+        const int row = ti.row0 + half * HN + p * 32 + lane;
+        xs[p] = args.xs + (int64_t)(row < ti.row_end ? row : ti.row0) * args.xs_ld;
+      }
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int i = 0; i < HN / 2; ++i) sum[a][i] = 0;
+      float x_next[PL], w0_next = 0.f, w1_next = 0.f;
+#pragma unroll
+      for (int p = 0; p < PL; ++p) x_next[p] = kb0 < kb1 ? __ldg(xs[p] + kb0) : 0.f;
+      if (kb0 < kb1) {
+        w0_next = __ldg(args.ws0 + wat + kb0);
+        if constexpr (GATED) w1_next = __ldg(args.ws1 + wat + kb0);
+      }
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        float* now = sc + (kb & 1) * NA * HN;
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+          if (p * 32 + lane < HN) {
+            now[p * 32 + lane] = x_next[p] * w0_next;
+            if constexpr (GATED) now[HN + p * 32 + lane] = x_next[p] * w1_next;
+          }
+        }
+        if (kb + 1 < kb1) {
+#pragma unroll
+          for (int p = 0; p < PL; ++p) x_next[p] = __ldg(xs[p] + kb + 1);
+          w0_next = __ldg(args.ws0 + wat + kb + 1);
+          if constexpr (GATED) w1_next = __ldg(args.ws1 + wat + kb + 1);
+        }
+        ok = wait_in_line(&accf[acc], acc_ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_EPILOGUE);
+        ok = __all_sync(0xffffffffu, ok);  // also orders the scales' stores before their loads
+        if (!ok) break;
+        __syncwarp();
+        tc_fence_after();
+        constexpr int C = HN < 32 ? HN : 32;
+#pragma unroll
+        for (int a = 0; a < NA; ++a) {
+#pragma unroll
+          for (int c = 0; c < HN / C; ++c) {
+            uint32_t v[C];
+            tmem_ld<C>(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((acc * NA + a) * NT + half * HN + c * C), v);
+            if (a == NA - 1 && c == HN / C - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&acce[acc]);
+            }
+            const ulonglong2* s4 = reinterpret_cast<const ulonglong2*>(now + a * HN + c * C);
+#pragma unroll
+            for (int i = 0; i < C / 4; ++i) {
+              const ulonglong2 s = s4[i];
+              fma2(sum[a][c * (C / 2) + 2 * i], v[4 * i], v[4 * i + 1], s.x);
+              fma2(sum[a][c * (C / 2) + 2 * i + 1], v[4 * i + 2], v[4 * i + 3], s.y);
+            }
+          }
+        }
+        if (++acc == ACCS) {
+          acc = 0;
+          acc_ph ^= 1u;
+        }
+      }
+    }
+
+    // ------------------------------------------------------------------ results of the tile
+    const int ch = q * 32 + lane;  // weight row within the tile
+    const int col = ti.nt * 128 + ch;
+    const int esz = args.out_dtype == DMOE_F32 ? 4 : 2;
+    if constexpr (SPLIT) {
+      if (warp >= 2) {
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+#pragma unroll
+          for (int i = 0; i < HN / 2; ++i) {
+            const float2 v = unpack_f2(sum[a][i]);
+            red[(a * NT + half * HN + 2 * i) * 128 + ch] = v.x;
+            red[(a * NT + half * HN + 2 * i + 1) * 128 + ch] = v.y;
+          }
+      }
+      __syncwarp();
+      cluster_sync_all();
+      if (warp >= 2) {
+        // This rank finishes rows rank, rank + ranks, ... of the tile, the two halves in turn.
+        const int rows = min(NT, ti.row_end - ti.row0);
+        const uint32_t red0 = smem_u32(red);
+        for (int t = rank + half * ranks; t < rows; t += 2 * ranks) {
+          float v[NA];
+#pragma unroll
+          for (int a = 0; a < NA; ++a) {
+            v[a] = 0.f;
+            for (int r = 0; r < ranks; ++r)
+              v[a] += ld_cluster(map_to_cta(red0 + (uint32_t)(((a * NT + t) * 128 + ch) * 4), (uint32_t)r));
+          }
+          const int row = ti.row0 + t;
+          if constexpr (GATED) {
+            const float h = act_fn(v[0], args.act) * v[NA - 1];
+            const uint32_t top = __reduce_max_sync(0xffffffffu, finite_abs_bits(h));
+            uint32_t* at = tops + ((flip * 2 + half) * HN) * 4;
+            flip ^= 1;
+            if (lane == 0) at[q] = top;
+            named_sync(1 + half, 128);
+            const float s = block_scale(__uint_as_float(max(max(at[0], at[1]), max(at[2], at[3]))));
+            if (col < args.n_out) {
+              const float inv = 1.f / s;
+              const float c = fabsf(h) <= 3.402823466e38f ? h * inv : __int_as_float(0x7fffffff);
+              reinterpret_cast<uint8_t*>(args.out)[(int64_t)row * args.ldo + col] =
+                  __nv_cvt_float_to_fp8(c, __NV_SATFINITE, __NV_E4M3);
+            }
+            if (ch == 0) args.out_scale[(int64_t)row * args.os_ld + ti.nt] = s;
+          } else {
+            char* dst = blk_out_row(args, row, esz);
+            if (dst != nullptr && col < args.n_out) store_from_float(dst, col, v[0], args.out_dtype);
+          }
+        }
+      }
+      __syncwarp();
+      cluster_sync_all();
+    } else if (warp >= 2) {
+      // After a wait that ran out nothing is stored, but the warps of a half still meet.
+      const int rows = ok ? min(HN, ti.row_end - ti.row0 - half * HN) : 0;
+      const int row0 = ti.row0 + half * HN;
+      if constexpr (GATED) {
+        uint32_t* at = tops + ((flip * 2 + half) * HN) * 4;
+        flip ^= 1;
+        float h[HN];
+#pragma unroll
+        for (int i = 0; i < HN / 2; ++i) {
+          const float2 g = unpack_f2(sum[0][i]), u = unpack_f2(sum[NA - 1][i]);
+          h[2 * i] = act_fn(g.x, args.act) * u.x;
+          h[2 * i + 1] = act_fn(g.y, args.act) * u.y;
+        }
+#pragma unroll
+        for (int t = 0; t < HN; ++t) {
+          const uint32_t top = __reduce_max_sync(0xffffffffu, finite_abs_bits(h[t]));
+          if (lane == 0) at[t * 4 + q] = top;
+        }
+        named_sync(1 + half, 128);
+#pragma unroll
+        for (int t = 0; t < HN; ++t) {
+          if (t < rows) {
+            const uint4 m = *reinterpret_cast<const uint4*>(at + t * 4);
+            const float s = block_scale(__uint_as_float(max(max(m.x, m.y), max(m.z, m.w))));
+            const int row = row0 + t;
+            if (col < args.n_out) {
+              const float inv = 1.f / s;
+              const float c = fabsf(h[t]) <= 3.402823466e38f ? h[t] * inv : __int_as_float(0x7fffffff);
+              reinterpret_cast<uint8_t*>(args.out)[(int64_t)row * args.ldo + col] =
+                  __nv_cvt_float_to_fp8(c, __NV_SATFINITE, __NV_E4M3);
+            }
+            if (ch == 0) args.out_scale[(int64_t)row * args.os_ld + ti.nt] = s;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < HN; ++t) {
+          if (t < rows) {
+            const float2 v = unpack_f2(sum[0][t / 2]);
+            char* dst = blk_out_row(args, row0 + t, esz);
+            if (dst != nullptr && col < args.n_out) store_from_float(dst, col, t & 1 ? v.y : v.x, args.out_dtype);
+          }
+        }
+      }
+    }
+  }
+
+  // Copies in flight land and MMAs complete before the CTA's shared memory and TMEM go.
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < S; ++s)
+      if (armed >> s & 1u) wait_or_report(&full[s], armed_ph >> s & 1u, args.status);
+  } else if (warp == 1 && lane == 0) {
+    umma_commit(fin);
+    wait_or_report(fin, 0, args.status);
+  }
+  if (args.scatter) __threadfence_system();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, F::kTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------------------------- host
+// Row-major e4m3 tensor map, dims innermost first, rows ld bytes apart, 128-byte swizzle.
+int code_map(CUtensorMap* map, const void* base, int rank, uint64_t cols, uint64_t rows, uint64_t stack, uint64_t ld,
+             uint32_t box_rows) {
+  PFN_encodeTiled enc = get_encode_fn();
+  DMOE_REQUIRE(enc != nullptr, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[3] = {cols, rows, stack};
+  const cuuint64_t strides[2] = {ld, ld * rows};
+  const cuuint32_t box[3] = {(cuuint32_t)kBlk, box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank, const_cast<void*>(base), dims, strides,
+                         box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return DMOE_ERR_CUDA;
+  }
+  return DMOE_OK;
+}
+
+// One product: x [m_rows, K] codes against the stack(s) [E, N, K].
+struct Product {
+  const void* x;
+  int64_t x_ld;
+  const void* w0;
+  const void* w1;  // up weights of the gated form, else null
+  int E, N, K;
+  BlkArgs args;
+};
+
+template <bool GATED>
+int launch_pair(const Product& p, const BlkSegs& segs, int m_tiles, cudaStream_t stream) {
+  static PerDeviceOnce once;
+  static int max_clusters[64];
+  int dev = 0;
+  DMOE_CUDA(cudaGetDevice(&dev));
+  DMOE_REQUIRE(dev >= 0 && dev < 64, "block-scaled product: device index %d out of range", dev);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kPThreads);
+  cfg.dynamicSmemBytes = kPSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const int r = once_per_device(once, dev, [&] {
+    DMOE_CUDA(cudaFuncSetAttribute(blk_pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmemBytes));
+    cfg.gridDim = dim3(2 * 74);
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, blk_pair_kernel<GATED>, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = 64;
+    }
+    max_clusters[dev] = n;
+    return DMOE_OK;
+  });
+  if (r) return r;
+  CUtensorMap tx, t0, t1;
+  if (int e = code_map(&tx, p.x, 2, p.K, segs.m_rows, 1, p.x_ld, 128)) return e;
+  if (int e = code_map(&t0, p.w0, 3, p.K, p.N, p.E, p.K, 128)) return e;
+  t1 = t0;
+  if (GATED)
+    if (int e = code_map(&t1, p.w1, 3, p.K, p.N, p.E, p.K, 128)) return e;
+  BlkArgs a = p.args;
+  a.n_tiles_n = GATED ? (p.N + 127) / 128 : (p.N + kPN - 1) / kPN;
+  int pairs = max_clusters[dev] - (gemm_sm_reserve() + 1) / 2;
+  const int64_t tiles = (int64_t)m_tiles * a.n_tiles_n;
+  if (tiles < pairs) pairs = (int)tiles;
+  if (pairs < 1) pairs = 1;
+  cfg.gridDim = dim3(2 * pairs);
+  DMOE_CUDA(cudaLaunchKernelEx(&cfg, blk_pair_kernel<GATED>, tx, t0, t1, segs, a));
+  DMOE_LAUNCH_CHECK();
+  return DMOE_OK;
+}
+
+template <bool GATED, int NT, bool SPLIT>
+int launch_few(const Product& p, const BlkSegs& segs, int m_tiles, int ranks, cudaStream_t stream) {
+  using F = Few<GATED, NT, SPLIT>;
+  static PerDeviceOnce once;
+  int dev = 0;
+  DMOE_CUDA(cudaGetDevice(&dev));
+  const int r = once_per_device(once, dev, [] {
+    DMOE_CUDA(cudaFuncSetAttribute(blk_few_kernel<GATED, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   F::kSmemBytes));
+    return DMOE_OK;
+  });
+  if (r) return r;
+  CUtensorMap tx, t0, t1;
+  if (int e = code_map(&tx, p.x, 2, p.K, segs.m_rows, 1, p.x_ld, NT)) return e;
+  if (int e = code_map(&t0, p.w0, 3, p.K, p.N, p.E, p.K, 128)) return e;
+  t1 = t0;
+  if (GATED)
+    if (int e = code_map(&t1, p.w1, 3, p.K, p.N, p.E, p.K, 128)) return e;
+  BlkArgs a = p.args;
+  a.n_tiles_n = (p.N + 127) / 128;
+  const int64_t tiles = (int64_t)m_tiles * a.n_tiles_n;
+  int groups = gemm_usable_sms() / ranks;
+  if (tiles < groups) groups = (int)tiles;
+  if (groups < 1) groups = 1;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(groups * ranks);
+  cfg.blockDim = dim3(kBlkThreads);
+  cfg.dynamicSmemBytes = F::kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = SPLIT ? 1 : 0;
+  DMOE_CUDA(cudaLaunchKernelEx(&cfg, blk_few_kernel<GATED, NT, SPLIT>, tx, t0, t1, segs, a, ranks));
+  DMOE_LAUNCH_CHECK();
+  return DMOE_OK;
+}
+
+// Rows of x that a segment is expected to have: what the caller says, else the mean over the
+// segments that can have any.
+int expected_rows(const BlkSegs& segs, int hint) {
+  if (hint > 0) return hint;
+  const int used = segs.n_seg < segs.m_rows ? segs.n_seg : segs.m_rows;
+  return used > 0 ? (segs.m_rows + used - 1) / used : 0;
+}
+
+// Row tiles of `tile_m` rows: counted for a host table, for a device table the most that
+// m_rows rows in n_seg segments can make.
+int row_tiles(const BlkSegs& segs, int tile_m) {
+  if (segs.dev_end == nullptr) {
+    int prev = 0, n = 0;
+    for (int i = 0; i < segs.n_seg; ++i) {
+      n += (segs.end[i] - prev + tile_m - 1) / tile_m;
+      prev = segs.end[i];
+    }
+    return n;
+  }
+  const int64_t most = (int64_t)segs.m_rows / tile_m + segs.n_seg;
+  return (int)(most < segs.m_rows ? most : segs.m_rows);
+}
+
+template <bool GATED, int NT>
+int run_few(const Product& p, const BlkSegs& segs, int rows, cudaStream_t stream) {
+  const int m_tiles = row_tiles(segs, NT);
+  if constexpr (NT <= 32) {
+    // Few tiles: split the reduction over a cluster of up to 8 SMs, at least 2 steps each.
+    const int used = segs.n_seg < segs.m_rows ? segs.n_seg : segs.m_rows;
+    const int64_t likely = (int64_t)(segs.dev_end ? used * ((rows + NT - 1) / NT) : m_tiles) * ((p.N + 127) / 128);
+    int ranks = 1;
+    while (ranks < 8 && likely * ranks * 2 <= gemm_usable_sms() && p.args.k_blk >= ranks * 4) ranks *= 2;
+    if (ranks > 1) return launch_few<GATED, NT, true>(p, segs, m_tiles, ranks, stream);
+  }
+  return launch_few<GATED, NT, false>(p, segs, m_tiles, 1, stream);
+}
+
+template <bool GATED>
+int run_product(Product& p, const BlkSegs& segs, int hint, cudaStream_t stream) {
+  p.args.n_out = p.N;
+  p.args.K = p.K;
+  p.args.n_blk = (p.N + kBlk - 1) / kBlk;
+  p.args.k_blk = (p.K + kBlk - 1) / kBlk;
+  const int rows = expected_rows(segs, hint);
+  if (rows > 128) return launch_pair<GATED>(p, segs, row_tiles(segs, kPM), stream);
+  if constexpr (!GATED)
+    if (rows > 64) return run_few<GATED, 128>(p, segs, rows, stream);
+  if (rows > 32) return run_few<GATED, 64>(p, segs, rows, stream);
+  if (rows > 16) return run_few<GATED, 32>(p, segs, rows, stream);
+  return run_few<GATED, 16>(p, segs, rows, stream);
+}
+
+int fill_blk_segs(const char* name, BlkSegs& s, const int32_t* seg_expert, const int32_t* seg_end, int n_seg,
+                  int seg_on_device, int m_rows, int E_stack) {
+  s.n_seg = n_seg;
+  s.m_rows = m_rows;
+  s.e_stack = E_stack;
+  if (seg_on_device) {
+    DMOE_REQUIRE(n_seg <= kMaxSegs, "%s: n_seg=%d > %d", name, n_seg, kMaxSegs);
+    s.dev_expert = seg_expert;
+    s.dev_end = seg_end;
+    return DMOE_OK;
+  }
+  DMOE_REQUIRE(n_seg <= kMaxHostSegs, "%s: n_seg=%d > %d for host segment tables", name, n_seg, kMaxHostSegs);
+  s.dev_expert = s.dev_end = nullptr;
+  int prev = 0;
+  for (int i = 0; i < n_seg; ++i) {
+    DMOE_REQUIRE(seg_end[i] >= prev && seg_end[i] <= m_rows, "%s: segment %d end %d invalid", name, i, seg_end[i]);
+    DMOE_REQUIRE(seg_expert[i] >= 0 && seg_expert[i] < E_stack, "%s: segment %d expert %d", name, i, seg_expert[i]);
+    s.expert[i] = seg_expert[i];
+    s.end[i] = seg_end[i];
+    prev = seg_end[i];
+  }
+  return DMOE_OK;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int64_t blocks_of(int64_t n) { return (n + kBlk - 1) / kBlk; }
+
+// Gate/up product into codes and scales of h in the workspace, then the down product.
+int run_blk_mlp(const void* x, int64_t x_ld, const float* xs, int64_t xs_ld, const void* wg, const float* gs,
+                const void* wu, const float* us, const void* wd, const float* ds, int E, int d, int I,
+                const BlkSegs& segs, int hint, int act, void* Y, const int32_t* scatter_map, char* const* scatter_base,
+                void* workspace, int32_t* status, cudaStream_t stream) {
+  uint8_t* h = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+  float* hs = reinterpret_cast<float*>(h + (((int64_t)segs.m_rows * I + 255) & ~int64_t(255)));
+  Product g{x, x_ld, wg, wu, E, I, d, {}};
+  g.args.xs = xs;
+  g.args.xs_ld = xs_ld;
+  g.args.ws0 = gs;
+  g.args.ws1 = us;
+  g.args.act = act;
+  g.args.out = h;
+  g.args.ldo = I;
+  g.args.out_dtype = DMOE_E4M3;
+  g.args.out_scale = hs;
+  g.args.os_ld = blocks_of(I);
+  g.args.status = status;
+  if (int r = run_product<true>(g, segs, hint, stream)) return r;
+  Product dn{h, I, wd, nullptr, E, d, I, {}};
+  dn.args.xs = hs;
+  dn.args.xs_ld = blocks_of(I);
+  dn.args.ws0 = ds;
+  dn.args.out = Y;
+  dn.args.ldo = d;
+  dn.args.out_dtype = DMOE_BF16;
+  dn.args.status = status;
+  if (scatter_map != nullptr) {
+    dn.args.scatter = 1;
+    dn.args.scatter_map = scatter_map;
+    for (int g2 = 0; g2 < DMOE_EP_MAX_RANKS; ++g2) dn.args.scatter_base[g2] = scatter_base[g2];
+  }
+  return run_product<false>(dn, segs, hint, stream);
+}
+
+}  // namespace
+}  // namespace dmoe
+
+using namespace dmoe;
+
+extern "C" int dmoe_grouped_matmul_fp8_blocks(const void* Xq, int64_t x_ld, const float* x_scale, int64_t xs_ld,
+                                              const void* w_q, const float* w_scale, int E_stack, int N, int K,
+                                              const int32_t* seg_expert, const int32_t* seg_end, int n_seg,
+                                              int seg_on_device, int m_rows, int rows_hint, void* Y, int64_t y_ld,
+                                              int out_dtype, int32_t* dev_status, void* stream) {
+  clear_error();
+  const char* name = "dmoe_grouped_matmul_fp8_blocks";
+  DMOE_REQUIRE(dtype_ok(out_dtype), "%s: output dtype must be f32, f16 or bf16", name);
+  DMOE_REQUIRE(N > 0 && K > 0 && N % 8 == 0 && K % 16 == 0, "%s: N=%d must be a multiple of 8, K=%d of 16", name, N, K);
+  DMOE_REQUIRE(E_stack >= 1 && m_rows >= 0 && n_seg >= 0 && rows_hint >= 0, "%s: bad E_stack/m_rows/n_seg/rows_hint",
+               name);
+  DMOE_REQUIRE(x_ld >= K && x_ld % 16 == 0 && xs_ld >= blocks_of(K), "%s: x_ld=%lld, xs_ld=%lld too small or odd", name,
+               (long long)x_ld, (long long)xs_ld);
+  DMOE_REQUIRE(y_ld >= N && y_ld % 8 == 0, "%s: y_ld=%lld must be >= N and a multiple of 8", name, (long long)y_ld);
+  if (n_seg == 0 || m_rows == 0) return DMOE_OK;
+  DMOE_REQUIRE(Xq && x_scale && w_q && w_scale && Y && dev_status && seg_expert && seg_end, "%s: null pointer", name);
+  DMOE_REQUIRE(aligned16(Xq) && aligned16(w_q) && aligned16(Y), "%s: tensors must be 16-byte aligned", name);
+  DMOE_REQUIRE(aligned4(x_scale) && aligned4(w_scale), "%s: scales must be 4-byte aligned", name);
+  DMOE_REQUIRE(((int64_t)m_rows + n_seg) * blocks_of(N) < INT32_MAX, "%s: too many tiles", name);
+  static thread_local BlkSegs segs;
+  if (int r = fill_blk_segs(name, segs, seg_expert, seg_end, n_seg, seg_on_device, m_rows, E_stack)) return r;
+  Product p{Xq, x_ld, w_q, nullptr, E_stack, N, K, {}};
+  p.args.xs = x_scale;
+  p.args.xs_ld = xs_ld;
+  p.args.ws0 = w_scale;
+  p.args.out = Y;
+  p.args.ldo = y_ld;
+  p.args.out_dtype = out_dtype;
+  p.args.status = dev_status;
+  return run_product<false>(p, segs, rows_hint, as_stream(stream));
+}
+
+extern "C" size_t dmoe_grouped_mlp_fp8_blocks_workspace_size(int m_rows, int I) {
+  if (m_rows < 0 || I < 0) return 0;
+  return (size_t)m_rows * (size_t)I + (size_t)m_rows * (size_t)blocks_of(I) * 4 + 1024;
+}
+
+namespace dmoe {
+namespace {
+int check_blk_mlp(const char* name, const void* x, const void* wg, const float* gs, const void* wu, const float* us,
+                  const void* wd, const float* ds, int d, int I, int n_seg, const int32_t* seg_expert,
+                  const int32_t* seg_end, int64_t m_rows, const void* workspace, size_t workspace_bytes,
+                  const int32_t* dev_status) {
+  DMOE_REQUIRE(x && wg && gs && wu && us && wd && ds && workspace && dev_status && seg_expert && seg_end,
+               "%s: null pointer", name);
+  DMOE_REQUIRE(aligned16(x) && aligned16(wg) && aligned16(wu) && aligned16(wd) && aligned16(workspace),
+               "%s: tensors must be 16-byte aligned", name);
+  DMOE_REQUIRE(aligned4(gs) && aligned4(us) && aligned4(ds), "%s: scales must be 4-byte aligned", name);
+  DMOE_REQUIRE(workspace_bytes >= dmoe_grouped_mlp_fp8_blocks_workspace_size((int)m_rows, I), "%s: workspace %zu < %zu bytes",
+               name, workspace_bytes, dmoe_grouped_mlp_fp8_blocks_workspace_size((int)m_rows, I));
+  DMOE_REQUIRE((m_rows + n_seg) * blocks_of(d > I ? d : I) < INT32_MAX, "%s: too many tiles", name);
+  return DMOE_OK;
+}
+}  // namespace
+}  // namespace dmoe
+
+extern "C" int dmoe_grouped_gated_mlp_fp8_blocks(const void* Xq, int64_t x_ld, const float* x_scale, int64_t xs_ld,
+                                                 const void* wg_q, const float* wg_scale, const void* wu_q,
+                                                 const float* wu_scale, const void* wd_q, const float* wd_scale,
+                                                 int E_stack, int d, int I, const int32_t* seg_expert,
+                                                 const int32_t* seg_end, int n_seg, int seg_on_device, int m_rows,
+                                                 int rows_hint, int act, void* Y, void* workspace,
+                                                 size_t workspace_bytes, int32_t* dev_status, void* stream) {
+  clear_error();
+  const char* name = "dmoe_grouped_gated_mlp_fp8_blocks";
+  DMOE_REQUIRE(act == DMOE_ACT_RELU || act == DMOE_ACT_SILU, "%s: bad activation %d", name, act);
+  DMOE_REQUIRE(d > 0 && I > 0 && d % 16 == 0 && I % 16 == 0, "%s: d=%d and I=%d must be multiples of 16", name, d, I);
+  DMOE_REQUIRE(E_stack >= 1 && m_rows >= 0 && n_seg >= 0 && rows_hint >= 0, "%s: bad E_stack/m_rows/n_seg/rows_hint",
+               name);
+  DMOE_REQUIRE(x_ld >= d && x_ld % 16 == 0 && xs_ld >= blocks_of(d), "%s: x_ld=%lld, xs_ld=%lld too small or odd", name,
+               (long long)x_ld, (long long)xs_ld);
+  if (n_seg == 0 || m_rows == 0) return DMOE_OK;
+  DMOE_REQUIRE(x_scale && Y, "%s: null pointer", name);
+  DMOE_REQUIRE(aligned4(x_scale) && aligned16(Y), "%s: misaligned scales or output", name);
+  if (int r = check_blk_mlp(name, Xq, wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale, d, I, n_seg, seg_expert, seg_end,
+                            m_rows, workspace, workspace_bytes, dev_status))
+    return r;
+  static thread_local BlkSegs segs;
+  if (int r = fill_blk_segs(name, segs, seg_expert, seg_end, n_seg, seg_on_device, m_rows, E_stack)) return r;
+  return run_blk_mlp(Xq, x_ld, x_scale, xs_ld, wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale, E_stack, d, I, segs,
+                     rows_hint, act, Y, nullptr, nullptr, workspace, dev_status, as_stream(stream));
+}

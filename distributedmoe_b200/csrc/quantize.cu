@@ -108,3 +108,177 @@ extern "C" int dmoe_quantize_rows_e4m3(const void* x, int dtype, int64_t rows, i
   DMOE_LAUNCH_CHECK();
   return DMOE_OK;
 }
+
+// ------------------------------------------------------------------------ blocks of 128 columns
+// Scales for blocks of 1 x 128 (activations) or 128 x 128 (weights): s = max(amax / 448, 2^-126),
+// 1 for an all-zero block, q = e4m3(x / s) with the quotient rounded to fp32 first, as above.  The
+// lower bound keeps the scale a normal number (a subnormal one could not be divided by).  A value
+// that is not finite becomes a NaN code and leaves its block's scale alone.
+//
+// Each thread holds the eight neighbouring values of one 16-byte load (two for fp32); 16 lanes make
+// a row of 128, so the row's amax is four shuffles and x is read once.
+namespace dmoe {
+namespace {
+
+constexpr float kFiniteMax = 3.402823466e38f;
+
+template <int DT>
+__device__ __forceinline__ float abs_max8(const float* f) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(f[i]);
+    m = fmaxf(m, a <= kFiniteMax ? a : 0.f);
+  }
+  return m;
+}
+
+__device__ __forceinline__ float scale_of(float amax) {
+  return amax > 0.f ? fmaxf(__fdiv_rn(amax, 448.f), 1.17549435e-38f) : 1.f;
+}
+
+__device__ __forceinline__ uint2 codes8(const float* f, float s) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = fabsf(f[4 * h + i]) <= kFiniteMax ? __fdiv_rn(f[4 * h + i], s) : __int_as_float(0x7fffffff);
+    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
+    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
+    w[h] = (uint32_t)lo | ((uint32_t)hi << 16);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// 1 x 128: a warp takes kRowCols consecutive columns of one row, two blocks per load.
+constexpr int kRowCols = 1024;
+
+template <int DT>
+__global__ void __launch_bounds__(kQuantWarps * 32)
+    quantize_row_blocks_kernel(const void* __restrict__ x, int64_t rows, int cols, int parts, uint8_t* __restrict__ q,
+                               int64_t q_ld, float* __restrict__ scale, int64_t scale_ld) {
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
+  const int64_t row = item / parts;
+  if (row >= rows) return;
+  const int c0 = (int)(item - row * parts) * kRowCols + lane * 8;
+  float f[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = c0 + i * 256;
+    if (c < cols) {
+      load8<DT>(x, row * cols + c, f[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = c0 + i * 256;
+    float m = abs_max8<DT>(f[i]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float s = scale_of(m);
+    if (c < cols) {
+      if ((lane & 15) == 0) scale[row * scale_ld + (c >> 7)] = s;
+      *reinterpret_cast<uint2*>(q + row * q_ld + c) = codes8(f[i], s);
+    }
+  }
+}
+
+// 128 x 128: a CTA takes one block of one matrix of the batch, 64 values a thread.
+template <int DT>
+__global__ void __launch_bounds__(256)
+    quantize_square_blocks_kernel(const void* __restrict__ x, int64_t rows, int cols, int col_blocks,
+                                  int64_t row_blocks, uint8_t* __restrict__ q, float* __restrict__ scale) {
+  __shared__ float tops[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t rb_all = blockIdx.x / col_blocks;  // row block within the whole batch
+  const int cb = (int)(blockIdx.x - rb_all * col_blocks);
+  const int64_t mat = rb_all / row_blocks;
+  const int64_t r0 = (rb_all - mat * row_blocks) * 128 + warp * 2 + (lane >> 4);
+  const int c = cb * 128 + (lane & 15) * 8;
+  const int64_t base = mat * rows * cols;
+  float f[8][8];
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + i * 16;
+    if (r < rows && c < cols) {
+      load8<DT>(x, base + r * cols + c, f[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, abs_max8<DT>(f[i]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) tops[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, tops[w]);
+  const float s = scale_of(m);
+  if (threadIdx.x == 0) scale[rb_all * col_blocks + cb] = s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + i * 16;
+    if (r < rows && c < cols) *reinterpret_cast<uint2*>(q + base + r * cols + c) = codes8(f[i], s);
+  }
+}
+
+template <int DT>
+int run_quantize_blocks(const void* x, int64_t batch, int64_t rows, int cols, int block_rows, uint8_t* q, int64_t q_ld,
+                        float* scale, int64_t scale_ld, cudaStream_t s) {
+  if (block_rows == 1) {
+    const int parts = (cols + kRowCols - 1) / kRowCols;
+    const int64_t grid = (batch * rows * parts + kQuantWarps - 1) / kQuantWarps;
+    DMOE_REQUIRE(grid <= INT32_MAX, "dmoe_quantize_blocks_e4m3: %lld rows", (long long)(batch * rows));
+    quantize_row_blocks_kernel<DT><<<(unsigned)grid, kQuantWarps * 32, 0, s>>>(x, batch * rows, cols, parts, q, q_ld,
+                                                                               scale, scale_ld);
+  } else {
+    const int64_t row_blocks = (rows + 127) / 128;
+    const int col_blocks = (cols + 127) / 128;
+    const int64_t grid = batch * row_blocks * col_blocks;
+    DMOE_REQUIRE(grid <= INT32_MAX, "dmoe_quantize_blocks_e4m3: %lld blocks", (long long)grid);
+    quantize_square_blocks_kernel<DT><<<(unsigned)grid, 256, 0, s>>>(x, rows, cols, col_blocks, row_blocks, q, scale);
+  }
+  DMOE_LAUNCH_CHECK();
+  return DMOE_OK;
+}
+
+}  // namespace
+}  // namespace dmoe
+
+extern "C" int dmoe_quantize_blocks_e4m3(const void* x, int dtype, int64_t batch, int64_t rows, int cols,
+                                         int block_rows, void* q, int64_t q_ld, float* scale, int64_t scale_ld,
+                                         void* stream) {
+  clear_error();
+  const char* name = "dmoe_quantize_blocks_e4m3";
+  DMOE_REQUIRE(dtype_ok(dtype), "%s: dtype must be f32, f16 or bf16", name);
+  DMOE_REQUIRE(block_rows == 1 || block_rows == 128, "%s: block_rows=%d must be 1 or 128", name, block_rows);
+  DMOE_REQUIRE(batch >= 0 && rows >= 0 && cols > 0 && cols % 16 == 0, "%s: cols=%d must be a multiple of 16", name,
+               cols);
+  if (batch == 0 || rows == 0) return DMOE_OK;
+  DMOE_REQUIRE(batch <= (INT64_MAX >> 24) / rows, "%s: %lld x %lld rows", name, (long long)batch, (long long)rows);
+  DMOE_REQUIRE(x && q && scale, "%s: null pointer", name);
+  DMOE_REQUIRE(aligned16(x) && aligned16(q) && (reinterpret_cast<uintptr_t>(scale) & 3u) == 0,
+               "%s: x and q must be 16-byte aligned, scale 4-byte", name);
+  const int col_blocks = (cols + 127) / 128;
+  DMOE_REQUIRE(q_ld >= cols && q_ld % 16 == 0 && scale_ld >= (block_rows == 1 ? col_blocks : 0),
+               "%s: q_ld=%lld must be >= cols and a multiple of 16, scale_ld=%lld >= %d", name, (long long)q_ld,
+               (long long)scale_ld, col_blocks);
+  DMOE_REQUIRE(block_rows == 1 || (q_ld == cols && scale_ld == col_blocks), "%s: 128 x 128 blocks take packed q and scale",
+               name);
+  uint8_t* qb = reinterpret_cast<uint8_t*>(q);
+  cudaStream_t s = as_stream(stream);
+  if (dtype == DMOE_BF16)
+    return run_quantize_blocks<DMOE_BF16>(x, batch, rows, cols, block_rows, qb, q_ld, scale, scale_ld, s);
+  if (dtype == DMOE_F16)
+    return run_quantize_blocks<DMOE_F16>(x, batch, rows, cols, block_rows, qb, q_ld, scale, scale_ld, s);
+  return run_quantize_blocks<DMOE_F32>(x, batch, rows, cols, block_rows, qb, q_ld, scale, scale_ld, s);
+}

@@ -220,6 +220,81 @@ int dmoe_grouped_gated_mlp_fp8(const void* Xq, const float* x_scale, const void*
                                int m_rows, int act, void* Y, void* workspace, size_t workspace_bytes,
                                int32_t* dev_status, int tile_policy, void* stream);
 
+/* 8-bit operands with a scale for each block of 128 (the layout of 8-bit checkpoints; no
+ * counterpart in the reference, whose "fp8" has no scales).
+ *
+ * dmoe_quantize_blocks_e4m3: `batch` matrices x [rows, cols] (f32/f16/bf16, packed) -> codes q and
+ *   one fp32 scale for each block of block_rows x 128 (block_rows 1: activations, 128: weights; the
+ *   last block of either axis may be smaller).  s = max(amax / 448, 2^-126), 1 for an all-zero
+ *   block; q = e4m3_rn(x / s), the quotient rounded to fp32 first.  A value that is not finite
+ *   becomes a NaN code and does not enter amax.
+ *   block_rows 1: q rows q_ld bytes apart, scale[row * scale_ld + col / 128] (batch * rows rows);
+ *   block_rows 128: q packed, scale [batch, ceil(rows / 128), ceil(cols / 128)].
+ *   cols % 16 == 0, q_ld % 16 == 0; x and q 16-byte aligned.
+ *
+ * dmoe_grouped_matmul_fp8_blocks: for the rows r of segment i (as dmoe_grouped_gated_mlp), with
+ *   e = seg_expert[i],
+ *     Y[r, n] = sum_b x_scale[r, b] * w_scale[e, n / 128, b] * sum_{j in b} Xq[r, j] * w_q[e, n, j]
+ *   over the 128-wide blocks b of K.  Xq: rows x_ld bytes apart, x_scale rows xs_ld floats apart;
+ *   w_q [E_stack, N, K], w_scale [E_stack, ceil(N / 128), ceil(K / 128)]; Y rows y_ld elements apart
+ *   in out_dtype (DMOE_BF16, DMOE_F16, DMOE_F32).  Sums in fp32.  Rows outside the segments are not
+ *   written.  One segment with E_stack = 1 is a plain linear layer.
+ *   N % 8 == 0, K % 16 == 0, x_ld % 16 == 0, y_ld % 8 == 0; codes and Y 16-byte aligned.
+ *   rows_hint: rows a segment is expected to have (0: m_rows / n_seg), which picks the tile shape
+ *   where the table is on the device or m_rows is a capacity; any value gives correct results.
+ *   Host tables hold up to 256 segments, device tables up to 1024; an end out of order or past
+ *   m_rows is clamped, a segment whose expert is outside the stack is left out, and both report
+ *   DMOE_DEVERR_BAD_SEGMENT.
+ *
+ * dmoe_grouped_gated_mlp_fp8_blocks: the gated MLP on such operands, down projection included:
+ *   wg_q, wu_q [E_stack, I, d], wd_q [E_stack, d, I] with 128 x 128 scales; h = act(gate) * up is
+ *   quantised 1 x 128 from the fp32 sums (its quotients h * (1 / s), within an ulp of h / s), Y
+ *   [m_rows, d] bf16.  d % 16 == 0, I % 16 == 0;
+ *   workspace >= dmoe_grouped_mlp_fp8_blocks_workspace_size(m_rows, I).
+ */
+int dmoe_quantize_blocks_e4m3(const void* x, int dtype, int64_t batch, int64_t rows, int cols, int block_rows, void* q,
+                              int64_t q_ld, float* scale, int64_t scale_ld, void* stream);
+int dmoe_grouped_matmul_fp8_blocks(const void* Xq, int64_t x_ld, const float* x_scale, int64_t xs_ld, const void* w_q,
+                                   const float* w_scale, int E_stack, int N, int K, const int32_t* seg_expert,
+                                   const int32_t* seg_end, int n_seg, int seg_on_device, int m_rows, int rows_hint,
+                                   void* Y, int64_t y_ld, int out_dtype, int32_t* dev_status, void* stream);
+size_t dmoe_grouped_mlp_fp8_blocks_workspace_size(int m_rows, int I);
+int dmoe_grouped_gated_mlp_fp8_blocks(const void* Xq, int64_t x_ld, const float* x_scale, int64_t xs_ld,
+                                      const void* wg_q, const float* wg_scale, const void* wu_q, const float* wu_scale,
+                                      const void* wd_q, const float* wd_scale, int E_stack, int d, int I,
+                                      const int32_t* seg_expert, const int32_t* seg_end, int n_seg, int seg_on_device,
+                                      int m_rows, int rows_hint, int act, void* Y, void* workspace,
+                                      size_t workspace_bytes, int32_t* dev_status, void* stream);
+
+/*
+ * Load-balance loss of a router, its per-expert counts and its gradient (no counterpart in the
+ * reference, which only runs forward).
+ *  logits  [T, E] (f32/f16/bf16); idx [T, k] the selected experts (entries outside [0, E) are
+ *          dropped activations and count nothing; a repeated one counts each time)
+ *  mode    DMOE_ROUTER_SOFTMAX: p = softmax(l); DMOE_ROUTER_SIGMOID_GROUP: p = sigmoid(l) / sum sigmoid(l)
+ *  seq_end [n_seq] ascending token ends of the sequences (device), NULL: one sequence of T tokens
+ *          (n_seq = 1).  Tokens behind the last one belong to none.
+ *  mask    [T] bytes, 0: the token does not count and its logits are not read; NULL: all count
+ *  counts  [n_seq * (E + 1) + 1] int32, written: C [n_seq, E], then the counted tokens n [n_seq],
+ *          then a scratch word; the backward call takes it as the forward call left it
+ *  loss    [2] fp32: balance = mean over sequences with tokens of
+ *            sum_e (E C[s,e] / (k n[s])) (sum_t p[t,e] / n[s]),
+ *          z = mean over counted tokens of logsumexp(l)^2; both 0 without tokens.
+ *  A row of -inf alone has p = 0 and adds nothing to either sum.
+ *  workspace: dmoe_balance_loss_workspace_size() bytes, 8-byte aligned.
+ *  dmoe_balance_loss_backward: grad [T, E] (dtype of the logits) = *g_balance d balance / d l +
+ *  *g_z d z / d l, C held constant; a NULL upstream gradient is zero; rows that do not count get 0.
+ *  Limits: E <= 1024, 1 <= k <= E, n_seq <= 2^20, T * k < 2^31.  Results do not depend on the order
+ *  in which CTAs run.  An invalid seq_end reports DMOE_DEVERR_BAD_SEGMENT.
+ */
+size_t dmoe_balance_loss_workspace_size(void);
+int dmoe_balance_loss(const void* logits, int dtype, const int64_t* idx, int T, int E, int k, int mode,
+                      const int32_t* seq_end, int n_seq, const uint8_t* mask, int32_t* counts, float* loss,
+                      void* workspace, size_t workspace_bytes, int32_t* dev_status, void* stream);
+int dmoe_balance_loss_backward(const void* logits, int dtype, int T, int E, int k, int mode, const int32_t* seq_end,
+                               int n_seq, const uint8_t* mask, const int32_t* counts, const float* g_balance,
+                               const float* g_z, void* grad, void* stream);
+
 /*
  * Number of SMs (0..64, process-wide, default 0) that later dmoe_grouped_gated_mlp launches
  * leave free.  No counterpart in the reference.  The grouped MLP is a persistent kernel that
