@@ -194,6 +194,23 @@ __device__ __forceinline__ char* blk_out_row(const BlkArgs& a, int row, int esz)
   return base == nullptr ? nullptr : base + (int64_t)(code & 0x7ffffff) * a.ldo * esz;
 }
 
+// tmem_ld32 in two halves: the registers hold their values after the second, which waits for every
+// load this warp has started.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : DMOE_R8(0), DMOE_R8(8), DMOE_R8(16), DMOE_R8(24)
+      : "r"(taddr)
+      : "memory");
+}
+#define BLK_RW8(b) "+r"(r[b + 0]), "+r"(r[b + 1]), "+r"(r[b + 2]), "+r"(r[b + 3]), "+r"(r[b + 4]), "+r"(r[b + 5]), \
+                   "+r"(r[b + 6]), "+r"(r[b + 7])
+__device__ __forceinline__ void tmem_ld32_finish(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : BLK_RW8(0), BLK_RW8(8), BLK_RW8(16), BLK_RW8(24)::"memory");
+}
+#undef BLK_RW8
+
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]);
 template <>
@@ -430,18 +447,22 @@ __global__ void __launch_bounds__(kPThreads, 1)
         tc_fence_after();
         const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kPN);
         const uint64_t s0p = pack_f2(s0, s0), s1p = pack_f2(s1, s1);
+        uint32_t v[2][32];  // the next 32 columns come while these are added
+        tmem_ld32_start(tbase + (GATED ? half * 64 : half * 128), v[0]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int col = GATED ? (j < 2 ? half * 64 + j * 32 : 128 + half * 64 + (j - 2) * 32) : half * 128 + j * 32;
-          uint32_t v[32];
-          tmem_ld32(tbase + col, v);
-          if (j == 3) {
+          tmem_ld32_finish(v[j & 1]);
+          if (j < 3) {
+            const int n = j + 1;
+            const int col = GATED ? (n < 2 ? half * 64 + n * 32 : 128 + half * 64 + (n - 2) * 32) : half * 128 + n * 32;
+            tmem_ld32_start(tbase + col, v[n & 1]);
+          } else {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acce_leader0 + (uint32_t)(acc * sizeof(uint64_t)));
+            if (lane == 0) mbar_arrive_remote(acce_leader0 + (uint32_t)(acc * sizeof(uint64_t)));
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) fma2(sum[j * 16 + i], v[2 * i], v[2 * i + 1], j < 2 ? s0p : s1p);
+          for (int i = 0; i < 16; ++i) fma2(sum[j * 16 + i], v[j & 1][2 * i], v[j & 1][2 * i + 1], j < 2 ? s0p : s1p);
         }
         acc ^= 1;
         if (acc == 0) acc_ph ^= 1u;
