@@ -379,26 +379,31 @@ __global__ void __launch_bounds__(kPThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (leader CTA)
-    if (leader && lane == 0) {
+    // The whole warp walks the steps and one lane issues: with uniform control flow around it an
+    // issue takes a fraction of what it does inside a branch of one lane.
+    if (leader) {
       constexpr uint32_t idesc = blk_idesc(kPM, kPN);
+      const uint64_t xd0 = sdesc_sw128(smem_u32(smem)), wd0 = sdesc_sw128(smem_u32(smem + kPOpBytes));
       int stage = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
       for (int tile = pair; tile < total && ok; tile += n_pairs) {
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_wait(&full[stage], ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA) ||
-              !mbar_wait(&acce[acc], acc_ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA)) {
-            ok = false;
-            break;
-          }
+          ok = wait_in_line(&full[stage], ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA) &&
+               wait_in_line(&acce[acc], acc_ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           tc_fence_after();
-          const uint64_t xd = sdesc_sw128(smem_u32(smem + stage * kPStageBytes));
-          const uint64_t wd = sdesc_sw128(smem_u32(smem + stage * kPStageBytes + kPOpBytes));
+          if (elect_one()) {
+            const uint64_t off = (uint64_t)(stage * (kPStageBytes >> 4));
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // 32 codes of K per MMA; the first starts a fresh sum
-            umma_f16_pair<DMOE_E4M3>(tmem_base + (uint32_t)(acc * kPN), xd + 2 * k, wd + 2 * k, idesc, k != 0);
-          umma_commit_both(&empty[stage]);
-          umma_commit_both(&accf[acc]);
+            for (int k = 0; k < 4; ++k)  // 32 codes of K per MMA; the first starts a fresh sum
+              umma_f16_pair<DMOE_E4M3>(tmem_base + (uint32_t)(acc * kPN), xd0 + off + 2 * k, wd0 + off + 2 * k, idesc,
+                                       k != 0);
+            umma_commit_both(&empty[stage]);
+            umma_commit_both(&accf[acc]);
+          }
+          __syncwarp();
           if (++stage == kPStages) {
             stage = 0;
             ph ^= 1u;
@@ -407,7 +412,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
           if (acc == 0) acc_ph ^= 1u;
         }
       }
-      umma_commit_both(fin);
+      if (elect_one()) umma_commit_both(fin);
+      __syncwarp();
     }
     // Every MMA of the pair (issued by the leader) has completed once `fin` fires in this CTA.
     if (lane == 0) wait_or_report(fin, 0, args.status);

@@ -182,6 +182,17 @@ __device__ __forceinline__ void tmem_ld32x2(uint32_t ta, uint32_t tb, uint32_t (
       : "memory");
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(p)::"memory");
+  return p != 0;
+}
+
 // Shared-memory matrix descriptor, K-major operand in the 128-byte swizzle layout written by
 // TMA (rows of 128 bytes, 8-row groups 1024 bytes apart): LBO = 16 B (unused), SBO = 1024 B,
 // descriptor version 1 (sm_100), layout type 2 (SWIZZLE_128B).
