@@ -201,7 +201,10 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # The raw handle: building a torch.cuda.Stream object for it takes several microseconds.
+    if device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _require_cuda(*ts: Optional[torch.Tensor]) -> torch.device:
@@ -232,9 +235,12 @@ def _one_device(*ts: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(dev: torch.device):
     """Make `dev` current for a launch (its streams belong to it)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 # ----------------------------------------------------------------------------- scratch
@@ -640,9 +646,10 @@ def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Te
         batch = x.numel() // (rows * cols) if rows else 0
         scale = torch.empty(*x.shape[:-2], _blocks(rows), _blocks(cols), dtype=torch.float32, device=dev)
     with _on(dev):
-        tm = _Timed("quantize_blocks_e4m3", _stream(dev), dev)
+        st = _stream(dev)
+        tm = _Timed("quantize_blocks_e4m3", st, dev)
         rc = lib().dmoe_quantize_blocks_e4m3(x.data_ptr(), dtype_code(x.dtype), batch, rows, cols, block_rows,
-                                             q.data_ptr(), cols, scale.data_ptr(), _blocks(cols), _stream(dev))
+                                             q.data_ptr(), cols, scale.data_ptr(), _blocks(cols), st)
         _check(rc, "dmoe_quantize_blocks_e4m3")
         tm.done()
     return q, scale
@@ -712,11 +719,12 @@ def grouped_matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torc
     y_ld = out.stride(0) if m > 1 else Nn
     se, sn, n_seg, on_dev, keep = _segments(seg_expert, seg_end, dev)
     with _on(dev):
-        tm = _Timed("grouped_matmul_fp8_blocks", _stream(dev), dev)
+        st = _stream(dev)
+        tm = _Timed("grouped_matmul_fp8_blocks", st, dev)
         rc = lib().dmoe_grouped_matmul_fp8_blocks(xq.data_ptr(), x_ld, x_scale.data_ptr(), xs_ld, w_q.data_ptr(),
                                                   w_scale.data_ptr(), E, Nn, K, se, sn, n_seg, on_dev, m,
                                                   int(rows_hint), out.data_ptr(), y_ld, dtype_code(out.dtype),
-                                                  scratch.status(dev).data_ptr(), _stream(dev))
+                                                  scratch.status(dev).data_ptr(), st)
         del keep
         _check(rc, "dmoe_grouped_matmul_fp8_blocks")
         tm.done()
@@ -787,12 +795,13 @@ def grouped_gated_mlp_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, expert
     ws = torch.empty(lib().dmoe_grouped_mlp_fp8_blocks_workspace_size(m, I), dtype=torch.uint8, device=dev)
     se, sn, n_seg, on_dev, keep = _segments(seg_expert, seg_end, dev)
     with _on(dev):
-        tm = _Timed("grouped_gated_mlp_fp8_blocks", _stream(dev), dev)
+        st = _stream(dev)
+        tm = _Timed("grouped_gated_mlp_fp8_blocks", st, dev)
         rc = lib().dmoe_grouped_gated_mlp_fp8_blocks(
             xq.data_ptr(), x_ld, x_scale.data_ptr(), xs_ld, experts.wg_q.data_ptr(), experts.wg_scale.data_ptr(),
             experts.wu_q.data_ptr(), experts.wu_scale.data_ptr(), experts.wd_q.data_ptr(), experts.wd_scale.data_ptr(),
             E, d, I, se, sn, n_seg, on_dev, m, int(rows_hint), int(act), Y.data_ptr(), ws.data_ptr(), ws.numel(),
-            scratch.status(dev).data_ptr(), _stream(dev))
+            scratch.status(dev).data_ptr(), st)
         del keep
         _check(rc, "dmoe_grouped_gated_mlp_fp8_blocks")
         tm.done()
@@ -811,18 +820,20 @@ class _BalanceLoss(torch.autograd.Function):
         loss = torch.empty(2, dtype=torch.float32, device=dev)
         ws = torch.empty(lib().dmoe_balance_loss_workspace_size(), dtype=torch.uint8, device=dev)
         with _on(dev):
-            tm = _Timed("balance_loss", _stream(dev), dev)
+            st = _stream(dev)
+            tm = _Timed("balance_loss", st, dev)
             rc = lib().dmoe_balance_loss(logits.data_ptr(), dtype_code(logits.dtype), idx.data_ptr(), T, E, k, mode,
                                          _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), loss.data_ptr(),
-                                         ws.data_ptr(), ws.numel(), scratch.status(dev).data_ptr(), _stream(dev))
+                                         ws.data_ptr(), ws.numel(), scratch.status(dev).data_ptr(), st)
             _check(rc, "dmoe_balance_loss")
             tm.done()
         ctx.save_for_backward(logits, seq_end, mask, counts)
         ctx.args = (T, E, k, mode, S)
         ctx.set_materialize_grads(False)
-        per_expert = counts[:S * E].view(S, E)
+        per_expert = counts.as_strided((S, E), (E, 1))
         ctx.mark_non_differentiable(per_expert)
-        return loss[0], loss[1], per_expert
+        balance, z = loss.unbind()
+        return balance, z, per_expert
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -834,10 +845,11 @@ class _BalanceLoss(torch.autograd.Function):
         dev = logits.device
         grad = torch.empty_like(logits)
         with _on(dev):
-            tm = _Timed("balance_loss_backward", _stream(dev), dev)
+            st = _stream(dev)
+            tm = _Timed("balance_loss_backward", st, dev)
             rc = lib().dmoe_balance_loss_backward(logits.data_ptr(), dtype_code(logits.dtype), T, E, k, mode,
                                                   _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), _ptr(g_balance),
-                                                  _ptr(g_z), grad.data_ptr(), _stream(dev))
+                                                  _ptr(g_z), grad.data_ptr(), st)
             _check(rc, "dmoe_balance_loss_backward")
             tm.done()
         return grad, None, None, None, None

@@ -122,14 +122,18 @@ namespace {
 
 constexpr float kFiniteMax = 3.402823466e38f;
 
-template <int DT>
+// Largest magnitude; fmaxf prefers a number to NaN, so only an infinity shows in it.
 __device__ __forceinline__ float abs_max8(const float* f) {
+  float m = fabsf(f[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
+  return fmaxf(m, 0.f);
+}
+
+__device__ __forceinline__ float finite_max8(const float* f) {
   float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(f[i]);
-    m = fmaxf(m, a <= kFiniteMax ? a : 0.f);
-  }
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]) <= kFiniteMax ? fabsf(f[i]) : 0.f);
   return m;
 }
 
@@ -137,33 +141,47 @@ __device__ __forceinline__ float scale_of(float amax) {
   return amax > 0.f ? fmaxf(__fdiv_rn(amax, 448.f), 1.17549435e-38f) : 1.f;
 }
 
-__device__ __forceinline__ uint2 codes8(const float* f, float s) {
+// Codes of eight values by a block's scale and its rounded reciprocal.  x / s as a product with the
+// reciprocal and one correction by the residual, which the fused steps compute exactly (Markstein,
+// 1990): the value before the last rounding is within 1.5 x 2^-24 ulp of the quotient, so it rounds
+// as the quotient does unless that lies so near the middle between two fp32 numbers.  `fast` must be
+// false for scales below 2^-90, where the residual could be subnormal, and where infinities have
+// to become NaN codes (the conversion saturates them); those take the division.
+__device__ __forceinline__ uint2 codes8(const float* f, float s, float inv, bool fast) {
+  float v[8];
+  if (fast) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float r = __fmul_rn(f[i], inv);
+      v[i] = __fmaf_rn(__fmaf_rn(-r, s, f[i]), inv, r);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fabsf(f[i]) <= kFiniteMax ? __fdiv_rn(f[i], s) : __int_as_float(0x7fffffff);
+  }
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = fabsf(f[4 * h + i]) <= kFiniteMax ? __fdiv_rn(f[4 * h + i], s) : __int_as_float(0x7fffffff);
-    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
-    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
+    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h], v[4 * h + 1]), __NV_SATFINITE, __NV_E4M3);
+    const __nv_fp8x2_storage_t hi =
+        __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h + 2], v[4 * h + 3]), __NV_SATFINITE, __NV_E4M3);
     w[h] = (uint32_t)lo | ((uint32_t)hi << 16);
   }
   return make_uint2(w[0], w[1]);
 }
+constexpr float kFastScale = 8.0779357e-28f;  // 2^-90
 
 // 1 x 128: a warp takes kRowCols consecutive columns of one row, two blocks per load.
 constexpr int kRowCols = 1024;
 
 template <int DT>
 __global__ void __launch_bounds__(kQuantWarps * 32)
-    quantize_row_blocks_kernel(const void* __restrict__ x, int64_t rows, int cols, int parts, uint8_t* __restrict__ q,
+    quantize_row_blocks_kernel(const void* __restrict__ x, int64_t rows, int cols, uint8_t* __restrict__ q,
                                int64_t q_ld, float* __restrict__ scale, int64_t scale_ld) {
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
-  const int64_t row = item / parts;
+  const int64_t row = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const int c0 = (int)(item - row * parts) * kRowCols + lane * 8;
+  const int c0 = blockIdx.y * kRowCols + lane * 8;
   float f[4][8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -178,13 +196,19 @@ __global__ void __launch_bounds__(kQuantWarps * 32)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = c0 + i * 256;
-    float m = abs_max8<DT>(f[i]);
+    float m = abs_max8(f[i]);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool infinite = m > kFiniteMax;
+    if (__any_sync(0xffffffffu, infinite)) {
+      m = finite_max8(f[i]);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    }
     const float s = scale_of(m);
     if (c < cols) {
       if ((lane & 15) == 0) scale[row * scale_ld + (c >> 7)] = s;
-      *reinterpret_cast<uint2*>(q + row * q_ld + c) = codes8(f[i], s);
+      *reinterpret_cast<uint2*>(q + row * q_ld + c) = codes8(f[i], s, __frcp_rn(s), !infinite && s >= kFastScale);
     }
   }
 }
@@ -215,19 +239,26 @@ __global__ void __launch_bounds__(256)
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, abs_max8<DT>(f[i]));
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, abs_max8(f[i]));
+  const bool infinite = __syncthreads_or(m > kFiniteMax);
+  if (infinite) {
+    m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_max8(f[i]));
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) tops[warp] = m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 8; ++w) m = fmaxf(m, tops[w]);
-  const float s = scale_of(m);
+  const float s = scale_of(m), inv = __frcp_rn(s);
+  const bool fast = !infinite && s >= kFastScale;
   if (threadIdx.x == 0) scale[rb_all * col_blocks + cb] = s;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t r = r0 + i * 16;
-    if (r < rows && c < cols) *reinterpret_cast<uint2*>(q + base + r * cols + c) = codes8(f[i], s);
+    if (r < rows && c < cols) *reinterpret_cast<uint2*>(q + base + r * cols + c) = codes8(f[i], s, inv, fast);
   }
 }
 
@@ -236,10 +267,11 @@ int run_quantize_blocks(const void* x, int64_t batch, int64_t rows, int cols, in
                         float* scale, int64_t scale_ld, cudaStream_t s) {
   if (block_rows == 1) {
     const int parts = (cols + kRowCols - 1) / kRowCols;
-    const int64_t grid = (batch * rows * parts + kQuantWarps - 1) / kQuantWarps;
-    DMOE_REQUIRE(grid <= INT32_MAX, "dmoe_quantize_blocks_e4m3: %lld rows", (long long)(batch * rows));
-    quantize_row_blocks_kernel<DT><<<(unsigned)grid, kQuantWarps * 32, 0, s>>>(x, batch * rows, cols, parts, q, q_ld,
-                                                                               scale, scale_ld);
+    const int64_t grid = (batch * rows + kQuantWarps - 1) / kQuantWarps;
+    DMOE_REQUIRE(grid <= INT32_MAX && parts <= 65535, "dmoe_quantize_blocks_e4m3: %lld rows of %d", (long long)(batch * rows),
+                 cols);
+    quantize_row_blocks_kernel<DT><<<dim3((unsigned)grid, parts), kQuantWarps * 32, 0, s>>>(x, batch * rows, cols, q,
+                                                                                            q_ld, scale, scale_ld);
   } else {
     const int64_t row_blocks = (rows + 127) / 128;
     const int col_blocks = (cols + 127) / 128;
