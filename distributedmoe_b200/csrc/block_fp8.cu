@@ -13,12 +13,15 @@
 // with a scale for each row and 128 columns, made from the fp32 accumulators in the epilogue; it
 // is the input of the down product, which is the plain form.
 //
-// Two kernels:
-//   pair      256 rows x 256 weight rows on two SMs (tcgen05 cta_group::2): many rows a segment,
-//             bound by the tensor cores.
-//   few rows  128 weight rows as the MMA's M, 16..128 rows of x as its N, one SM: few rows a
-//             segment, bound by reading the weights; with few tiles the reduction is split over a
-//             cluster and joined through distributed shared memory, in the order of the ranks.
+// Two kernels of one shape, x as the MMA's M and 256 weight rows as its N:
+//   pair    256 rows of x on two SMs (tcgen05 cta_group::2): many rows a segment, bound by the tensor
+//           cores.
+//   single  a row tile of 32, 64 or 128 rows on one SM: few rows a segment, bound by reading the
+//           weights.  With few tiles the reduction is split over a cluster and joined through
+//           distributed shared memory, in the order of the ranks.
+// The weights are never the M operand, although they have more rows than a decode batch: an MMA takes
+// 123 cycles to load its 128 rows of M whatever N is (128 for N = 256), so 256 weight rows a step
+// cost 4 x 128 cycles as N and 8 x 123 as M.
 #include <cuda_fp8.h>
 
 #include "dmoe_common.cuh"
@@ -31,7 +34,6 @@ constexpr int kBlk = 128;          // scale block; also bytes of one swizzle row
 constexpr int kMaxSegs = 1024;     // device segment tables
 constexpr int kMaxHostSegs = 256;  // host tables travel in the launch parameters
 constexpr int kEpiWarps = 8;
-constexpr int kBlkThreads = 64 + 32 * kEpiWarps;  // TMA warp, MMA warp, epilogue warps
 
 struct BlkSegs {
   int n_seg, m_rows, e_stack;
@@ -79,9 +81,17 @@ __device__ __forceinline__ SegTable seg_table_at(void* p) {
   return SegTable{b, b + (kMaxSegs + 4), b + 2 * (kMaxSegs + 4), b + 3 * (kMaxSegs + 4)};
 }
 
-// One warp reads the table, 32 segments at a time: ends are clamped to [previous end, m_rows]
-// (reported in *status where that changes one), entries outside the stack are left out.
-__device__ void read_segments(const BlkSegs& segs, const SegTable& t, int tile_m, int32_t* status) {
+// The whole CTA fetches the table at once (one trip to memory), ...
+__device__ __forceinline__ void fetch_segments(const BlkSegs& segs, const SegTable& t) {
+  for (int i = threadIdx.x; i < segs.n_seg; i += blockDim.x) {
+    t.end[i] = segs.dev_end ? segs.dev_end[i] : segs.end[i];
+    t.expert[i] = segs.dev_expert ? segs.dev_expert[i] : segs.expert[i];
+  }
+}
+
+// ... and one warp makes tiles of it, 32 segments at a time: ends are clamped to [previous end,
+// m_rows] (reported in *status where that changes one), entries outside the stack are left out.
+__device__ __forceinline__ void read_segments(const BlkSegs& segs, const SegTable& t, int tile_m, int32_t* status) {
   const int lane = threadIdx.x & 31;
   const int n = segs.n_seg;
   int prev = 0, tiles = 0, bad = 0;
@@ -89,8 +99,8 @@ __device__ void read_segments(const BlkSegs& segs, const SegTable& t, int tile_m
     const int i = base + lane;
     int en = 0, e = -1;
     if (i < n) {
-      en = segs.dev_end ? segs.dev_end[i] : segs.end[i];
-      e = segs.dev_expert ? segs.dev_expert[i] : segs.expert[i];
+      en = t.end[i];
+      e = t.expert[i];
     }
     const int given = en;
     en = min(max(en, 0), segs.m_rows);
@@ -164,10 +174,11 @@ __device__ __forceinline__ float2 unpack_f2(uint64_t v) {
   return make_float2(__uint_as_float(a), __uint_as_float(b));
 }
 
-// |v|, 0 for infinities and NaN, as an unsigned number (non-negative floats order as their bits).
-__device__ __forceinline__ uint32_t finite_abs_bits(float v) {
-  const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0u;
+constexpr float kFinite = 3.402823466e38f;
+
+// silu(g) or relu(g), the division as a product with the approximate reciprocal (2 ulp).
+__device__ __forceinline__ float blk_act(float g, int act) {
+  return act == DMOE_ACT_SILU ? __fdividef(g, 1.f + __expf(-g)) : fmaxf(g, 0.f);
 }
 
 // Scale of a block with this largest finite magnitude.
@@ -175,13 +186,12 @@ __device__ __forceinline__ float block_scale(float amax) {
   return amax > 0.f ? fmaxf(__fdiv_rn(amax, 448.f), 1.17549435e-38f) : 1.f;
 }
 
-// Four codes of h * inv; infinities become NaN codes (the conversion saturates them otherwise).
+__device__ __forceinline__ float finite_abs(float v) { return fabsf(v) <= kFinite ? fabsf(v) : 0.f; }
+
+// Four codes of h * inv (NaN stays NaN).
 __device__ __forceinline__ uint32_t codes4(const float* h, float inv) {
-  float v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = fabsf(h[i]) <= 3.402823466e38f ? h[i] * inv : __int_as_float(0x7fffffff);
-  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
-  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(h[0] * inv, h[1] * inv), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(h[2] * inv, h[3] * inv), __NV_SATFINITE, __NV_E4M3);
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
@@ -210,31 +220,6 @@ __device__ __forceinline__ void tmem_ld32_finish(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : BLK_RW8(0), BLK_RW8(8), BLK_RW8(16), BLK_RW8(24)::"memory");
 }
 #undef BLK_RW8
-
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]);
-template <>
-__device__ __forceinline__ void tmem_ld<32>(uint32_t taddr, uint32_t (&r)[32]) {
-  tmem_ld32(taddr, r);
-}
-template <>
-__device__ __forceinline__ void tmem_ld<16>(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];\n\ttcgen05.wait::ld.sync.aligned;"
-      : DMOE_R8(0), DMOE_R8(8)
-      : "r"(taddr)
-      : "memory");
-}
-template <>
-__device__ __forceinline__ void tmem_ld<8>(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : DMOE_R8(0)
-      : "r"(taddr)
-      : "memory");
-}
 
 // kind::f8f6f4, D fp32, A and B e4m3 (format 0), both K-major.
 __host__ __device__ constexpr uint32_t blk_idesc(int m, int n) {
@@ -271,33 +256,182 @@ __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// ------------------------------------------------------------------------------- pair kernel
-// A CTA pair computes 256 rows x 256 weight rows (gated: 128 gate and 128 up rows).  Each CTA
-// loads its 128 rows of x and its 128 weight rows (gated: CTA 0 the gate rows, CTA 1 the up rows);
-// its TMEM holds its 128 rows of x by all 256 columns, twice.  Eight epilogue warps: warp pairs
-// share a lane quadrant, each takes half of the columns (gated: 64 gate and the matching 64 up
-// columns), 128 fp32 sums a thread.  The sums need more registers than 65,536 / 384 threads: the
-// first warpgroup (TMA, MMA, segment table, one idle warp) hands its own to the other two.
-constexpr int kPM = 256, kPN = 256;
-constexpr int kPThreads = 128 + 32 * kEpiWarps;
-constexpr int kPRegsIssue = 56, kPRegsSums = 224;  // 128 * 56 + 256 * 224 = 384 * 168, the registers at launch
-constexpr int kPStages = 5;
-constexpr int kPOpBytes = 128 * kBlk;
-constexpr int kPStageBytes = 2 * kPOpBytes;
-constexpr int kPBarBytes = 256;
-constexpr int kPXchBytes = 2 * 2 * 128 * 4;
-constexpr int kPOutBytes = kEpiWarps * 32 * 128;  // 128 bytes of 32 rows for each epilogue warp
-constexpr int kPSmemBytes = 1024 + kPStages * kPStageBytes + kPOutBytes + kPBarBytes + kPXchBytes + kSegTableBytes;
+// --------------------------------------------------------------------- the epilogue of both kernels
+// Eight epilogue warps: warp pairs share a lane quadrant (rows of x), each takes half of the 256
+// columns (gated: 64 gate and the matching 64 up columns), 128 fp32 sums a thread.  The sums need more
+// registers than 65,536 / 384 threads: the first warpgroup (TMA, MMA, segment table, one idle warp)
+// hands its own to the other two.
+constexpr int kN = 256;                // weight rows of a tile: gated 128 gate and 128 up rows
+constexpr int kThreadsBlk = 128 + 32 * kEpiWarps;
+constexpr int kRegsIssue = 56, kRegsSums = 224;  // 128 * 56 + 256 * 224 = 384 * 168, the registers at launch
+constexpr int kOpBytes = 128 * kBlk;             // one step of 128 operand rows
+constexpr int kBarBytes = 256;
+constexpr int kXchBytes = 2 * 2 * 128 * 4;
+constexpr int kOutBytes = kEpiWarps * 32 * 128;  // 128 bytes of 32 rows for each epilogue warp
 
 template <bool GATED>
-__global__ void __launch_bounds__(kPThreads, 1)
+__device__ __forceinline__ int tmem_col(int half, int j) {  // first of the 32 columns of chunk j
+  return GATED ? (j < 2 ? half * 64 + j * 32 : 128 + half * 64 + (j - 2) * 32) : half * 128 + j * 32;
+}
+
+// Reads back this warp's 32 rows and 128 columns of an accumulator and adds them, scaled; `release`
+// hands the accumulator back as soon as the last columns are in registers.
+template <bool GATED, class F>
+__device__ __forceinline__ void add_step(uint64_t (&sum)[64], uint32_t tbase, int half, float s0, float s1, F&& release) {
+  const uint64_t s0p = pack_f2(s0, s0), s1p = pack_f2(s1, s1);
+  uint32_t v[2][32];  // the next 32 columns come while these are added
+  tmem_ld32_start(tbase + tmem_col<GATED>(half, 0), v[0]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    tmem_ld32_finish(v[j & 1]);
+    if (j < 3)
+      tmem_ld32_start(tbase + tmem_col<GATED>(half, j + 1), v[(j + 1) & 1]);
+    else
+      release();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) fma2(sum[j * 16 + i], v[j & 1][2 * i], v[j & 1][2 * i + 1], j < 2 ? s0p : s1p);
+  }
+}
+
+// Results of a tile, the row `row` in each lane.  They go through shared memory (`st`: this warp's
+// 4 KB), so that a store instruction writes runs of 64 or 128 bytes of a few rows rather than 16
+// bytes of 32: 6,300 cycles a tile before, at 256 columns of bf16.
+
+// h = act(gate) * up as codes, with the scale of the row's 128 columns; the other 64 of them are in
+// the warp that shares this quadrant (`xch`: both warps' largest magnitudes).
+__device__ __forceinline__ void store_codes(const uint64_t (&sum)[64], const BlkArgs& a, int row, int row_end, bool ok,
+                                            int nt, int half, int q, uint32_t* xch, uint4* st) {
+  const int lane = threadIdx.x & 31;
+  float h[64];
+  float top = 0.f;  // fmaxf prefers a number to NaN, so only an infinity shows in it
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const float2 g = unpack_f2(sum[i]), u = unpack_f2(sum[32 + i]);
+    h[2 * i] = blk_act(g.x, a.act) * u.x;
+    h[2 * i + 1] = blk_act(g.y, a.act) * u.y;
+    top = fmaxf(top, fmaxf(fabsf(h[2 * i]), fabsf(h[2 * i + 1])));
+  }
+  if (top > kFinite) {  // infinities become NaN codes and leave the scale alone
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+      top = fmaxf(top, finite_abs(h[i]));
+      if (fabsf(h[i]) > kFinite) h[i] = __int_as_float(0x7fffffff);
+    }
+  }
+  xch[half * 128 + q * 32 + lane] = __float_as_uint(top);
+  named_sync(1 + q, 64);
+  const float s = block_scale(fmaxf(top, __uint_as_float(xch[(half ^ 1) * 128 + q * 32 + lane])));
+  const float inv = __frcp_rn(s);
+  if (half == 0 && ok && row < row_end) a.out_scale[(int64_t)row * a.os_ld + nt] = s;
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+    st[lane * 4 + (v ^ ((lane >> 1) & 3))] = make_uint4(codes4(h + v * 16, inv), codes4(h + v * 16 + 4, inv),
+                                                        codes4(h + v * 16 + 8, inv), codes4(h + v * 16 + 12, inv));
+  __syncwarp();
+  const int col = nt * 128 + half * 64 + (lane & 3) * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    const uint4 v = st[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
+    const int64_t orow = row - lane + r;
+    if (ok && orow < row_end && col < a.n_out)
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.out) + orow * a.ldo + col) = v;
+  }
+  __syncwarp();
+}
+
+// A plain product's columns, rounded to the output type.
+__device__ __forceinline__ void store_rows(const uint64_t (&sum)[64], const BlkArgs& a, int row, bool valid, int nt,
+                                           int half, uint4* st) {
+  const int lane = threadIdx.x & 31;
+  const bool f32 = a.out_dtype == DMOE_F32;
+  const int esz = f32 ? 4 : 2;
+  const int col0 = nt * kN + half * 128;
+  char* const dst = valid ? blk_out_row(a, row, esz) : nullptr;
+  const int vec = 16 / esz;  // columns of 16 bytes
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {  // 32 columns a thread; 128 bytes of each row at a time
+    if (f32) {
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        const float2 x = unpack_f2(sum[p * 16 + 2 * v]), y = unpack_f2(sum[p * 16 + 2 * v + 1]);
+        st[lane * 8 + (v ^ (lane & 7))] =
+            make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        uint32_t pk[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = unpack_f2(sum[p * 16 + 4 * v + i]);
+          pk[i] = a.out_dtype == DMOE_BF16 ? pack2<DMOE_BF16>(x.x, x.y) : pack2<DMOE_F16>(x.x, x.y);
+        }
+        st[lane * 8 + (((p & 1) * 4 + v) ^ (lane & 7))] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+      }
+      if ((p & 1) == 0) continue;
+    }
+    __syncwarp();
+    const int col = col0 + (f32 ? p * 32 : (p >> 1) * 64) + (lane & 7) * vec;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3);
+      char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+      const uint4 v = st[r * 8 + ((lane & 7) ^ (r & 7))];
+      if (to != nullptr && col < a.n_out) *reinterpret_cast<uint4*>(to + (int64_t)col * esz) = v;
+    }
+    __syncwarp();
+  }
+}
+
+// Scales of the steps of one row and of the two column blocks of a tile, each fetched a step ahead.
+struct StepScales {
+  const float *x, *w0, *w1;
+  float xn, an, bn;
+  template <bool GATED>
+  __device__ __forceinline__ void start(const BlkArgs& a, const BlkTile& t, int row, bool valid, int half, int kb) {
+    x = a.xs + (int64_t)(valid ? row : t.row0) * a.xs_ld;
+    // Gated: this column block of both stacks; plain: this half's block (the last tile's second half
+    // may lie past the last block: its sums are never stored).
+    const int nb = GATED ? t.nt : min(t.nt * 2 + half, a.n_blk - 1);
+    const int64_t at = ((int64_t)t.expert * a.n_blk + nb) * a.k_blk;
+    w0 = a.ws0 + at;
+    w1 = GATED ? a.ws1 + at : w0;
+    xn = __ldg(x + kb);
+    an = __ldg(w0 + kb);
+    bn = GATED ? __ldg(w1 + kb) : an;
+  }
+  template <bool GATED>
+  __device__ __forceinline__ void take(int kb, int end, float& s0, float& s1) {
+    s0 = xn * an;
+    s1 = xn * bn;
+    if (kb + 1 < end) {
+      xn = __ldg(x + kb + 1);
+      an = __ldg(w0 + kb + 1);
+      bn = GATED ? __ldg(w1 + kb + 1) : an;
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------- pair kernel
+// A CTA pair computes 256 rows x 256 weight rows.  Each CTA loads its 128 rows of x and its 128 weight
+// rows (gated: CTA 0 the gate rows, CTA 1 the up rows); its TMEM holds its 128 rows of x by all 256
+// columns, twice.
+constexpr int kPM = 256;
+constexpr int kPStages = 5;
+constexpr int kPStageBytes = 2 * kOpBytes;
+constexpr int kPSmemBytes = 1024 + kPStages * kPStageBytes + kOutBytes + kBarBytes + kXchBytes + kSegTableBytes;
+
+template <bool GATED>
+__global__ void __launch_bounds__(kThreadsBlk, 1)
     blk_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w0,
                     const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ BlkSegs segs,
                     const __grid_constant__ BlkArgs args) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* out_buf = smem + kPStages * kPStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + kPOutBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + kOutBytes);
   uint64_t* empty = full + kPStages;
   uint64_t* accf = empty + kPStages;
   uint64_t* acce = accf + 2;
@@ -305,8 +439,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
   uint64_t* bye = fin + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bye + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* xch = reinterpret_cast<uint32_t*>(out_buf + kPOutBytes + kPBarBytes);
-  const SegTable tab = seg_table_at(out_buf + kPOutBytes + kPBarBytes + kPXchBytes);
+  uint32_t* xch = reinterpret_cast<uint32_t*>(out_buf + kOutBytes + kBarBytes);
+  const SegTable tab = seg_table_at(out_buf + kOutBytes + kBarBytes + kXchBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -315,7 +449,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
   const int pair = blockIdx.x >> 1;
   const int n_pairs = gridDim.x >> 1;
 
-  if (warp == 2) read_segments(segs, tab, kPM, args.status);
+  fetch_segments(segs, tab);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPStages; ++s) {
       mbar_init(&full[s], 1);
@@ -331,10 +465,12 @@ __global__ void __launch_bounds__(kPThreads, 1)
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc_pair(tmem_slot, 2 * kPN);
+    tmem_alloc_pair(tmem_slot, 2 * kN);
     tmem_relinquish_pair();
   }
   tc_fence_before();
+  __syncthreads();
+  if (warp == 2) read_segments(segs, tab, kPM, args.status);
   __syncthreads();
   cluster_sync_all();  // both CTAs' barriers exist before any remote arrive or TMA signal
   tc_fence_after();
@@ -343,7 +479,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
   const int nk = args.k_blk;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsIssue));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
@@ -354,7 +490,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
       for (int tile = pair; tile < total && ok; tile += n_pairs) {
         const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, kPM, tab);
         const int xrow = ti.row0 + (int)rank * 128;
-        const int wrow = GATED ? ti.nt * 128 : ti.nt * kPN + (int)rank * 128;
+        const int wrow = GATED ? ti.nt * 128 : ti.nt * kN + (int)rank * 128;
         const CUtensorMap* tw = (GATED && rank == 1) ? &tm_w1 : &tm_w0;
         for (int kb = 0; kb < nk; ++kb) {
           if (!mbar_wait(&empty[stage], ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_PRODUCER)) {
@@ -365,7 +501,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
           const uint32_t fbar = full_leader0 + (uint32_t)(stage * sizeof(uint64_t));
           if (leader) mbar_arrive_expect_tx(&full[stage], 2 * kPStageBytes);
           tma_load_2d_pair(sx, &tm_x, fbar, kb * kBlk, xrow);
-          tma_load_3d_pair(sx + kPOpBytes, tw, fbar, kb * kBlk, wrow, ti.expert);
+          tma_load_3d_pair(sx + kOpBytes, tw, fbar, kb * kBlk, wrow, ti.expert);
           armed |= 1u << stage;
           armed_ph = (armed_ph & ~(1u << stage)) | (ph << stage);
           if (++stage == kPStages) {
@@ -384,8 +520,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
     // The whole warp walks the steps and one lane issues: with uniform control flow around it an
     // issue takes a fraction of what it does inside a branch of one lane.
     if (leader) {
-      constexpr uint32_t idesc = blk_idesc(kPM, kPN);
-      const uint64_t xd0 = sdesc_sw128(smem_u32(smem)), wd0 = sdesc_sw128(smem_u32(smem + kPOpBytes));
+      constexpr uint32_t idesc = blk_idesc(kPM, kN);
+      const uint64_t xd0 = sdesc_sw128(smem_u32(smem)), wd0 = sdesc_sw128(smem_u32(smem + kOpBytes));
       int stage = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
@@ -400,7 +536,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
             const uint64_t off = (uint64_t)(stage * (kPStageBytes >> 4));
 #pragma unroll
             for (int k = 0; k < 4; ++k)  // 32 codes of K per MMA; the first starts a fresh sum
-              umma_f16_pair<DMOE_E4M3>(tmem_base + (uint32_t)(acc * kPN), xd0 + off + 2 * k, wd0 + off + 2 * k, idesc,
+              umma_f16_pair<DMOE_E4M3>(tmem_base + (uint32_t)(acc * kN), xd0 + off + 2 * k, wd0 + off + 2 * k, idesc,
                                        k != 0);
             umma_commit_both(&empty[stage]);
             umma_commit_both(&accf[acc]);
@@ -422,10 +558,11 @@ __global__ void __launch_bounds__(kPThreads, 1)
   }
   } else {
     // ------------------------------------------------------------------ epilogue (both CTAs)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPRegsSums));
-    const int q = warp & 3;               // TMEM lane quadrant this warp may access
-    const int half = (warp - 4) >> 2;     // its half of the columns
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSums));
+    const int q = warp & 3;  // TMEM lane quadrant this warp may access
+    const int half = (warp - 4) >> 2;
     const uint32_t acce_leader0 = map_to_cta(smem_u32(&acce[0]), 0);
+    uint4* st = reinterpret_cast<uint4*>(out_buf + (warp - 4) * 32 * 128);
     int acc = 0, flip = 0;
     uint32_t acc_ph = 0;
     bool ok = true;
@@ -433,127 +570,31 @@ __global__ void __launch_bounds__(kPThreads, 1)
       const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, kPM, tab);
       const int row = ti.row0 + (int)rank * 128 + q * 32 + lane;
       const bool valid = row < ti.row_end;
-      const float* xs = args.xs + (int64_t)(valid ? row : ti.row0) * args.xs_ld;
-      // Weight scales: gated, of this column block of both stacks; plain, of this half's block
-      // (the last tile's second half may lie past the last block: its sums are never stored).
-      const int nb = GATED ? ti.nt : min(ti.nt * 2 + half, args.n_blk - 1);
-      const int64_t wat = ((int64_t)ti.expert * args.n_blk + nb) * args.k_blk;
+      StepScales sc;
+      sc.start<GATED>(args, ti, row, valid, half, 0);
       uint64_t sum[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) sum[i] = 0;
-      float x_next = __ldg(xs), w0_next = __ldg(args.ws0 + wat), w1_next = GATED ? __ldg(args.ws1 + wat) : 0.f;
       for (int kb = 0; kb < nk && ok; ++kb) {
-        const float s0 = x_next * w0_next, s1 = GATED ? x_next * w1_next : s0;
-        if (kb + 1 < nk) {
-          x_next = __ldg(xs + kb + 1);
-          w0_next = __ldg(args.ws0 + wat + kb + 1);
-          if constexpr (GATED) w1_next = __ldg(args.ws1 + wat + kb + 1);
-        }
+        float s0, s1;
+        sc.take<GATED>(kb, nk, s0, s1);
         ok = wait_in_line(&accf[acc], acc_ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_EPILOGUE);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kPN);
-        const uint64_t s0p = pack_f2(s0, s0), s1p = pack_f2(s1, s1);
-        uint32_t v[2][32];  // the next 32 columns come while these are added
-        tmem_ld32_start(tbase + (GATED ? half * 64 : half * 128), v[0]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          tmem_ld32_finish(v[j & 1]);
-          if (j < 3) {
-            const int n = j + 1;
-            const int col = GATED ? (n < 2 ? half * 64 + n * 32 : 128 + half * 64 + (n - 2) * 32) : half * 128 + n * 32;
-            tmem_ld32_start(tbase + col, v[n & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_remote(acce_leader0 + (uint32_t)(acc * sizeof(uint64_t)));
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) fma2(sum[j * 16 + i], v[j & 1][2 * i], v[j & 1][2 * i + 1], j < 2 ? s0p : s1p);
-        }
+        add_step<GATED>(sum, tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN), half, s0, s1, [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(acce_leader0 + (uint32_t)(acc * sizeof(uint64_t)));
+        });
         acc ^= 1;
         if (acc == 0) acc_ph ^= 1u;
       }
-      // The results go through shared memory, so that a store instruction writes runs of 64 or 128
-      // bytes of a few rows rather than 16 bytes of 32: 6,300 cycles a tile before, at 256 columns
-      // of bf16.  After a wait that ran out nothing is stored, but the warps that share a quadrant
-      // still meet.
-      uint4* st = reinterpret_cast<uint4*>(out_buf + (warp - 4) * 32 * 128);
-      if constexpr (GATED) {
-        float h[64];
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float2 g = unpack_f2(sum[i]), u = unpack_f2(sum[32 + i]);
-          h[2 * i] = act_fn(g.x, args.act) * u.x;
-          h[2 * i + 1] = act_fn(g.y, args.act) * u.y;
-          top = max(top, max(finite_abs_bits(h[2 * i]), finite_abs_bits(h[2 * i + 1])));
-        }
-        // The row's other 64 columns are in the warp that shares this quadrant.
-        uint32_t* mine = xch + (flip * 2 + half) * 128 + q * 32 + lane;
-        uint32_t* other = xch + (flip * 2 + (half ^ 1)) * 128 + q * 32 + lane;
-        *mine = top;
-        named_sync(1 + q, 64);
-        top = max(top, *other);
-        const float s = block_scale(__uint_as_float(top));
-        const float inv = 1.f / s;
-        if (half == 0 && valid && ok) args.out_scale[(int64_t)row * args.os_ld + ti.nt] = s;
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          st[lane * 4 + (v ^ ((lane >> 1) & 3))] = make_uint4(codes4(h + v * 16, inv), codes4(h + v * 16 + 4, inv),
-                                                              codes4(h + v * 16 + 8, inv), codes4(h + v * 16 + 12, inv));
-        __syncwarp();
-        const int col = ti.nt * 128 + half * 64 + (lane & 3) * 16;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i * 8 + (lane >> 2);
-          const uint4 v = st[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
-          const int64_t orow = row - lane + r;
-          if (ok && orow < ti.row_end && col < args.n_out)
-            *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(args.out) + orow * args.ldo + col) = v;
-        }
-        __syncwarp();
-      } else {
-        const int esz = args.out_dtype == DMOE_F32 ? 4 : 2;
-        const int col0 = ti.nt * kPN + half * 128;
-        char* const dst = valid && ok ? blk_out_row(args, row, esz) : nullptr;
-        const int vec = 16 / esz;  // columns of 16 bytes
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {  // 32 columns a thread; 128 bytes of each row at a time
-          const bool f32 = args.out_dtype == DMOE_F32;
-          if (f32) {
-#pragma unroll
-            for (int v = 0; v < 8; ++v) {
-              const float2 a = unpack_f2(sum[p * 16 + 2 * v]), b = unpack_f2(sum[p * 16 + 2 * v + 1]);
-              st[lane * 8 + (v ^ (lane & 7))] = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x),
-                                                           __float_as_uint(b.y));
-            }
-          } else {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              uint32_t pk[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 a = unpack_f2(sum[p * 16 + 4 * v + i]);
-                pk[i] = args.out_dtype == DMOE_BF16 ? pack2<DMOE_BF16>(a.x, a.y) : pack2<DMOE_F16>(a.x, a.y);
-              }
-              st[lane * 8 + (((p & 1) * 4 + v) ^ (lane & 7))] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            }
-            if ((p & 1) == 0) continue;
-          }
-          __syncwarp();
-          const int col = col0 + (f32 ? p * 32 : (p >> 1) * 64) + (lane & 7) * vec;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3);
-            char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
-            const uint4 v = st[r * 8 + ((lane & 7) ^ (r & 7))];
-            if (to != nullptr && col < args.n_out) *reinterpret_cast<uint4*>(to + (int64_t)col * esz) = v;
-          }
-          __syncwarp();
-        }
-      }
+      // After a wait that ran out nothing is stored, but the warps that share a quadrant still meet.
+      if constexpr (GATED)
+        store_codes(sum, args, row, ti.row_end, ok, ti.nt, half, q, xch + flip * 256, st);
+      else
+        store_rows(sum, args, row, valid && ok, ti.nt, half, st);
     }
   }
 
@@ -570,32 +611,25 @@ __global__ void __launch_bounds__(kPThreads, 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc_pair(tmem_base, 2 * kPN);
+    tmem_dealloc_pair(tmem_base, 2 * kN);
   }
 }
 
-// --------------------------------------------------------------------------- few-rows kernel
-// D[weight row, row of x]: M = 128 weight rows (gated: two MMAs, gate and up rows), N = NT rows
-// of x.  Eight epilogue warps: a thread holds one weight row and half of the tile's rows of x.
-// The scales differ by row of x here, that is by column of D: each warp multiplies its rows'
-// scales by the step's weight scale once (a lane a row) and reads them back from shared memory.
-template <bool GATED, int NT, bool SPLIT>
-struct Few {
-  static constexpr int kA = GATED ? 2 : 1;
-  static constexpr int kHalf = NT / 2;
-  static constexpr int kStageBytes = kA * 128 * kBlk + NT * kBlk;
-  static constexpr int kAccs = 512 / (kA * NT) >= 4 ? 4 : 2;  // TMEM accumulators (of kA x NT columns)
-  static constexpr int kTmemCols = kAccs * kA * NT < 32 ? 32 : kAccs * kA * NT;
-  static constexpr int kBarBytes = 512;
-  static constexpr int kScaleBytes = kEpiWarps * 2 * kA * kHalf * 4;
-  static constexpr int kTopBytes = 2 * 2 * 4 * kHalf * 4;
-  static constexpr int kRedBytes = SPLIT ? kA * NT * 128 * 4 : 0;
-  static constexpr int kFixed = 1024 + kBarBytes + kScaleBytes + kTopBytes + kRedBytes + kSegTableBytes;
-  static constexpr int kFit = (227 * 1024 - kFixed) / kStageBytes;
-  static constexpr int kStages = kFit > 12 ? 12 : kFit;
-  static constexpr int kSmemBytes = kFixed + kStages * kStageBytes;
-  static_assert(kStages >= 3 && kTmemCols <= 512, "few-rows tile does not fit");
-};
+// ----------------------------------------------------------------------------- single-SM kernel
+// Row tiles of tile_m rows (32, 64 or 128) x 256 weight rows.  The MMA's M is 128: the rows past the
+// tile come from whatever lies behind it in shared memory, give rows of D that nobody reads, and
+// the warps of their quadrants only pass the accumulators on.
+// With SPLIT the CTAs of a cluster take parts of the reduction of the same tile; each leaves its sums
+// in its own shared memory (where the operands were) and finishes some of the rows, adding the
+// ranks' sums in order.
+__host__ __device__ constexpr int single_stage_bytes(int tile_m) { return tile_m * kBlk + 2 * kOpBytes; }
+constexpr int kSingleFixed = 1024 + kOutBytes + kBarBytes + kXchBytes + kSegTableBytes;
+__host__ __device__ constexpr int single_stages(int tile_m) {
+  return (227 * 1024 - kSingleFixed) / single_stage_bytes(tile_m);
+}
+static_assert(single_stages(32) <= 8 && single_stages(128) >= 3, "stages of the single-SM kernel");
+// Sums of a split tile, 256 fp32 a row, fit where the operands were.
+static_assert(32 * kN * 4 <= single_stages(32) * single_stage_bytes(32), "sums of 32 rows");
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
@@ -603,31 +637,25 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   return v;
 }
 
-template <bool GATED, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kBlkThreads, 1)
-    blk_few_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w0,
-                   const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ BlkSegs segs,
-                   const __grid_constant__ BlkArgs args, int ranks) {
-  using F = Few<GATED, NT, SPLIT>;
-  constexpr int S = F::kStages, NA = F::kA, HN = F::kHalf, ACCS = F::kAccs;
+template <bool GATED, bool SPLIT>
+__global__ void __launch_bounds__(kThreadsBlk, 1)
+    blk_single_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w0,
+                      const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ BlkSegs segs,
+                      const __grid_constant__ BlkArgs args, const int tile_m, const int stages, const int ranks) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* after = smem + S * F::kStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(after);
-  uint64_t* empty = full + S;
-  uint64_t* accf = empty + S;
-  uint64_t* acce = accf + ACCS;
-  uint64_t* fin = acce + ACCS;
+  // Rows of x first: an MMA reads 128 of them from the start of a stage's tile_m.
+  uint8_t* wbuf = smem + stages * tile_m * kBlk;
+  uint8_t* out_buf = wbuf + stages * 2 * kOpBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(out_buf + kOutBytes);
+  uint64_t* empty = full + 8;
+  uint64_t* accf = empty + 8;
+  uint64_t* acce = accf + 2;
+  uint64_t* fin = acce + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  after += F::kBarBytes;
-  float* red = reinterpret_cast<float*>(after);  // SPLIT: [NA][NT][128] partial sums
-  after += F::kRedBytes;
-  float* scales = reinterpret_cast<float*>(after);  // [warp][2][NA][HN]
-  after += F::kScaleBytes;
-  uint32_t* tops = reinterpret_cast<uint32_t*>(after);  // [2][half][HN][4 quadrants]
-  after += F::kTopBytes;
-  const SegTable tab = seg_table_at(after);
+  uint32_t* xch = reinterpret_cast<uint32_t*>(out_buf + kOutBytes + kBarBytes);
+  const SegTable tab = seg_table_at(out_buf + kOutBytes + kBarBytes + kXchBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -635,13 +663,13 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
   const int group = SPLIT ? (int)blockIdx.x / ranks : (int)blockIdx.x;
   const int n_groups = SPLIT ? (int)gridDim.x / ranks : (int)gridDim.x;
 
-  if (warp == 2) read_segments(segs, tab, NT, args.status);
+  fetch_segments(segs, tab);
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int a = 0; a < ACCS; ++a) {
+    for (int a = 0; a < 2; ++a) {
       mbar_init(&accf[a], 1);
       mbar_init(&acce[a], kEpiWarps);
     }
@@ -650,10 +678,12 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, F::kTmemCols);
+    tmem_alloc(tmem_slot, 2 * kN);
     tmem_relinquish();
   }
   tc_fence_before();
+  __syncthreads();
+  if (warp == 2) read_segments(segs, tab, tile_m, args.status);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
@@ -661,246 +691,183 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
   const int kb0 = SPLIT ? (int)((int64_t)args.k_blk * rank / ranks) : 0;
   const int kb1 = SPLIT ? (int)((int64_t)args.k_blk * (rank + 1) / ranks) : args.k_blk;
 
-  // Every role walks the same tiles; with a split reduction all warps of the cluster's CTAs meet
-  // twice a tile (partial sums written; partial sums read).
-  int stage = 0, acc = 0, flip = 0;
-  uint32_t ph = 0, acc_ph = 0, armed = 0, armed_ph = 0;
-  bool ok = true;
-  const int q = warp & 3, half = (warp - 2) >> 2;
-  for (int tile = group; tile < total; tile += n_groups) {
-    const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, NT, tab);
-    uint64_t sum[NA][HN / 2];  // epilogue: pairs of rows of x
-    if (warp == 0) {
-      // ---------------------------------------------------------------- TMA producer
-      if (lane == 0 && ok) {
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&empty[stage], ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_PRODUCER)) {
-            ok = false;
-            break;
+  // Every role walks the same tiles; with SPLIT all warps of the cluster's CTAs meet twice a tile
+  // (sums written; sums read), which also keeps the next tile's operands off the sums.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    int stage = 0, acc = 0;
+    uint32_t ph = 0, acc_ph = 0, armed = 0, armed_ph = 0;
+    bool ok = true;
+    const uint64_t xd0 = sdesc_sw128(smem_u32(smem)), wd0 = sdesc_sw128(smem_u32(wbuf));
+    for (int tile = group; tile < total; tile += n_groups) {
+      const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
+      if (warp == 0) {
+        // -------------------------------------------------------------- TMA producer
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+          ok = wait_in_line(&empty[stage], ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_PRODUCER);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (elect_one()) {
+            uint8_t* sw = wbuf + stage * 2 * kOpBytes;
+            mbar_arrive_expect_tx(&full[stage], single_stage_bytes(tile_m));
+            if constexpr (GATED) {
+              tma_load_3d(sw, &tm_w0, &full[stage], kb * kBlk, ti.nt * 128, ti.expert);
+              tma_load_3d(sw + kOpBytes, &tm_w1, &full[stage], kb * kBlk, ti.nt * 128, ti.expert);
+            } else {
+              tma_load_3d(sw, &tm_w0, &full[stage], kb * kBlk, ti.nt * kN, ti.expert);
+            }
+            tma_load_2d(smem + stage * tile_m * kBlk, &tm_x, &full[stage], kb * kBlk, ti.row0);
           }
-          uint8_t* sw = smem + stage * F::kStageBytes;
-          mbar_arrive_expect_tx(&full[stage], F::kStageBytes);
-          tma_load_3d(sw, &tm_w0, &full[stage], kb * kBlk, ti.nt * 128, ti.expert);
-          if constexpr (GATED) tma_load_3d(sw + 128 * kBlk, &tm_w1, &full[stage], kb * kBlk, ti.nt * 128, ti.expert);
-          tma_load_2d(sw + NA * 128 * kBlk, &tm_x, &full[stage], kb * kBlk, ti.row0);
+          __syncwarp();
           armed |= 1u << stage;
           armed_ph = (armed_ph & ~(1u << stage)) | (ph << stage);
-          if (++stage == S) {
+          if (++stage == stages) {
             stage = 0;
             ph ^= 1u;
           }
         }
-      }
-    } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMA issuer
-      if (lane == 0 && ok) {
-        constexpr uint32_t idesc = blk_idesc(128, NT);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&full[stage], ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA) ||
-              !mbar_wait(&acce[acc], acc_ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA)) {
-            ok = false;
-            break;
-          }
+      } else if (warp == 1) {
+        // -------------------------------------------------------------- MMA issuer
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+          ok = wait_in_line(&full[stage], ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA) &&
+               wait_in_line(&acce[acc], acc_ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t sw = smem_u32(smem + stage * F::kStageBytes);
-          const uint64_t xd = sdesc_sw128(sw + NA * 128 * kBlk);
-#pragma unroll
-          for (int a = 0; a < NA; ++a) {
-            const uint64_t wd = sdesc_sw128(sw + a * 128 * kBlk);
+          if (elect_one()) {
+            const uint64_t xd = xd0 + (uint64_t)(stage * (tile_m * kBlk >> 4));
+            const uint64_t wd = wd0 + (uint64_t)(stage * (2 * kOpBytes >> 4));
 #pragma unroll
             for (int k = 0; k < 4; ++k)  // 32 codes of K per MMA; the first starts a fresh sum
-              umma_f16<DMOE_E4M3>(tmem_base + (uint32_t)((acc * NA + a) * NT), wd + 2 * k, xd + 2 * k, idesc, k != 0);
+              umma_f16<DMOE_E4M3>(tmem_base + (uint32_t)(acc * kN), xd + 2 * k, wd + 2 * k, blk_idesc(128, kN), k != 0);
+            umma_commit(&empty[stage]);
+            umma_commit(&accf[acc]);
           }
-          umma_commit(&empty[stage]);
-          umma_commit(&accf[acc]);
-          if (++stage == S) {
+          __syncwarp();
+          if (++stage == stages) {
             stage = 0;
             ph ^= 1u;
           }
-          if (++acc == ACCS) {
-            acc = 0;
-            acc_ph ^= 1u;
-          }
+          acc ^= 1;
+          if (acc == 0) acc_ph ^= 1u;
         }
       }
-    } else {
-      // ---------------------------------------------------------------- epilogue: scaled sums
-      constexpr int PL = (HN + 31) / 32;  // rows of x whose scales a lane fetches
-      float* sc = scales + (warp - 2) * 2 * NA * HN;
-      const int64_t wat = ((int64_t)ti.expert * args.n_blk + ti.nt) * args.k_blk;
-      const float* xs[PL];
-#pragma unroll
-      for (int p = 0; p < PL; ++p) {
-        const int row = ti.row0 + half * HN + p * 32 + lane;
-        xs[p] = args.xs + (int64_t)(row < ti.row_end ? row : ti.row0) * args.xs_ld;
-      }
-#pragma unroll
-      for (int a = 0; a < NA; ++a)
-#pragma unroll
-        for (int i = 0; i < HN / 2; ++i) sum[a][i] = 0;
-      float x_next[PL], w0_next = 0.f, w1_next = 0.f;
-#pragma unroll
-      for (int p = 0; p < PL; ++p) x_next[p] = kb0 < kb1 ? __ldg(xs[p] + kb0) : 0.f;
-      if (kb0 < kb1) {
-        w0_next = __ldg(args.ws0 + wat + kb0);
-        if constexpr (GATED) w1_next = __ldg(args.ws1 + wat + kb0);
-      }
-      for (int kb = kb0; kb < kb1 && ok; ++kb) {
-        float* now = sc + (kb & 1) * NA * HN;
-#pragma unroll
-        for (int p = 0; p < PL; ++p) {
-          if (p * 32 + lane < HN) {
-            now[p * 32 + lane] = x_next[p] * w0_next;
-            if constexpr (GATED) now[HN + p * 32 + lane] = x_next[p] * w1_next;
-          }
-        }
-        if (kb + 1 < kb1) {
-#pragma unroll
-          for (int p = 0; p < PL; ++p) x_next[p] = __ldg(xs[p] + kb + 1);
-          w0_next = __ldg(args.ws0 + wat + kb + 1);
-          if constexpr (GATED) w1_next = __ldg(args.ws1 + wat + kb + 1);
-        }
-        ok = wait_in_line(&accf[acc], acc_ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_EPILOGUE);
-        ok = __all_sync(0xffffffffu, ok);  // also orders the scales' stores before their loads
-        if (!ok) break;
+      if constexpr (SPLIT) {
         __syncwarp();
-        tc_fence_after();
-        constexpr int C = HN < 32 ? HN : 32;
-#pragma unroll
-        for (int a = 0; a < NA; ++a) {
-#pragma unroll
-          for (int c = 0; c < HN / C; ++c) {
-            uint32_t v[C];
-            tmem_ld<C>(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((acc * NA + a) * NT + half * HN + c * C), v);
-            if (a == NA - 1 && c == HN / C - 1) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&acce[acc]);
-            }
-            const ulonglong2* s4 = reinterpret_cast<const ulonglong2*>(now + a * HN + c * C);
-#pragma unroll
-            for (int i = 0; i < C / 4; ++i) {
-              const ulonglong2 s = s4[i];
-              fma2(sum[a][c * (C / 2) + 2 * i], v[4 * i], v[4 * i + 1], s.x);
-              fma2(sum[a][c * (C / 2) + 2 * i + 1], v[4 * i + 2], v[4 * i + 3], s.y);
-            }
-          }
-        }
-        if (++acc == ACCS) {
-          acc = 0;
-          acc_ph ^= 1u;
-        }
+        cluster_sync_all();
+        cluster_sync_all();
       }
     }
-
-    // ------------------------------------------------------------------ results of the tile
-    const int ch = q * 32 + lane;  // weight row within the tile
-    const int col = ti.nt * 128 + ch;
-    const int esz = args.out_dtype == DMOE_F32 ? 4 : 2;
-    if constexpr (SPLIT) {
-      if (warp >= 2) {
-#pragma unroll
-        for (int a = 0; a < NA; ++a)
-#pragma unroll
-          for (int i = 0; i < HN / 2; ++i) {
-            const float2 v = unpack_f2(sum[a][i]);
-            red[(a * NT + half * HN + 2 * i) * 128 + ch] = v.x;
-            red[(a * NT + half * HN + 2 * i + 1) * 128 + ch] = v.y;
-          }
-      }
+    // Copies in flight land and MMAs complete before the CTA's shared memory and TMEM go.
+    if (warp == 0 && lane == 0) {
+      for (int s = 0; s < stages; ++s)
+        if (armed >> s & 1u) wait_or_report(&full[s], armed_ph >> s & 1u, args.status);
+    } else if (warp == 1) {
+      if (elect_one()) umma_commit(fin);
       __syncwarp();
-      cluster_sync_all();
-      if (warp >= 2) {
-        // This rank finishes rows rank, rank + ranks, ... of the tile, the two halves in turn.
-        const int rows = min(NT, ti.row_end - ti.row0);
-        const uint32_t red0 = smem_u32(red);
-        for (int t = rank + half * ranks; t < rows; t += 2 * ranks) {
-          float v[NA];
+      if (lane == 0) wait_or_report(fin, 0, args.status);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSums));
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    uint4* st = reinterpret_cast<uint4*>(out_buf + (warp - 4) * 32 * 128);
+    int acc = 0, flip = 0;
+    uint32_t acc_ph = 0;
+    bool ok = true;
+    for (int tile = group; tile < total; tile += n_groups) {
+      const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
+      const int rows = min(tile_m, ti.row_end - ti.row0);
+      const bool active = q * 32 < rows;  // some row of this quadrant belongs to the tile
+      const int row = ti.row0 + q * 32 + lane;
+      const bool valid = q * 32 + lane < rows;
+      StepScales sc;
+      if (active) sc.start<GATED>(args, ti, row, valid, half, kb0);
+      uint64_t sum[64];
 #pragma unroll
-          for (int a = 0; a < NA; ++a) {
-            v[a] = 0.f;
-            for (int r = 0; r < ranks; ++r)
-              v[a] += ld_cluster(map_to_cta(red0 + (uint32_t)(((a * NT + t) * 128 + ch) * 4), (uint32_t)r));
+      for (int i = 0; i < 64; ++i) sum[i] = 0;
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        float s0, s1;
+        if (active) sc.take<GATED>(kb, kb1, s0, s1);
+        ok = wait_in_line(&accf[acc], acc_ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_EPILOGUE);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (active) {
+          tc_fence_after();
+          add_step<GATED>(sum, tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN), half, s0, s1, [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acce[acc]);
+          });
+        } else if (lane == 0) {
+          mbar_arrive(&acce[acc]);
+        }
+        acc ^= 1;
+        if (acc == 0) acc_ph ^= 1u;
+      }
+      // After a wait that ran out nothing is stored, but warps that meet below still do.
+      if constexpr (!SPLIT) {
+        if (active) {
+          if constexpr (GATED)
+            store_codes(sum, args, row, ti.row0 + rows, ok, ti.nt, half, q, xch + flip * 256, st);
+          else
+            store_rows(sum, args, row, valid && ok, ti.nt, half, st);
+        }
+        flip ^= 1;
+      } else {
+        // Sums as [row][256 columns], 16-byte units exchanged within a row against bank conflicts.
+        float4* red = reinterpret_cast<float4*>(smem);
+        if (active) {
+#pragma unroll
+          for (int v = 0; v < 32; ++v) {
+            const float2 x = unpack_f2(sum[2 * v]), y = unpack_f2(sum[2 * v + 1]);
+            const int unit = (tmem_col<GATED>(half, v >> 3) >> 2) + (v & 7);
+            red[(q * 32 + lane) * 64 + (unit ^ (lane & 7))] = make_float4(x.x, x.y, y.x, y.y);
           }
-          const int row = ti.row0 + t;
-          if constexpr (GATED) {
-            const float h = act_fn(v[0], args.act) * v[NA - 1];
-            const uint32_t top = __reduce_max_sync(0xffffffffu, finite_abs_bits(h));
-            uint32_t* at = tops + ((flip * 2 + half) * HN) * 4;
+        }
+        __syncwarp();
+        cluster_sync_all();
+        const uint32_t red0 = smem_u32(smem);
+        auto total_of = [&](int r, int col) {  // the ranks' sums of one element, in order
+          const uint32_t at = red0 + (uint32_t)((r * 64 + ((col >> 2) ^ (r & 7))) * 16 + (col & 3) * 4);
+          float v = 0.f;
+          for (int g = 0; g < ranks; ++g) v += ld_cluster(map_to_cta(at, (uint32_t)g));
+          return v;
+        };
+        const int c = (threadIdx.x - 128) & 127;
+        if constexpr (GATED) {
+          // Rank g finishes rows g, g + ranks, ...; 128 threads a row, one h each.
+          for (int r = rank + half * ranks; r < rows; r += 2 * ranks) {
+            float h = blk_act(total_of(r, c), args.act) * total_of(r, 128 + c);
+            const float top = finite_abs(h);  // non-negative floats order as their bits
+            const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+            uint32_t* at = xch + (flip * 2 + half) * 4;
             flip ^= 1;
-            if (lane == 0) at[q] = top;
+            if (lane == 0) at[q] = most;
             named_sync(1 + half, 128);
             const float s = block_scale(__uint_as_float(max(max(at[0], at[1]), max(at[2], at[3]))));
-            if (col < args.n_out) {
-              const float inv = 1.f / s;
-              const float c = fabsf(h) <= 3.402823466e38f ? h * inv : __int_as_float(0x7fffffff);
-              reinterpret_cast<uint8_t*>(args.out)[(int64_t)row * args.ldo + col] =
-                  __nv_cvt_float_to_fp8(c, __NV_SATFINITE, __NV_E4M3);
-            }
-            if (ch == 0) args.out_scale[(int64_t)row * args.os_ld + ti.nt] = s;
-          } else {
-            char* dst = blk_out_row(args, row, esz);
-            if (dst != nullptr && col < args.n_out) store_from_float(dst, col, v[0], args.out_dtype);
+            if (fabsf(h) > kFinite) h = __int_as_float(0x7fffffff);
+            const int col = ti.nt * 128 + c;
+            if (ok && col < args.n_out)
+              reinterpret_cast<uint8_t*>(args.out)[(int64_t)(ti.row0 + r) * args.ldo + col] =
+                  __nv_cvt_float_to_fp8(h * __frcp_rn(s), __NV_SATFINITE, __NV_E4M3);
+            if (ok && c == 0) args.out_scale[(int64_t)(ti.row0 + r) * args.os_ld + ti.nt] = s;
+          }
+        } else {
+          const int esz = args.out_dtype == DMOE_F32 ? 4 : 2;
+          const int col = ti.nt * kN + half * 128 + c;
+          for (int r = rank; r < rows; r += ranks) {
+            const float v = total_of(r, half * 128 + c);
+            char* dst = blk_out_row(args, ti.row0 + r, esz);
+            if (ok && dst != nullptr && col < args.n_out) store_from_float(dst, col, v, args.out_dtype);
           }
         }
-      }
-      __syncwarp();
-      cluster_sync_all();
-    } else if (warp >= 2) {
-      // After a wait that ran out nothing is stored, but the warps of a half still meet.
-      const int rows = ok ? min(HN, ti.row_end - ti.row0 - half * HN) : 0;
-      const int row0 = ti.row0 + half * HN;
-      if constexpr (GATED) {
-        uint32_t* at = tops + ((flip * 2 + half) * HN) * 4;
-        flip ^= 1;
-        float h[HN];
-#pragma unroll
-        for (int i = 0; i < HN / 2; ++i) {
-          const float2 g = unpack_f2(sum[0][i]), u = unpack_f2(sum[NA - 1][i]);
-          h[2 * i] = act_fn(g.x, args.act) * u.x;
-          h[2 * i + 1] = act_fn(g.y, args.act) * u.y;
-        }
-#pragma unroll
-        for (int t = 0; t < HN; ++t) {
-          const uint32_t top = __reduce_max_sync(0xffffffffu, finite_abs_bits(h[t]));
-          if (lane == 0) at[t * 4 + q] = top;
-        }
-        named_sync(1 + half, 128);
-#pragma unroll
-        for (int t = 0; t < HN; ++t) {
-          if (t < rows) {
-            const uint4 m = *reinterpret_cast<const uint4*>(at + t * 4);
-            const float s = block_scale(__uint_as_float(max(max(m.x, m.y), max(m.z, m.w))));
-            const int row = row0 + t;
-            if (col < args.n_out) {
-              const float inv = 1.f / s;
-              const float c = fabsf(h[t]) <= 3.402823466e38f ? h[t] * inv : __int_as_float(0x7fffffff);
-              reinterpret_cast<uint8_t*>(args.out)[(int64_t)row * args.ldo + col] =
-                  __nv_cvt_float_to_fp8(c, __NV_SATFINITE, __NV_E4M3);
-            }
-            if (ch == 0) args.out_scale[(int64_t)row * args.os_ld + ti.nt] = s;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < HN; ++t) {
-          if (t < rows) {
-            const float2 v = unpack_f2(sum[0][t / 2]);
-            char* dst = blk_out_row(args, row0 + t, esz);
-            if (dst != nullptr && col < args.n_out) store_from_float(dst, col, t & 1 ? v.y : v.x, args.out_dtype);
-          }
-        }
+        // The next tile's copies write where the sums were read.
+        asm volatile("fence.proxy.async;" ::: "memory");
+        __syncwarp();
+        cluster_sync_all();
       }
     }
-  }
-
-  // Copies in flight land and MMAs complete before the CTA's shared memory and TMEM go.
-  if (warp == 0 && lane == 0) {
-    for (int s = 0; s < S; ++s)
-      if (armed >> s & 1u) wait_or_report(&full[s], armed_ph >> s & 1u, args.status);
-  } else if (warp == 1 && lane == 0) {
-    umma_commit(fin);
-    wait_or_report(fin, 0, args.status);
   }
   if (args.scatter) __threadfence_system();
   tc_fence_before();
@@ -908,7 +875,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem_base, F::kTmemCols);
+    tmem_dealloc(tmem_base, 2 * kN);
   }
 }
 
@@ -955,7 +922,7 @@ int launch_pair(const Product& p, const BlkSegs& segs, int m_tiles, cudaStream_t
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kPThreads);
+  cfg.blockDim = dim3(kThreadsBlk);
   cfg.dynamicSmemBytes = kPSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -979,7 +946,7 @@ int launch_pair(const Product& p, const BlkSegs& segs, int m_tiles, cudaStream_t
   if (GATED)
     if (int e = code_map(&t1, p.w1, 3, p.K, p.N, p.E, p.K, 128)) return e;
   BlkArgs a = p.args;
-  a.n_tiles_n = GATED ? (p.N + 127) / 128 : (p.N + kPN - 1) / kPN;
+  a.n_tiles_n = GATED ? (p.N + 127) / 128 : (p.N + kN - 1) / kN;
   int pairs = max_clusters[dev] - (gemm_sm_reserve() + 1) / 2;
   const int64_t tiles = (int64_t)m_tiles * a.n_tiles_n;
   if (tiles < pairs) pairs = (int)tiles;
@@ -990,30 +957,29 @@ int launch_pair(const Product& p, const BlkSegs& segs, int m_tiles, cudaStream_t
   return DMOE_OK;
 }
 
-template <bool GATED, int NT, bool SPLIT>
-int launch_few(const Product& p, const BlkSegs& segs, int m_tiles, int ranks, cudaStream_t stream) {
-  using F = Few<GATED, NT, SPLIT>;
+template <bool GATED, bool SPLIT>
+int launch_single(const Product& p, const BlkSegs& segs, int tile_m, int m_tiles, int ranks, cudaStream_t stream) {
   static PerDeviceOnce once;
   int dev = 0;
   DMOE_CUDA(cudaGetDevice(&dev));
   const int r = once_per_device(once, dev, [] {
-    DMOE_CUDA(cudaFuncSetAttribute(blk_few_kernel<GATED, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   F::kSmemBytes));
+    DMOE_CUDA(cudaFuncSetAttribute(blk_single_kernel<GATED, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     return DMOE_OK;
   });
   if (r) return r;
   CUtensorMap tx, t0, t1;
-  if (int e = code_map(&tx, p.x, 2, p.K, segs.m_rows, 1, p.x_ld, NT)) return e;
-  if (int e = code_map(&t0, p.w0, 3, p.K, p.N, p.E, p.K, 128)) return e;
+  if (int e = code_map(&tx, p.x, 2, p.K, segs.m_rows, 1, p.x_ld, tile_m)) return e;
+  if (int e = code_map(&t0, p.w0, 3, p.K, p.N, p.E, p.K, GATED ? 128 : kN)) return e;
   t1 = t0;
   if (GATED)
     if (int e = code_map(&t1, p.w1, 3, p.K, p.N, p.E, p.K, 128)) return e;
   BlkArgs a = p.args;
-  a.n_tiles_n = (p.N + 127) / 128;
+  a.n_tiles_n = GATED ? (p.N + 127) / 128 : (p.N + kN - 1) / kN;
   const int64_t tiles = (int64_t)m_tiles * a.n_tiles_n;
   int groups = gemm_usable_sms() / ranks;
   if (tiles < groups) groups = (int)tiles;
   if (groups < 1) groups = 1;
+  const int stages = single_stages(tile_m);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1021,12 +987,12 @@ int launch_few(const Product& p, const BlkSegs& segs, int m_tiles, int ranks, cu
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3(groups * ranks);
-  cfg.blockDim = dim3(kBlkThreads);
-  cfg.dynamicSmemBytes = F::kSmemBytes;
+  cfg.blockDim = dim3(kThreadsBlk);
+  cfg.dynamicSmemBytes = kSingleFixed + stages * single_stage_bytes(tile_m);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = SPLIT ? 1 : 0;
-  DMOE_CUDA(cudaLaunchKernelEx(&cfg, blk_few_kernel<GATED, NT, SPLIT>, tx, t0, t1, segs, a, ranks));
+  DMOE_CUDA(cudaLaunchKernelEx(&cfg, blk_single_kernel<GATED, SPLIT>, tx, t0, t1, segs, a, tile_m, stages, ranks));
   DMOE_LAUNCH_CHECK();
   return DMOE_OK;
 }
@@ -1054,20 +1020,6 @@ int row_tiles(const BlkSegs& segs, int tile_m) {
   return (int)(most < segs.m_rows ? most : segs.m_rows);
 }
 
-template <bool GATED, int NT>
-int run_few(const Product& p, const BlkSegs& segs, int rows, cudaStream_t stream) {
-  const int m_tiles = row_tiles(segs, NT);
-  if constexpr (NT <= 32) {
-    // Few tiles: split the reduction over a cluster of up to 8 SMs, at least 2 steps each.
-    const int used = segs.n_seg < segs.m_rows ? segs.n_seg : segs.m_rows;
-    const int64_t likely = (int64_t)(segs.dev_end ? used * ((rows + NT - 1) / NT) : m_tiles) * ((p.N + 127) / 128);
-    int ranks = 1;
-    while (ranks < 8 && likely * ranks * 2 <= gemm_usable_sms() && p.args.k_blk >= ranks * 4) ranks *= 2;
-    if (ranks > 1) return launch_few<GATED, NT, true>(p, segs, m_tiles, ranks, stream);
-  }
-  return launch_few<GATED, NT, false>(p, segs, m_tiles, 1, stream);
-}
-
 template <bool GATED>
 int run_product(Product& p, const BlkSegs& segs, int hint, cudaStream_t stream) {
   p.args.n_out = p.N;
@@ -1076,11 +1028,20 @@ int run_product(Product& p, const BlkSegs& segs, int hint, cudaStream_t stream) 
   p.args.k_blk = (p.K + kBlk - 1) / kBlk;
   const int rows = expected_rows(segs, hint);
   if (rows > 128) return launch_pair<GATED>(p, segs, row_tiles(segs, kPM), stream);
-  if constexpr (!GATED)
-    if (rows > 64) return run_few<GATED, 128>(p, segs, rows, stream);
-  if (rows > 32) return run_few<GATED, 64>(p, segs, rows, stream);
-  if (rows > 16) return run_few<GATED, 32>(p, segs, rows, stream);
-  return run_few<GATED, 16>(p, segs, rows, stream);
+  // Row tiles with room for segments half again as long as expected: a segment that needs a second
+  // tile reads its weights twice.
+  const int tile_m = rows <= 20 ? 32 : rows <= 40 ? 64 : 128;
+  const int m_tiles = row_tiles(segs, tile_m);
+  const int n_tiles = GATED ? (p.N + 127) / 128 : (p.N + kN - 1) / kN;
+  if (tile_m == 32) {
+    // Few tiles: split the reduction over a cluster of up to 8 SMs, at least 2 steps each.
+    const int used = segs.n_seg < segs.m_rows ? segs.n_seg : segs.m_rows;
+    const int64_t likely = (int64_t)(segs.dev_end ? used * ((rows + tile_m - 1) / tile_m) : m_tiles) * n_tiles;
+    int ranks = 1;
+    while (ranks < 8 && likely * ranks * 2 <= gemm_usable_sms() && p.args.k_blk >= ranks * 4) ranks *= 2;
+    if (ranks > 1) return launch_single<GATED, true>(p, segs, tile_m, m_tiles, ranks, stream);
+  }
+  return launch_single<GATED, false>(p, segs, tile_m, m_tiles, 1, stream);
 }
 
 int fill_blk_segs(const char* name, BlkSegs& s, const int32_t* seg_expert, const int32_t* seg_end, int n_seg,
