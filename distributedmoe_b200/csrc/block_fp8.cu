@@ -176,9 +176,16 @@ __device__ __forceinline__ float2 unpack_f2(uint64_t v) {
 
 constexpr float kFinite = 3.402823466e38f;
 
-// silu(g) or relu(g), the division as a product with the approximate reciprocal (2 ulp).
-__device__ __forceinline__ float blk_act(float g, int act) {
-  return act == DMOE_ACT_SILU ? __fdividef(g, 1.f + __expf(-g)) : fmaxf(g, 0.f);
+// silu(g) = g / (1 + 2^(-g log2 e)) or relu(g), by the two approximate instructions (2 ulp each; a
+// sigmoid below 2^-126 is 0).  Without flushing, the subnormals that cannot matter here cost as many
+// instructions again.
+template <int ACT>
+__device__ __forceinline__ float blk_act(float g) {
+  if constexpr (ACT != DMOE_ACT_SILU) return fmaxf(g, 0.f);
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.442695041f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r;
 }
 
 // Scale of a block with this largest finite magnitude.
@@ -204,20 +211,20 @@ __device__ __forceinline__ char* blk_out_row(const BlkArgs& a, int row, int esz)
   return base == nullptr ? nullptr : base + (int64_t)(code & 0x7ffffff) * a.ldo * esz;
 }
 
-// tmem_ld32 in two halves: the registers hold their values after the second, which waits for every
-// load this warp has started.
-__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&r)[32]) {
+// 32 lanes x 16 fp32 columns in two halves: the registers hold their values after the second, which
+// waits for every load this warp has started.
+__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : DMOE_R8(0), DMOE_R8(8), DMOE_R8(16), DMOE_R8(24)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : DMOE_R8(0), DMOE_R8(8)
       : "r"(taddr)
       : "memory");
 }
 #define BLK_RW8(b) "+r"(r[b + 0]), "+r"(r[b + 1]), "+r"(r[b + 2]), "+r"(r[b + 3]), "+r"(r[b + 4]), "+r"(r[b + 5]), \
                    "+r"(r[b + 6]), "+r"(r[b + 7])
-__device__ __forceinline__ void tmem_ld32_finish(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : BLK_RW8(0), BLK_RW8(8), BLK_RW8(16), BLK_RW8(24)::"memory");
+__device__ __forceinline__ void tmem_ld16_finish(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : BLK_RW8(0), BLK_RW8(8)::"memory");
 }
 #undef BLK_RW8
 
@@ -263,15 +270,15 @@ __device__ __forceinline__ void named_sync(int id, int threads) {
 // hands its own to the other two.
 constexpr int kN = 256;                // weight rows of a tile: gated 128 gate and 128 up rows
 constexpr int kThreadsBlk = 128 + 32 * kEpiWarps;
-constexpr int kRegsIssue = 56, kRegsSums = 224;  // 128 * 56 + 256 * 224 = 384 * 168, the registers at launch
+constexpr int kRegsIssue = 72, kRegsSums = 216;  // 128 * 72 + 256 * 216 = 384 * 168, the registers at launch
 constexpr int kOpBytes = 128 * kBlk;             // one step of 128 operand rows
 constexpr int kBarBytes = 256;
 constexpr int kXchBytes = 2 * 2 * 128 * 4;
 constexpr int kOutBytes = kEpiWarps * 32 * 128;  // 128 bytes of 32 rows for each epilogue warp
 
 template <bool GATED>
-__device__ __forceinline__ int tmem_col(int half, int j) {  // first of the 32 columns of chunk j
-  return GATED ? (j < 2 ? half * 64 + j * 32 : 128 + half * 64 + (j - 2) * 32) : half * 128 + j * 32;
+__device__ __forceinline__ int tmem_col(int half, int j) {  // first of the 16 columns of chunk j
+  return GATED ? (j < 4 ? half * 64 + j * 16 : 128 + half * 64 + (j - 4) * 16) : half * 128 + j * 16;
 }
 
 // Reads back this warp's 32 rows and 128 columns of an accumulator and adds them, scaled; `release`
@@ -279,23 +286,34 @@ __device__ __forceinline__ int tmem_col(int half, int j) {  // first of the 32 c
 template <bool GATED, class F>
 __device__ __forceinline__ void add_step(uint64_t (&sum)[64], uint32_t tbase, int half, float s0, float s1, F&& release) {
   const uint64_t s0p = pack_f2(s0, s0), s1p = pack_f2(s1, s1);
-  uint32_t v[2][32];  // the next 32 columns come while these are added
-  tmem_ld32_start(tbase + tmem_col<GATED>(half, 0), v[0]);
+  uint32_t v[2][16];  // the next 16 columns come while these are added
+  tmem_ld16_start(tbase + tmem_col<GATED>(half, 0), v[0]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    tmem_ld32_finish(v[j & 1]);
-    if (j < 3)
-      tmem_ld32_start(tbase + tmem_col<GATED>(half, j + 1), v[(j + 1) & 1]);
+  for (int j = 0; j < 8; ++j) {
+    tmem_ld16_finish(v[j & 1]);
+    if (j < 7)
+      tmem_ld16_start(tbase + tmem_col<GATED>(half, j + 1), v[(j + 1) & 1]);
     else
       release();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) fma2(sum[j * 16 + i], v[j & 1][2 * i], v[j & 1][2 * i + 1], j < 2 ? s0p : s1p);
+    for (int i = 0; i < 8; ++i) fma2(sum[j * 8 + i], v[j & 1][2 * i], v[j & 1][2 * i + 1], j < 4 ? s0p : s1p);
   }
 }
 
 // Results of a tile, the row `row` in each lane.  They go through shared memory (`st`: this warp's
 // 4 KB), so that a store instruction writes runs of 64 or 128 bytes of a few rows rather than 16
 // bytes of 32: 6,300 cycles a tile before, at 256 columns of bf16.
+
+template <int ACT>
+__device__ __forceinline__ void gated_values(const uint64_t (&sum)[64], float (&h)[64], float& top) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const float2 g = unpack_f2(sum[i]), u = unpack_f2(sum[32 + i]);
+    h[2 * i] = blk_act<ACT>(g.x) * u.x;
+    h[2 * i + 1] = blk_act<ACT>(g.y) * u.y;
+    top = fmaxf(top, fmaxf(fabsf(h[2 * i]), fabsf(h[2 * i + 1])));
+  }
+}
 
 // h = act(gate) * up as codes, with the scale of the row's 128 columns; the other 64 of them are in
 // the warp that shares this quadrant (`xch`: both warps' largest magnitudes).
@@ -304,13 +322,10 @@ __device__ __forceinline__ void store_codes(const uint64_t (&sum)[64], const Blk
   const int lane = threadIdx.x & 31;
   float h[64];
   float top = 0.f;  // fmaxf prefers a number to NaN, so only an infinity shows in it
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const float2 g = unpack_f2(sum[i]), u = unpack_f2(sum[32 + i]);
-    h[2 * i] = blk_act(g.x, a.act) * u.x;
-    h[2 * i + 1] = blk_act(g.y, a.act) * u.y;
-    top = fmaxf(top, fmaxf(fabsf(h[2 * i]), fabsf(h[2 * i + 1])));
-  }
+  if (a.act == DMOE_ACT_SILU)
+    gated_values<DMOE_ACT_SILU>(sum, h, top);
+  else
+    gated_values<DMOE_ACT_RELU>(sum, h, top);
   if (top > kFinite) {  // infinities become NaN codes and leave the scale alone
     top = 0.f;
 #pragma unroll
@@ -821,7 +836,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
 #pragma unroll
           for (int v = 0; v < 32; ++v) {
             const float2 x = unpack_f2(sum[2 * v]), y = unpack_f2(sum[2 * v + 1]);
-            const int unit = (tmem_col<GATED>(half, v >> 3) >> 2) + (v & 7);
+            const int unit = (tmem_col<GATED>(half, v >> 2) >> 2) + (v & 3);
             red[(q * 32 + lane) * 64 + (unit ^ (lane & 7))] = make_float4(x.x, x.y, y.x, y.y);
           }
         }
@@ -838,7 +853,8 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
         if constexpr (GATED) {
           // Rank g finishes rows g, g + ranks, ...; 128 threads a row, one h each.
           for (int r = rank + half * ranks; r < rows; r += 2 * ranks) {
-            float h = blk_act(total_of(r, c), args.act) * total_of(r, 128 + c);
+            const float g = total_of(r, c);
+            float h = (args.act == DMOE_ACT_SILU ? blk_act<DMOE_ACT_SILU>(g) : blk_act<DMOE_ACT_RELU>(g)) * total_of(r, 128 + c);
             const float top = finite_abs(h);  // non-negative floats order as their bits
             const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
             uint32_t* at = xch + (flip * 2 + half) * 4;
