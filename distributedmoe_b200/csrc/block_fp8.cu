@@ -259,6 +259,12 @@ __device__ __forceinline__ void wait_or_report(uint64_t* bar, uint32_t parity, i
   }
 }
 
+// Programmatic dependent launch: a product starts while the kernel before it in the stream drains,
+// sets itself up, and waits here for that kernel's results.  The next kernel may be launched once
+// every CTA has passed its own wait.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -464,7 +470,6 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
   const int pair = blockIdx.x >> 1;
   const int n_pairs = gridDim.x >> 1;
 
-  fetch_segments(segs, tab);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPStages; ++s) {
       mbar_init(&full[s], 1);
@@ -483,6 +488,9 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     tmem_alloc_pair(tmem_slot, 2 * kN);
     tmem_relinquish_pair();
   }
+  wait_for_previous_kernel();
+  let_next_kernel_start();
+  fetch_segments(segs, tab);
   tc_fence_before();
   __syncthreads();
   if (warp == 2) read_segments(segs, tab, kPM, args.status);
@@ -644,7 +652,10 @@ __host__ __device__ constexpr int single_stages(int tile_m) {
 }
 static_assert(single_stages(32) <= 8 && single_stages(128) >= 3, "stages of the single-SM kernel");
 // Sums of a split tile, 256 fp32 a row, fit where the operands were.
-static_assert(32 * kN * 4 <= single_stages(32) * single_stage_bytes(32), "sums of 32 rows");
+static_assert(32 * kN * 4 <= single_stages(32) * single_stage_bytes(32) &&
+                  64 * kN * 4 <= single_stages(64) * single_stage_bytes(64) &&
+                  128 * kN * 4 <= single_stages(128) * single_stage_bytes(128),
+              "sums of a split tile");
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
@@ -678,7 +689,6 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
   const int group = SPLIT ? (int)blockIdx.x / ranks : (int)blockIdx.x;
   const int n_groups = SPLIT ? (int)gridDim.x / ranks : (int)gridDim.x;
 
-  fetch_segments(segs, tab);
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
@@ -696,6 +706,9 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     tmem_alloc(tmem_slot, 2 * kN);
     tmem_relinquish();
   }
+  wait_for_previous_kernel();
+  let_next_kernel_start();
+  fetch_segments(segs, tab);
   tc_fence_before();
   __syncthreads();
   if (warp == 2) read_segments(segs, tab, tile_m, args.status);
@@ -926,6 +939,11 @@ struct Product {
 };
 
 template <bool GATED>
+int n_tiles_of(int N) {
+  return GATED ? (N + 127) / 128 : (N + kN - 1) / kN;
+}
+
+template <bool GATED>
 int launch_pair(const Product& p, const BlkSegs& segs, int m_tiles, cudaStream_t stream) {
   static PerDeviceOnce once;
   static int max_clusters[64];
@@ -933,16 +951,18 @@ int launch_pair(const Product& p, const BlkSegs& segs, int m_tiles, cudaStream_t
   DMOE_CUDA(cudaGetDevice(&dev));
   DMOE_REQUIRE(dev >= 0 && dev < 64, "block-scaled product: device index %d out of range", dev);
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kThreadsBlk);
   cfg.dynamicSmemBytes = kPSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const int r = once_per_device(once, dev, [&] {
     DMOE_CUDA(cudaFuncSetAttribute(blk_pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmemBytes));
     cfg.gridDim = dim3(2 * 74);
@@ -962,7 +982,7 @@ int launch_pair(const Product& p, const BlkSegs& segs, int m_tiles, cudaStream_t
   if (GATED)
     if (int e = code_map(&t1, p.w1, 3, p.K, p.N, p.E, p.K, 128)) return e;
   BlkArgs a = p.args;
-  a.n_tiles_n = GATED ? (p.N + 127) / 128 : (p.N + kN - 1) / kN;
+  a.n_tiles_n = n_tiles_of<GATED>(p.N);
   int pairs = max_clusters[dev] - (gemm_sm_reserve() + 1) / 2;
   const int64_t tiles = (int64_t)m_tiles * a.n_tiles_n;
   if (tiles < pairs) pairs = (int)tiles;
@@ -971,6 +991,39 @@ int launch_pair(const Product& p, const BlkSegs& segs, int m_tiles, cudaStream_t
   DMOE_CUDA(cudaLaunchKernelEx(&cfg, blk_pair_kernel<GATED>, tx, t0, t1, segs, a));
   DMOE_LAUNCH_CHECK();
   return DMOE_OK;
+}
+
+// Clusters of `ranks` CTAs of the single-SM kernel that fit on the device at once.
+template <bool GATED>
+int max_split_clusters(int dev, int ranks, int* out) {
+  static PerDeviceOnce once;
+  static int fit[64][9];
+  DMOE_REQUIRE(dev >= 0 && dev < 64, "block-scaled product: device index %d out of range", dev);
+  const int r = once_per_device(once, dev, [&] {
+    DMOE_CUDA(cudaFuncSetAttribute(blk_single_kernel<GATED, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    for (int n = 2; n <= 8; ++n) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = n;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3(n * 74);
+      cfg.blockDim = dim3(kThreadsBlk);
+      cfg.dynamicSmemBytes = kSingleFixed + single_stages(32) * single_stage_bytes(32);
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int got = 0;
+      if (cudaOccupancyMaxActiveClusters(&got, blk_single_kernel<GATED, true>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        got = 0;
+      }
+      fit[dev][n] = got;
+    }
+    return DMOE_OK;
+  });
+  *out = r == DMOE_OK ? fit[dev][ranks] : 0;
+  return r;
 }
 
 template <bool GATED, bool SPLIT>
@@ -990,24 +1043,26 @@ int launch_single(const Product& p, const BlkSegs& segs, int tile_m, int m_tiles
   if (GATED)
     if (int e = code_map(&t1, p.w1, 3, p.K, p.N, p.E, p.K, 128)) return e;
   BlkArgs a = p.args;
-  a.n_tiles_n = GATED ? (p.N + 127) / 128 : (p.N + kN - 1) / kN;
+  a.n_tiles_n = n_tiles_of<GATED>(p.N);
   const int64_t tiles = (int64_t)m_tiles * a.n_tiles_n;
   int groups = gemm_usable_sms() / ranks;
   if (tiles < groups) groups = (int)tiles;
   if (groups < 1) groups = 1;
   const int stages = single_stages(tile_m);
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ranks;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3(groups * ranks);
   cfg.blockDim = dim3(kThreadsBlk);
   cfg.dynamicSmemBytes = kSingleFixed + stages * single_stage_bytes(tile_m);
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = SPLIT ? 1 : 0;
+  cfg.numAttrs = SPLIT ? 2 : 1;
   DMOE_CUDA(cudaLaunchKernelEx(&cfg, blk_single_kernel<GATED, SPLIT>, tx, t0, t1, segs, a, tile_m, stages, ranks));
   DMOE_LAUNCH_CHECK();
   return DMOE_OK;
@@ -1043,20 +1098,35 @@ int run_product(Product& p, const BlkSegs& segs, int hint, cudaStream_t stream) 
   p.args.n_blk = (p.N + kBlk - 1) / kBlk;
   p.args.k_blk = (p.K + kBlk - 1) / kBlk;
   const int rows = expected_rows(segs, hint);
-  if (rows > 128) return launch_pair<GATED>(p, segs, row_tiles(segs, kPM), stream);
-  // Row tiles with room for segments half again as long as expected: a segment that needs a second
-  // tile reads its weights twice.
+  const int n_tiles = n_tiles_of<GATED>(p.N);
+  const int used = segs.n_seg < segs.m_rows ? segs.n_seg : segs.m_rows;
+  // Row tiles of the single-SM kernel: room for segments half again as long as expected, since a
+  // segment that needs a second tile reads its weights twice.
   const int tile_m = rows <= 20 ? 32 : rows <= 40 ? 64 : 128;
   const int m_tiles = row_tiles(segs, tile_m);
-  const int n_tiles = GATED ? (p.N + 127) / 128 : (p.N + kN - 1) / kN;
-  if (tile_m == 32) {
-    // Few tiles: split the reduction over a cluster of up to 8 SMs, at least 2 steps each.
-    const int used = segs.n_seg < segs.m_rows ? segs.n_seg : segs.m_rows;
-    const int64_t likely = (int64_t)(segs.dev_end ? used * ((rows + tile_m - 1) / tile_m) : m_tiles) * n_tiles;
-    int ranks = 1;
-    while (ranks < 8 && likely * ranks * 2 <= gemm_usable_sms() && p.args.k_blk >= ranks * 4) ranks *= 2;
-    if (ranks > 1) return launch_single<GATED, true>(p, segs, tile_m, m_tiles, ranks, stream);
+  const int64_t likely = (int64_t)(segs.dev_end ? used * ((rows + tile_m - 1) / tile_m) : m_tiles) * n_tiles;
+  const int sms = gemm_usable_sms();
+  if (likely * 2 <= sms) {
+    // Few tiles: split the reduction over as many SMs of a cluster as leave all clusters room at
+    // once, at least two steps each.
+    int dev = 0, ranks = (int)(sms / likely);
+    DMOE_CUDA(cudaGetDevice(&dev));
+    if (ranks > 8) ranks = 8;
+    if (ranks > p.args.k_blk / 2) ranks = p.args.k_blk / 2;
+    for (; ranks > 1; --ranks) {
+      int fit = 0;
+      if (int r = max_split_clusters<GATED>(dev, ranks, &fit)) return r;
+      if (fit >= likely) return launch_single<GATED, true>(p, segs, tile_m, m_tiles, ranks, stream);
+    }
   }
+  // Rows that the tiles of each kernel cover, the padding of each segment's last tile included (half
+  // a tile on average where the table is not at hand).  A pair does a row in about 0.93 of the time
+  // of a single SM twice: 4096 x 14336 x 4096 in 223 us against 238, 8192 x 8192 x 8192 in 549
+  // against 611; on ragged segments the finer tiles win (32 of 256 rows on average at 2048 x 7168: 172 us
+  // against 184).
+  const int64_t by_pair = segs.dev_end ? (int64_t)(rows + kPM / 2) * used : (int64_t)row_tiles(segs, kPM) * kPM;
+  const int64_t by_single = segs.dev_end ? (int64_t)(rows + 64) * used : (int64_t)row_tiles(segs, 128) * 128;
+  if (tile_m == 128 && by_pair * 93 < by_single * 100) return launch_pair<GATED>(p, segs, row_tiles(segs, kPM), stream);
   return launch_single<GATED, false>(p, segs, tile_m, m_tiles, 1, stream);
 }
 

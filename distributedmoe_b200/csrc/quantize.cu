@@ -178,6 +178,8 @@ template <int DT>
 __global__ void __launch_bounds__(kQuantWarps * 32)
     quantize_row_blocks_kernel(const void* __restrict__ x, int64_t rows, int cols, uint8_t* __restrict__ q,
                                int64_t q_ld, float* __restrict__ scale, int64_t scale_ld) {
+  // The product that follows may set itself up meanwhile; it waits for this kernel's end.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
