@@ -62,6 +62,10 @@ struct BlkArgs {
   // plain only: store row r at scatter_base[code >> 27] + (code & 0x7ffffff) rows with
   // code = scatter_map[r] (negative: not stored) instead of at row r of `out`; the bases may be
   // other GPUs' memory.
+  // The kernel before this one in the stream is the gate/up product of the same call: it writes
+  // nothing but this one's x and its scales, so the weights and the segment table are read before
+  // it has ended (it waited for its own predecessors before it let this one start).
+  int early;
   int scatter;
   const int32_t* scatter_map;
   char* scatter_base[DMOE_EP_MAX_RANKS];
@@ -89,55 +93,44 @@ __device__ __forceinline__ void fetch_segments(const BlkSegs& segs, const SegTab
   }
 }
 
-// ... and one warp makes tiles of it, 32 segments at a time: ends are clamped to [previous end,
-// m_rows] (reported in *status where that changes one), entries outside the stack are left out.
+// ... and one warp makes tiles of it, a run of segments in each lane: ends are clamped to [previous
+// end, m_rows] (reported in *status where that changes one), entries outside the stack are left out.
 __device__ __forceinline__ void read_segments(const BlkSegs& segs, const SegTable& t, int tile_m, int32_t* status) {
   const int lane = threadIdx.x & 31;
   const int n = segs.n_seg;
-  int prev = 0, tiles = 0, bad = 0;
-  for (int base = 0; base < n; base += 32) {
-    const int i = base + lane;
-    int en = 0, e = -1;
-    if (i < n) {
-      en = t.end[i];
-      e = t.expert[i];
-    }
-    const int given = en;
-    en = min(max(en, 0), segs.m_rows);
-    if (i >= n) en = 0;
-    int top = en;  // running maximum of the ends up to this one
+  const int run = (n + 31) >> 5;
+  const int i0 = min(lane * run, n), i1 = min(i0 + run, n);
+  int top = 0;  // running maximum of the clamped ends, over this lane's run, then over those before
+  for (int i = i0; i < i1; ++i) top = max(top, min(t.end[i], segs.m_rows));
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, top, o);
-      if (lane >= o) top = max(top, v);
-    }
-    top = max(top, prev);
-    int first = __shfl_up_sync(0xffffffffu, top, 1);
-    if (lane == 0) first = prev;
-    if (i < n && given != top) bad = 1;
-    int len = i < n ? top - first : 0;
-    if (i < n && (e < 0 || e >= segs.e_stack)) {
-      bad = 1;
-      len = 0;
-      e = 0;
-    }
-    const int mine = (len + tile_m - 1) / tile_m;
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += v;
-    }
-    if (i < n) {
-      t.start[i] = first;
-      t.end[i] = first + len;
-      t.expert[i] = e;
-      t.tile[i] = tiles + sum - mine;
-    }
-    tiles += __shfl_sync(0xffffffffu, sum, 31);
-    prev = __shfl_sync(0xffffffffu, top, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, top, o);
+    if (lane >= o) top = max(top, v);
   }
-  if (lane == 0) t.tile[n] = tiles;
+  int prev = __shfl_up_sync(0xffffffffu, top, 1);
+  if (lane == 0) prev = 0;
+  int tiles = 0, bad = 0;
+  for (int i = i0; i < i1; ++i) {
+    const int given = t.end[i], e = t.expert[i];
+    const int en = max(min(given, segs.m_rows), prev);
+    const bool in_stack = e >= 0 && e < segs.e_stack;
+    bad |= given != en || !in_stack;
+    t.start[i] = prev;
+    t.end[i] = in_stack ? en : prev;
+    t.expert[i] = in_stack ? e : 0;
+    t.tile[i] = tiles;
+    if (in_stack) tiles += (en - prev + tile_m - 1) / tile_m;
+    prev = en;
+  }
+  int before = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
+  }
+  if (lane == 31) t.tile[n] = before;
+  before -= tiles;
+  for (int i = i0; i < i1; ++i) t.tile[i] += before;
   if (__any_sync(0xffffffffu, bad) && lane == 0 && blockIdx.x == 0) atomicOr(status, DMOE_DEVERR_BAD_SEGMENT);
 }
 
@@ -250,6 +243,7 @@ __device__ __forceinline__ bool wait_in_line(uint64_t* bar, uint32_t parity, vol
 }
 
 __device__ __forceinline__ void wait_or_report(uint64_t* bar, uint32_t parity, int32_t* status) {
+  if (mbar_try_wait(bar, parity)) return;
   const uint64_t t0 = global_timer_ns();
   while (!mbar_try_wait(bar, parity)) {
     if (global_timer_ns() - t0 > kWaitTimeoutNs) {
@@ -470,6 +464,10 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
   const int pair = blockIdx.x >> 1;
   const int n_pairs = gridDim.x >> 1;
 
+  if (threadIdx.x == 64) {
+    tma_prefetch_map(&tm_x);
+    tma_prefetch_map(GATED && rank == 1 ? &tm_w1 : &tm_w0);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPStages; ++s) {
       mbar_init(&full[s], 1);
@@ -689,6 +687,11 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
   const int group = SPLIT ? (int)blockIdx.x / ranks : (int)blockIdx.x;
   const int n_groups = SPLIT ? (int)gridDim.x / ranks : (int)gridDim.x;
 
+  if (threadIdx.x == 64) {
+    tma_prefetch_map(&tm_w0);
+    if (GATED) tma_prefetch_map(&tm_w1);
+    tma_prefetch_map(&tm_x);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
@@ -706,8 +709,11 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     tmem_alloc(tmem_slot, 2 * kN);
     tmem_relinquish();
   }
-  wait_for_previous_kernel();
-  let_next_kernel_start();
+  const bool early = !GATED && args.early;
+  if (!early) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+  }
   fetch_segments(segs, tab);
   tc_fence_before();
   __syncthreads();
@@ -727,6 +733,28 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     uint32_t ph = 0, acc_ph = 0, armed = 0, armed_ph = 0;
     bool ok = true;
     const uint64_t xd0 = sdesc_sw128(smem_u32(smem)), wd0 = sdesc_sw128(smem_u32(wbuf));
+    auto load_w = [&](const BlkTile& ti, int kb, int at) {
+      uint8_t* sw = wbuf + at * 2 * kOpBytes;
+      mbar_arrive_expect_tx(&full[at], single_stage_bytes(tile_m));
+      if constexpr (GATED) {
+        tma_load_3d(sw, &tm_w0, &full[at], kb * kBlk, ti.nt * 128, ti.expert);
+        tma_load_3d(sw + kOpBytes, &tm_w1, &full[at], kb * kBlk, ti.nt * 128, ti.expert);
+      } else {
+        tma_load_3d(sw, &tm_w0, &full[at], kb * kBlk, ti.nt * kN, ti.expert);
+      }
+    };
+    int ahead = 0;  // steps of the first tile whose weights were asked for early
+    if (early && warp == 0) {
+      if (group < total) {
+        const BlkTile ti = blk_tile(group, args.n_tiles_n, segs.n_seg, tile_m, tab);
+        ahead = min(stages, kb1 - kb0);
+        if (elect_one())
+          for (int i = 0; i < ahead; ++i) load_w(ti, kb0 + i, i);
+        __syncwarp();
+      }
+      wait_for_previous_kernel();
+      let_next_kernel_start();
+    }
     for (int tile = group; tile < total; tile += n_groups) {
       const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
       if (warp == 0) {
@@ -736,17 +764,11 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (elect_one()) {
-            uint8_t* sw = wbuf + stage * 2 * kOpBytes;
-            mbar_arrive_expect_tx(&full[stage], single_stage_bytes(tile_m));
-            if constexpr (GATED) {
-              tma_load_3d(sw, &tm_w0, &full[stage], kb * kBlk, ti.nt * 128, ti.expert);
-              tma_load_3d(sw + kOpBytes, &tm_w1, &full[stage], kb * kBlk, ti.nt * 128, ti.expert);
-            } else {
-              tma_load_3d(sw, &tm_w0, &full[stage], kb * kBlk, ti.nt * kN, ti.expert);
-            }
+            if (ahead == 0) load_w(ti, kb, stage);
             tma_load_2d(smem + stage * tile_m * kBlk, &tm_x, &full[stage], kb * kBlk, ti.row0);
           }
           __syncwarp();
+          if (ahead > 0) --ahead;
           armed |= 1u << stage;
           armed_ph = (armed_ph & ~(1u << stage)) | (ph << stage);
           if (++stage == stages) {
@@ -786,18 +808,25 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
         cluster_sync_all();
       }
     }
-    // Copies in flight land and MMAs complete before the CTA's shared memory and TMEM go.
-    if (warp == 0 && lane == 0) {
-      for (int s = 0; s < stages; ++s)
-        if (armed >> s & 1u) wait_or_report(&full[s], armed_ph >> s & 1u, args.status);
-    } else if (warp == 1) {
-      if (elect_one()) umma_commit(fin);
-      __syncwarp();
-      if (lane == 0) wait_or_report(fin, 0, args.status);
+    // The epilogue has waited for every step's MMAs, and those for every copy, unless some wait ran
+    // out: then copies in flight land and MMAs complete before the CTA's shared memory and TMEM go.
+    named_sync(7, kThreadsBlk);
+    if (*abort_flag) {
+      if (warp == 0 && lane == 0) {
+        for (int s = 0; s < stages; ++s)
+          if (armed >> s & 1u) wait_or_report(&full[s], armed_ph >> s & 1u, args.status);
+      } else if (warp == 1) {
+        if (elect_one()) {
+          umma_commit(fin);
+          wait_or_report(fin, 0, args.status);
+        }
+        __syncwarp();
+      }
     }
   } else {
     // ------------------------------------------------------------------ epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSums));
+    if (early) wait_for_previous_kernel();
     const int q = warp & 3, half = (warp - 4) >> 2;
     uint4* st = reinterpret_cast<uint4*>(out_buf + (warp - 4) * 32 * 128);
     int acc = 0, flip = 0;
@@ -845,7 +874,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
       } else {
         // Sums as [row][256 columns], 16-byte units exchanged within a row against bank conflicts.
         float4* red = reinterpret_cast<float4*>(smem);
-        if (active) {
+        if (valid) {
 #pragma unroll
           for (int v = 0; v < 32; ++v) {
             const float2 x = unpack_f2(sum[2 * v]), y = unpack_f2(sum[2 * v + 1]);
@@ -858,8 +887,11 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
         const uint32_t red0 = smem_u32(smem);
         auto total_of = [&](int r, int col) {  // the ranks' sums of one element, in order
           const uint32_t at = red0 + (uint32_t)((r * 64 + ((col >> 2) ^ (r & 7))) * 16 + (col & 3) * 4);
-          float v = 0.f;
-          for (int g = 0; g < ranks; ++g) v += ld_cluster(map_to_cta(at, (uint32_t)g));
+          float part[8], v = 0.f;
+#pragma unroll
+          for (int g = 0; g < 8; ++g) part[g] = g < ranks ? ld_cluster(map_to_cta(at, (uint32_t)g)) : 0.f;
+#pragma unroll
+          for (int g = 0; g < 8; ++g) v += part[g];
           return v;
         };
         const int c = (threadIdx.x - 128) & 127;
@@ -897,6 +929,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
         cluster_sync_all();
       }
     }
+    named_sync(7, kThreadsBlk);
   }
   if (args.scatter) __threadfence_system();
   tc_fence_before();
@@ -1183,6 +1216,7 @@ int run_blk_mlp(const void* x, int64_t x_ld, const float* xs, int64_t xs_ld, con
   dn.args.xs_ld = blocks_of(I);
   dn.args.ws0 = ds;
   dn.args.out = Y;
+  dn.args.early = 1;
   dn.args.ldo = d;
   dn.args.out_dtype = DMOE_BF16;
   dn.args.status = status;
