@@ -8,7 +8,6 @@ sizes and the current CUDA stream; the kernels run inside the library.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -220,27 +219,37 @@ def _require_cuda(*ts: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
-def _one_device(*ts: Optional[torch.Tensor]) -> torch.device:
-    """The one CUDA device of these tensors."""
-    dev = None
+def _one_device(*ts: Optional[torch.Tensor]) -> int:
+    """Index of the one CUDA device of these tensors."""
+    dev = -1
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()
+        if i < 0:
             raise DMoEError("dmoe kernels take CUDA tensors only (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise DMoEError(f"tensors on different devices: {dev} and {t.device}")
+        if i != dev:
+            if dev >= 0:
+                raise DMoEError(f"tensors on different devices: cuda:{dev} and cuda:{i}")
+            dev = i
     return dev
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(dev: torch.device):
-    """Make `dev` current for a launch (its streams belong to it)."""
-    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+def _call(dev: int, name: str, fn, *args) -> None:
+    """One library call on the current stream of device `dev` (which is its last argument), with
+    that device current."""
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return _call(dev, name, fn, *args)
+    st = torch._C._cuda_getCurrentRawStream(dev)
+    if _timing is not None:
+        tm = _Timed(name, st, torch.device("cuda", dev))
+        _check(fn(*args, st), "dmoe_" + name)
+        tm.done()
+    else:
+        rc = fn(*args, st)
+        if rc:
+            _check(rc, "dmoe_" + name)
 
 
 # ----------------------------------------------------------------------------- scratch
@@ -631,67 +640,89 @@ def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Te
     scale = max(amax / 448, 2^-126), 1 for an all-zero block; codes = e4m3(x / scale), the quotient
     rounded to fp32 first.  A value that is not finite becomes a NaN code and leaves the scale of
     its block alone."""
-    dev = _require_cuda(x)
-    if block_rows not in (1, FP8_BLOCK):
-        raise DMoEError(f"block_rows={block_rows}: 1 or {FP8_BLOCK}")
-    if x.dim() < (1 if block_rows == 1 else 2) or x.shape[-1] == 0 or x.shape[-1] % 16:
+    dev = _one_device(x)
+    if not x.is_contiguous():
+        raise DMoEError("dmoe kernels take contiguous tensors")
+    shape = x.shape
+    cols = shape[-1] if shape else 0
+    if cols == 0 or cols % 16:
         raise DMoEError("x must be [..., cols] ([..., rows, cols] for 128 x 128 blocks) with cols a multiple of 16")
-    cols = x.shape[-1]
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    nb = _blocks(cols)
     if block_rows == 1:
         batch, rows = 1, x.numel() // cols
-        scale = torch.empty(*x.shape[:-1], _blocks(cols), dtype=torch.float32, device=dev)
-    else:
-        rows = x.shape[-2]
+        s_shape = (*shape[:-1], nb)
+    elif block_rows == FP8_BLOCK and len(shape) >= 2:
+        rows = shape[-2]
         batch = x.numel() // (rows * cols) if rows else 0
-        scale = torch.empty(*x.shape[:-2], _blocks(rows), _blocks(cols), dtype=torch.float32, device=dev)
-    with _on(dev):
-        st = _stream(dev)
-        tm = _Timed("quantize_blocks_e4m3", st, dev)
-        rc = lib().dmoe_quantize_blocks_e4m3(x.data_ptr(), dtype_code(x.dtype), batch, rows, cols, block_rows,
-                                             q.data_ptr(), cols, scale.data_ptr(), _blocks(cols), st)
-        _check(rc, "dmoe_quantize_blocks_e4m3")
-        tm.done()
+        s_shape = (*shape[:-2], _blocks(rows), nb)
+    else:
+        raise DMoEError(f"block_rows={block_rows}: 1, or {FP8_BLOCK} for x [..., rows, cols]")
+    code = dtype_code(x.dtype)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(s_shape, dtype=torch.float32, device=x.device)
+    _call(dev, "quantize_blocks_e4m3", lib().dmoe_quantize_blocks_e4m3, x.data_ptr(), code, batch, rows, cols,
+          block_rows, q.data_ptr(), cols, scale.data_ptr(), nb)
     return q, scale
 
 
-def _check_weight_blocks(q: torch.Tensor, scale: torch.Tensor, what: str) -> None:
-    if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.float32:
+def _check_weight_blocks(q: torch.Tensor, scale: torch.Tensor, shape: Sequence[int], what: str) -> None:
+    """A stack q of this shape [E, N, K] (or [N, K]) and its scales."""
+    if q.dtype is not torch.float8_e4m3fn or scale.dtype is not torch.float32:
         raise DMoEError(f"{what} must be float8_e4m3fn with fp32 scales")
-    if q.dim() != 3 or scale.shape != (q.shape[0], _blocks(q.shape[1]), _blocks(q.shape[2])):
-        raise DMoEError(f"{what} must be [E, N, K] with scales [E, ceil(N / 128), ceil(K / 128)]")
+    if scale.shape != (*shape[:-2], -(-shape[-2] // FP8_BLOCK), -(-shape[-1] // FP8_BLOCK)):
+        raise DMoEError(f"{what} must be [..., N, K] with scales [..., ceil(N / 128), ceil(K / 128)]")
     if not (q.is_contiguous() and scale.is_contiguous()):
         raise DMoEError("dmoe kernels take contiguous weights")
 
 
-def _check_row_blocks(xq: torch.Tensor, x_scale: torch.Tensor, K: int) -> Tuple[int, int]:
-    """Row strides (bytes, floats) of 2-D codes and scales of K columns; rows may be strided."""
-    if xq.dtype != torch.float8_e4m3fn or x_scale.dtype != torch.float32:
+def _check_row_blocks(xq: torch.Tensor, x_scale: torch.Tensor, K: int) -> Tuple[int, int, int]:
+    """Rows, and their strides (bytes, floats), of 2-D codes and scales of K columns."""
+    if xq.dtype is not torch.float8_e4m3fn or x_scale.dtype is not torch.float32:
         raise DMoEError("xq must be float8_e4m3fn with fp32 scales")
-    if xq.dim() != 2 or xq.shape[1] != K or x_scale.shape != (xq.shape[0], _blocks(K)):
-        raise DMoEError(f"xq must be [rows, {K}] with scales [rows, {_blocks(K)}]")
-    if (K > 1 and xq.stride(1) != 1) or (_blocks(K) > 1 and x_scale.stride(1) != 1):
+    shape, nb = xq.shape, -(-K // FP8_BLOCK)
+    if len(shape) != 2 or shape[1] != K or x_scale.shape != (shape[0], nb):
+        raise DMoEError(f"xq must be [rows, {K}] with scales [rows, {nb}]")
+    a, b = xq.stride(), x_scale.stride()
+    if (K > 1 and a[1] != 1) or (nb > 1 and b[1] != 1):
         raise DMoEError("the columns of xq and of its scales must be contiguous")
-    if xq.shape[0] < 2:
-        return K, _blocks(K)
-    return xq.stride(0), x_scale.stride(0)
+    return (shape[0], a[0], b[0]) if shape[0] > 1 else (shape[0], K, nb)
 
 
-def _segments(seg_expert, seg_end, dev: torch.device):
+def _segments(seg_expert, seg_end, dev: int):
     """(expert pointer, end pointer, count, on device, what to keep alive) of a segment table."""
-    if isinstance(seg_expert, torch.Tensor) or isinstance(seg_end, torch.Tensor):
-        if not (isinstance(seg_expert, torch.Tensor) and isinstance(seg_end, torch.Tensor)):
-            raise DMoEError("a segment table is two int32 CUDA tensors or two sequences of numbers")
-        if seg_expert.dtype != torch.int32 or seg_end.dtype != torch.int32 or seg_expert.dim() != 1 \
+    if isinstance(seg_expert, torch.Tensor) and isinstance(seg_end, torch.Tensor):
+        if seg_expert.dtype is not torch.int32 or seg_end.dtype is not torch.int32 or seg_expert.dim() != 1 \
                 or seg_expert.shape != seg_end.shape or not (seg_expert.is_contiguous() and seg_end.is_contiguous()):
             raise DMoEError("a segment table on the device is two contiguous int32 tensors of one length")
-        if seg_expert.device != dev or seg_end.device != dev:
-            raise DMoEError(f"the segment table must be on {dev}")
+        if seg_expert.get_device() != dev or seg_end.get_device() != dev:
+            raise DMoEError(f"the segment table must be on cuda:{dev}")
         return seg_expert.data_ptr(), seg_end.data_ptr(), seg_expert.numel(), 1, None
-    if len(seg_expert) != len(seg_end):
+    if isinstance(seg_expert, torch.Tensor) or isinstance(seg_end, torch.Tensor):
+        raise DMoEError("a segment table is two int32 CUDA tensors or two sequences of numbers")
+    n = len(seg_expert)
+    if n != len(seg_end):
         raise DMoEError("seg_expert and seg_end differ in length")
     a1, a2 = _i32_array(seg_expert), _i32_array(seg_end)
-    return ctypes.addressof(a1), ctypes.addressof(a2), len(seg_expert), 0, (a1, a2)
+    return ctypes.addressof(a1), ctypes.addressof(a2), n, 0, (a1, a2)
+
+
+def _product(xq, x_scale, w_q, w_scale, w_shape, E, seg_expert, seg_end, out, out_dtype, rows_hint) -> torch.Tensor:
+    dev = _one_device(xq, x_scale, w_q, w_scale, out)
+    _check_weight_blocks(w_q, w_scale, w_shape, "w_q")
+    Nn, K = w_shape[-2:]
+    m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, K)
+    if out is None:
+        out = torch.empty((m, Nn), dtype=out_dtype or torch.bfloat16, device=xq.device)
+        y_ld = Nn
+    else:
+        if out.shape != (m, Nn) or (Nn > 1 and out.stride(1) != 1) or (out_dtype is not None and out.dtype != out_dtype):
+            raise DMoEError(f"out must be [{m}, {Nn}] with contiguous columns, in out_dtype where that is given")
+        y_ld = out.stride(0) if m > 1 else Nn
+    se, sn, n_seg, on_dev, _keep = _segments(seg_expert, seg_end, dev)
+    _call(dev, "grouped_matmul_fp8_blocks", lib().dmoe_grouped_matmul_fp8_blocks, xq.data_ptr(), x_ld,
+          x_scale.data_ptr(), xs_ld, w_q.data_ptr(), w_scale.data_ptr(), E, Nn, K, se, sn, n_seg, on_dev, m,
+          int(rows_hint), out.data_ptr(), y_ld, dtype_code(out.dtype), scratch.status(xq.device).data_ptr())
+    return out
 
 
 def grouped_matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
@@ -706,39 +737,20 @@ def grouped_matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torc
     f16 or f32; bf16 if not said); rows outside the segments are not written.  rows_hint: rows
     expected per segment where that is not rows / segments (a capacity-sized buffer); it only picks
     the tile shape."""
-    dev = _one_device(xq, x_scale, w_q, w_scale, out)
-    _check_weight_blocks(w_q, w_scale, "w_q")
-    E, Nn, K = w_q.shape
-    x_ld, xs_ld = _check_row_blocks(xq, x_scale, K)
-    m = xq.shape[0]
-    if out is None:
-        out = torch.empty(m, Nn, dtype=out_dtype or torch.bfloat16, device=dev)
-    elif out.dim() != 2 or out.shape != (m, Nn) or (Nn > 1 and out.stride(1) != 1) or \
-            (out_dtype is not None and out.dtype != out_dtype):
-        raise DMoEError(f"out must be [{m}, {Nn}] with contiguous columns, in out_dtype where that is given")
-    y_ld = out.stride(0) if m > 1 else Nn
-    se, sn, n_seg, on_dev, keep = _segments(seg_expert, seg_end, dev)
-    with _on(dev):
-        st = _stream(dev)
-        tm = _Timed("grouped_matmul_fp8_blocks", st, dev)
-        rc = lib().dmoe_grouped_matmul_fp8_blocks(xq.data_ptr(), x_ld, x_scale.data_ptr(), xs_ld, w_q.data_ptr(),
-                                                  w_scale.data_ptr(), E, Nn, K, se, sn, n_seg, on_dev, m,
-                                                  int(rows_hint), out.data_ptr(), y_ld, dtype_code(out.dtype),
-                                                  scratch.status(dev).data_ptr(), st)
-        del keep
-        _check(rc, "dmoe_grouped_matmul_fp8_blocks")
-        tm.done()
-    return out
+    shape = w_q.shape
+    if len(shape) != 3:
+        raise DMoEError("w_q must be [E, N, K]")
+    return _product(xq, x_scale, w_q, w_scale, shape, shape[0], seg_expert, seg_end, out, out_dtype, rows_hint)
 
 
 def matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
                       out: Optional[torch.Tensor] = None, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """xq [rows, K] times the transpose of w_q [N, K], both e4m3 with fp32 scales for each 1 x 128
     and 128 x 128 block: :func:`grouped_matmul_fp8_blocks` with one segment."""
-    if w_q.dim() != 2 or w_scale.dim() != 2:
-        raise DMoEError("w_q must be [N, K] with scales [ceil(N / 128), ceil(K / 128)]")
-    return grouped_matmul_fp8_blocks(xq, x_scale, w_q.unsqueeze(0), w_scale.unsqueeze(0), (0,), (xq.shape[0],), out,
-                                     out_dtype=out_dtype)
+    shape = w_q.shape
+    if len(shape) != 2:
+        raise DMoEError("w_q must be [N, K]")
+    return _product(xq, x_scale, w_q, w_scale, shape, 1, (0,), (xq.shape[0],), out, out_dtype, 0)
 
 
 class Fp8BlockExperts:
@@ -760,17 +772,20 @@ class Fp8BlockExperts:
         return self
 
     def _set(self, wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale) -> None:
-        self.device = _one_device(wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale)
-        _check_weight_blocks(wg_q, wg_scale, "gate")
-        _check_weight_blocks(wu_q, wu_scale, "up")
-        _check_weight_blocks(wd_q, wd_scale, "down")
-        E, I, d = wg_q.shape
-        if wu_q.shape != (E, I, d) or wd_q.shape != (E, d, I):
+        self.dev = _one_device(wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale)
+        shape = wg_q.shape
+        if len(shape) != 3 or wu_q.shape != shape or wd_q.shape != (shape[0], shape[2], shape[1]):
             raise DMoEError("expert stacks must be gate/up [E, I, d] and down [E, d, I]")
+        E, I, d = shape
         if d % 16 or I % 16:
             raise DMoEError(f"8-bit experts need d % 16 == 0 and I % 16 == 0 (d={d}, I={I})")
+        _check_weight_blocks(wg_q, wg_scale, shape, "gate")
+        _check_weight_blocks(wu_q, wu_scale, shape, "up")
+        _check_weight_blocks(wd_q, wd_scale, (E, d, I), "down")
         self.wg_q, self.wg_scale, self.wu_q, self.wu_scale = wg_q, wg_scale, wu_q, wu_scale
         self.wd_q, self.wd_scale = wd_q, wd_scale
+        self._ptrs = (wg_q.data_ptr(), wg_scale.data_ptr(), wu_q.data_ptr(), wu_scale.data_ptr(), wd_q.data_ptr(),
+                      wd_scale.data_ptr(), E, d, I)
 
     @property
     def shape(self):
@@ -785,50 +800,39 @@ def grouped_gated_mlp_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, expert
     (rows may be strided); segments and rows_hint as :func:`grouped_matmul_fp8_blocks`; rows outside
     the segments are not written.  Returns Y [rows, d] (a new tensor if not given)."""
     dev = _one_device(xq, x_scale, experts.wg_q, Y)
-    E, I, d = experts.wg_q.shape
-    x_ld, xs_ld = _check_row_blocks(xq, x_scale, d)
-    m = xq.shape[0]
+    d, I = experts._ptrs[-2:]
+    m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, d)
     if Y is None:
-        Y = torch.empty(m, d, dtype=torch.bfloat16, device=dev)
+        Y = torch.empty((m, d), dtype=torch.bfloat16, device=xq.device)
     elif Y.dtype != torch.bfloat16 or Y.shape != (m, d) or not Y.is_contiguous():
         raise DMoEError(f"Y must be a contiguous bf16 [{m}, {d}] tensor")
-    ws = torch.empty(lib().dmoe_grouped_mlp_fp8_blocks_workspace_size(m, I), dtype=torch.uint8, device=dev)
-    se, sn, n_seg, on_dev, keep = _segments(seg_expert, seg_end, dev)
-    with _on(dev):
-        st = _stream(dev)
-        tm = _Timed("grouped_gated_mlp_fp8_blocks", st, dev)
-        rc = lib().dmoe_grouped_gated_mlp_fp8_blocks(
-            xq.data_ptr(), x_ld, x_scale.data_ptr(), xs_ld, experts.wg_q.data_ptr(), experts.wg_scale.data_ptr(),
-            experts.wu_q.data_ptr(), experts.wu_scale.data_ptr(), experts.wd_q.data_ptr(), experts.wd_scale.data_ptr(),
-            E, d, I, se, sn, n_seg, on_dev, m, int(rows_hint), int(act), Y.data_ptr(), ws.data_ptr(), ws.numel(),
-            scratch.status(dev).data_ptr(), st)
-        del keep
-        _check(rc, "dmoe_grouped_gated_mlp_fp8_blocks")
-        tm.done()
+    nbytes = lib().dmoe_grouped_mlp_fp8_blocks_workspace_size(m, I)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=xq.device)
+    se, sn, n_seg, on_dev, _keep = _segments(seg_expert, seg_end, dev)
+    _call(dev, "grouped_gated_mlp_fp8_blocks", lib().dmoe_grouped_gated_mlp_fp8_blocks, xq.data_ptr(), x_ld,
+          x_scale.data_ptr(), xs_ld, *experts._ptrs, se, sn, n_seg, on_dev, m, int(rows_hint), int(act), Y.data_ptr(),
+          ws.data_ptr(), nbytes, scratch.status(xq.device).data_ptr())
     return Y
 
 
 # ----------------------------------------------------------------------------- balance loss
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, idx, mode, seq_end, mask):
-        dev = logits.device
+    def forward(ctx, logits, idx, mode, seq_end, mask, dev):
+        device = logits.device
         T, E = logits.shape
         k = idx.shape[1]
         S = 1 if seq_end is None else seq_end.numel()
-        counts = torch.empty(S * (E + 1) + 1, dtype=torch.int32, device=dev)
-        loss = torch.empty(2, dtype=torch.float32, device=dev)
-        ws = torch.empty(lib().dmoe_balance_loss_workspace_size(), dtype=torch.uint8, device=dev)
-        with _on(dev):
-            st = _stream(dev)
-            tm = _Timed("balance_loss", st, dev)
-            rc = lib().dmoe_balance_loss(logits.data_ptr(), dtype_code(logits.dtype), idx.data_ptr(), T, E, k, mode,
-                                         _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), loss.data_ptr(),
-                                         ws.data_ptr(), ws.numel(), scratch.status(dev).data_ptr(), st)
-            _check(rc, "dmoe_balance_loss")
-            tm.done()
+        code = dtype_code(logits.dtype)
+        counts = torch.empty(S * (E + 1) + 1, dtype=torch.int32, device=device)
+        loss = torch.empty(2, dtype=torch.float32, device=device)
+        nbytes = lib().dmoe_balance_loss_workspace_size()
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _call(dev, "balance_loss", lib().dmoe_balance_loss, logits.data_ptr(), code, idx.data_ptr(), T, E, k, mode,
+              _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes,
+              scratch.status(device).data_ptr())
         ctx.save_for_backward(logits, seq_end, mask, counts)
-        ctx.args = (T, E, k, mode, S)
+        ctx.args = (dev, code, T, E, k, mode, S)
         ctx.set_materialize_grads(False)
         per_expert = counts.as_strided((S, E), (E, 1))
         ctx.mark_non_differentiable(per_expert)
@@ -839,20 +843,13 @@ class _BalanceLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_balance, g_z, _counts):
         if g_balance is None and g_z is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
         logits, seq_end, mask, counts = ctx.saved_tensors
-        T, E, k, mode, S = ctx.args
-        dev = logits.device
+        dev, code, T, E, k, mode, S = ctx.args
         grad = torch.empty_like(logits)
-        with _on(dev):
-            st = _stream(dev)
-            tm = _Timed("balance_loss_backward", st, dev)
-            rc = lib().dmoe_balance_loss_backward(logits.data_ptr(), dtype_code(logits.dtype), T, E, k, mode,
-                                                  _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), _ptr(g_balance),
-                                                  _ptr(g_z), grad.data_ptr(), st)
-            _check(rc, "dmoe_balance_loss_backward")
-            tm.done()
-        return grad, None, None, None, None
+        _call(dev, "balance_loss_backward", lib().dmoe_balance_loss_backward, logits.data_ptr(), code, T, E, k, mode,
+              _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), _ptr(g_balance), _ptr(g_z), grad.data_ptr())
+        return grad, None, None, None, None, None
 
 
 def balance_loss(logits: torch.Tensor, idx: torch.Tensor, *, mode: int = ROUTER_SOFTMAX,
@@ -871,15 +868,16 @@ def balance_loss(logits: torch.Tensor, idx: torch.Tensor, *, mode: int = ROUTER_
     autograd function, a backward pass is captured into a CUDA graph only once earlier eager graphs
     of the same leaf are dropped (torch raises otherwise)."""
     dev = _one_device(logits, idx, seq_end, mask)
-    _require_cuda(logits, idx, seq_end, mask)
+    for t in (logits, idx, seq_end, mask):
+        if t is not None and not t.is_contiguous():
+            raise DMoEError("dmoe kernels take contiguous tensors")
     if logits.dim() != 2 or idx.dim() != 2 or idx.shape[0] != logits.shape[0] or idx.dtype != torch.int64:
         raise DMoEError("logits must be [T, E] and the selected experts int64 [T, k]")
-    dtype_code(logits.dtype)
     if seq_end is not None and (seq_end.dtype != torch.int32 or seq_end.dim() != 1):
         raise DMoEError("seq_end must be an int32 vector")
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != logits.shape[:1]):
         raise DMoEError("mask must be bool [T]")
-    return _BalanceLoss.apply(logits, idx, int(mode), seq_end, mask)
+    return _BalanceLoss.apply(logits, idx, int(mode), seq_end, mask, dev)
 
 
 def set_gemm_sm_reserve(sms: int) -> None:
