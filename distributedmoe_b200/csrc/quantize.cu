@@ -122,14 +122,6 @@ namespace {
 
 constexpr float kFiniteMax = 3.402823466e38f;
 
-// Largest magnitude; fmaxf prefers a number to NaN, so only an infinity shows in it.
-__device__ __forceinline__ float abs_max8(const float* f) {
-  float m = fabsf(f[0]);
-#pragma unroll
-  for (int i = 1; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
-  return fmaxf(m, 0.f);
-}
-
 __device__ __forceinline__ float finite_max8(const float* f) {
   float m = 0.f;
 #pragma unroll
@@ -171,8 +163,56 @@ __device__ __forceinline__ uint2 codes8(const float* f, float s, float inv, bool
 }
 constexpr float kFastScale = 8.0779357e-28f;  // 2^-90
 
-// 1 x 128: a warp takes kRowCols consecutive columns of one row, two blocks per load.
-constexpr int kRowCols = 1024;
+// Eight neighbouring values as they lie in memory (a 16-bit value widened early would take twice the
+// registers), their largest magnitude and the values as numbers.
+template <int DT>
+struct Raw8 {
+  static constexpr int kVecs = DT == DMOE_F32 ? 2 : 1;
+  // Magnitudes order as their bits; from this one on they are not finite.
+  static constexpr uint32_t kInf = DT == DMOE_F32 ? 0x7f800000u : (DT == DMOE_BF16 ? 0x7f80u : 0x7c00u);
+  uint4 v[kVecs];
+  __device__ __forceinline__ void load(const void* base, int64_t i) {
+    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(base) + i * (DT == DMOE_F32 ? 4 : 2));
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) v[j] = __ldcs(p + j);  // read once
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) v[j] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void numbers(float* f) const {
+    if constexpr (DT == DMOE_F32) {
+      const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+    } else {
+      unpack8<DT>(v[0], f);
+    }
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (DT == DMOE_F32) {
+      const uint32_t m = 0x7fffffffu;
+      const uint4 a = v[0], b = v[1];
+      return max(max(max(a.x & m, a.y & m), max(a.z & m, a.w & m)), max(max(b.x & m, b.y & m), max(b.z & m, b.w & m)));
+    } else {
+      const uint32_t m = 0x7fff7fffu;
+      const uint32_t t = __vmaxu2(__vmaxu2(v[0].x & m, v[0].y & m), __vmaxu2(v[0].z & m, v[0].w & m));
+      return max(t & 0xffffu, t >> 16);
+    }
+  }
+  static __device__ __forceinline__ float value(uint32_t bits) {
+    if constexpr (DT == DMOE_F32) return __uint_as_float(bits);
+    if constexpr (DT == DMOE_BF16) return __uint_as_float(bits << 16);
+    return __half2float(__ushort_as_half((unsigned short)bits));
+  }
+};
+
+// 1 x 128: a warp takes kRowLoads x 256 consecutive columns of one row, two blocks per load, with all
+// its loads in flight at once.  A scale costs two divisions, some 35 instructions: lane i of each
+// half-warp does those of load i and hands them round, rather than all lanes for every load (8192 x
+// 7168 bf16: 44 us so).
+template <int DT>
+constexpr int kRowLoads = DT == DMOE_F32 ? 4 : 8;
 
 template <int DT>
 __global__ void __launch_bounds__(kQuantWarps * 32)
@@ -180,37 +220,53 @@ __global__ void __launch_bounds__(kQuantWarps * 32)
                                int64_t q_ld, float* __restrict__ scale, int64_t scale_ld) {
   // The product that follows may set itself up meanwhile; it waits for this kernel's end.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31;
+  constexpr int NL = kRowLoads<DT>;
+  const int lane = threadIdx.x & 31, at = lane & 15;
   const int64_t row = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const int c0 = blockIdx.y * kRowCols + lane * 8;
-  float f[4][8];
+  const int c0 = blockIdx.y * (NL * 256) + lane * 8;
+  Raw8<DT> raw[NL];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = c0 + i * 256;
-    if (c < cols) {
-      load8<DT>(x, row * cols + c, f[i]);
-    } else {
+  for (int i = 0; i < NL; ++i) {
+    if (c0 + i * 256 < cols)
+      raw[i].load(x, row * cols + c0 + i * 256);
+    else
+      raw[i].clear();
+  }
+  uint32_t bits = 0;  // of the block whose scale this lane makes
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
+  for (int i = 0; i < NL; ++i) {
+    uint32_t t = raw[i].top();
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+    if (at == i) bits = t;
+  }
+  const bool finite = bits < Raw8<DT>::kInf;
+  float m = Raw8<DT>::value(bits);
+  if (!__all_sync(0xffffffffu, finite)) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      float f[8];
+      raw[i].numbers(f);
+      float t = finite_max8(f);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+      if (at == i) m = t;
     }
   }
+  const float s = scale_of(m), inv = __frcp_rn(s);
+  const uint32_t fast = __ballot_sync(0xffffffffu, finite && s >= kFastScale);
+  const int block = blockIdx.y * (NL * 2) + at * 2 + (lane >> 4);
+  if (at < NL && block * 128 < cols) scale[row * scale_ld + block] = s;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NL; ++i) {
+    const int from = (lane & 16) | i;
+    const float si = __shfl_sync(0xffffffffu, s, from), ri = __shfl_sync(0xffffffffu, inv, from);
     const int c = c0 + i * 256;
-    float m = abs_max8(f[i]);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const bool infinite = m > kFiniteMax;
-    if (__any_sync(0xffffffffu, infinite)) {
-      m = finite_max8(f[i]);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    }
-    const float s = scale_of(m);
     if (c < cols) {
-      if ((lane & 15) == 0) scale[row * scale_ld + (c >> 7)] = s;
-      *reinterpret_cast<uint2*>(q + row * q_ld + c) = codes8(f[i], s, __frcp_rn(s), !infinite && s >= kFastScale);
+      float f[8];
+      raw[i].numbers(f);
+      *reinterpret_cast<uint2*>(q + row * q_ld + c) = codes8(f, si, ri, fast >> from & 1u);
     }
   }
 }
@@ -220,7 +276,7 @@ template <int DT>
 __global__ void __launch_bounds__(256)
     quantize_square_blocks_kernel(const void* __restrict__ x, int64_t rows, int cols, int col_blocks,
                                   int64_t row_blocks, uint8_t* __restrict__ q, float* __restrict__ scale) {
-  __shared__ float tops[8];
+  __shared__ uint32_t tops[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t rb_all = blockIdx.x / col_blocks;  // row block within the whole batch
   const int cb = (int)(blockIdx.x - rb_all * col_blocks);
@@ -228,39 +284,52 @@ __global__ void __launch_bounds__(256)
   const int64_t r0 = (rb_all - mat * row_blocks) * 128 + warp * 2 + (lane >> 4);
   const int c = cb * 128 + (lane & 15) * 8;
   const int64_t base = mat * rows * cols;
-  float f[8][8];
-  float m = 0.f;
+  Raw8<DT> raw[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t r = r0 + i * 16;
-    if (r < rows && c < cols) {
-      load8<DT>(x, base + r * cols + c, f[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
-    }
+    if (r < rows && c < cols)
+      raw[i].load(x, base + r * cols + c);
+    else
+      raw[i].clear();
   }
+  uint32_t bits = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, abs_max8(f[i]));
-  const bool infinite = __syncthreads_or(m > kFiniteMax);
-  if (infinite) {
-    m = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_max8(f[i]));
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) tops[warp] = m;
+  for (int i = 0; i < 8; ++i) bits = max(bits, raw[i].top());
+  bits = __reduce_max_sync(0xffffffffu, bits);
+  if (lane == 0) tops[warp] = bits;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, tops[w]);
+  for (int w = 0; w < 8; ++w) bits = max(bits, tops[w]);
+  const bool finite = bits < Raw8<DT>::kInf;  // of the whole block
+  float m = Raw8<DT>::value(bits);
+  if (!finite) {
+    m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float f[8];
+      raw[i].numbers(f);
+      m = fmaxf(m, finite_max8(f));
+    }
+    bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    __syncthreads();
+    if (lane == 0) tops[warp] = bits;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) bits = max(bits, tops[w]);
+    m = __uint_as_float(bits);
+  }
   const float s = scale_of(m), inv = __frcp_rn(s);
-  const bool fast = !infinite && s >= kFastScale;
+  const bool fast = finite && s >= kFastScale;
   if (threadIdx.x == 0) scale[rb_all * col_blocks + cb] = s;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t r = r0 + i * 16;
-    if (r < rows && c < cols) *reinterpret_cast<uint2*>(q + base + r * cols + c) = codes8(f[i], s, inv, fast);
+    if (r < rows && c < cols) {
+      float f[8];
+      raw[i].numbers(f);
+      *reinterpret_cast<uint2*>(q + base + r * cols + c) = codes8(f, s, inv, fast);
+    }
   }
 }
 
@@ -268,7 +337,7 @@ template <int DT>
 int run_quantize_blocks(const void* x, int64_t batch, int64_t rows, int cols, int block_rows, uint8_t* q, int64_t q_ld,
                         float* scale, int64_t scale_ld, cudaStream_t s) {
   if (block_rows == 1) {
-    const int parts = (cols + kRowCols - 1) / kRowCols;
+    const int parts = (cols + kRowLoads<DT> * 256 - 1) / (kRowLoads<DT> * 256);
     const int64_t grid = (batch * rows + kQuantWarps - 1) / kQuantWarps;
     DMOE_REQUIRE(grid <= INT32_MAX && parts <= 65535, "dmoe_quantize_blocks_e4m3: %lld rows of %d", (long long)(batch * rows),
                  cols);
