@@ -840,8 +840,13 @@ class _BalanceLoss(torch.autograd.Function):
         return balance, z, per_expert
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_balance, g_z, _counts):
+        if torch.is_grad_enabled():  # create_graph: the result refuses to be differentiated again
+            return _BalanceLoss._backward_once(ctx, g_balance, g_z)
+        return _BalanceLoss._backward(ctx, g_balance, g_z)
+
+    @staticmethod
+    def _backward(ctx, g_balance, g_z):
         if g_balance is None and g_z is None:
             return None, None, None, None, None, None
         logits, seq_end, mask, counts = ctx.saved_tensors
@@ -850,6 +855,8 @@ class _BalanceLoss(torch.autograd.Function):
         _call(dev, "balance_loss_backward", lib().dmoe_balance_loss_backward, logits.data_ptr(), code, T, E, k, mode,
               _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), _ptr(g_balance), _ptr(g_z), grad.data_ptr())
         return grad, None, None, None, None, None
+
+    _backward_once = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
 
 
 def balance_loss(logits: torch.Tensor, idx: torch.Tensor, *, mode: int = ROUTER_SOFTMAX,

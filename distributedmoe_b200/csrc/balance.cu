@@ -15,19 +15,22 @@
 // Three passes: counts (reads the selections), the losses (reads the logits), the gradient (reads
 // the logits again rather than keeping p: the same bytes as reading a kept p, and none written).
 //
-// p of the sigmoid form is taken relative to the row's largest logit, so that a row whose sigmoids
-// all underflow still has its probabilities.  A row of -inf alone has p = 0, adds nothing to
-// either sum and gets a zero gradient; rows that are masked or belong to no sequence are not read.
+// With e = exp(-|l|) both sigmoid(l) and 1 - sigmoid(l) are 1 or e over 1 + e: one exponential and one
+// reciprocal.  Where every logit of a row is below -40 the sigmoids are taken relative to the
+// largest, so that a row whose sigmoids all underflow still has its probabilities.  A row of -inf
+// alone has p = 0, adds nothing to either sum and gets a zero gradient; rows that are masked or
+// belong to no sequence are not read.
 //
-// A token is spread over G lanes (the power of two that E fills, at most a warp), V logits a lane.
-// Per-token terms are fp32; sums over tokens are kept in double and joined in a fixed order.
+// A token is spread over G lanes (the power of two that E fills, at most a warp), V logits a lane,
+// and the next token's logits are on their way while one is worked on.  Per-token terms are fp32;
+// sums over tokens are kept in double and joined in a fixed order.
 #include "dmoe_common.cuh"
 
 namespace dmoe {
 namespace {
 
 constexpr int kBalThreads = 256;
-constexpr int kMaxGrid = 1024;
+constexpr int kMaxGrid = 1184;  // 148 SMs x 8
 
 struct BalArgs {
   const void* logits;
@@ -38,16 +41,29 @@ struct BalArgs {
   int32_t* counts;      // [n_seq][E], then n [n_seq], then a ticket
 };
 
-__device__ __forceinline__ int seq_end_of(const BalArgs& a, int s) { return a.seq_end ? min(a.seq_end[s], a.T) : a.T; }
-
-// First sequence that ends behind token t (n_seq if none does).
-__device__ __forceinline__ int seq_of(const BalArgs& a, int t) {
-  int lo = 0, hi = a.n_seq;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (seq_end_of(a, mid) > t) hi = mid; else lo = mid + 1;
+// Ends of the sequences in shared memory where they fit: a search through global memory is a chain
+// of loads, 2 us for 37 sequences.
+constexpr int kSharedEnds = 1024;
+struct Ends {
+  const int32_t* at;  // shared or global
+  int n, T;
+  __device__ __forceinline__ int operator[](int s) const { return at ? min(at[s], T) : T; }
+  // First sequence that ends behind token t (n if none does).
+  __device__ __forceinline__ int of(int t) const {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if ((*this)[mid] > t) hi = mid; else lo = mid + 1;
+    }
+    return lo;
   }
-  return lo;
+};
+
+// `sh`: kSharedEnds int32 of shared memory; the caller synchronises the CTA before the first use.
+__device__ __forceinline__ Ends fetch_ends(const BalArgs& a, int32_t* sh) {
+  if (a.seq_end == nullptr || a.n_seq > kSharedEnds) return Ends{a.seq_end, a.n_seq, a.T};
+  for (int s = threadIdx.x; s < a.n_seq; s += kBalThreads) sh[s] = a.seq_end[s];
+  return Ends{sh, a.n_seq, a.T};
 }
 
 // Selections and counted tokens.  A CTA takes a run of tokens; a sequence that lies in it has its
@@ -55,6 +71,8 @@ __device__ __forceinline__ int seq_of(const BalArgs& a, int t) {
 __global__ void __launch_bounds__(kBalThreads)
     balance_count_kernel(BalArgs a, const int64_t* __restrict__ idx, int run, int32_t* __restrict__ status) {
   extern __shared__ int32_t hist[];  // [E], then the number of tokens
+  __shared__ int32_t sh_ends[kSharedEnds];
+  const Ends ends = fetch_ends(a, sh_ends);
   if (blockIdx.x == 0 && a.seq_end != nullptr) {
     int bad = 0;
     for (int s = threadIdx.x; s < a.n_seq; s += kBalThreads) {
@@ -63,18 +81,18 @@ __global__ void __launch_bounds__(kBalThreads)
     }
     if (bad) atomicOr(status, DMOE_DEVERR_BAD_SEGMENT);
   }
-  int t0 = min((int64_t)blockIdx.x * run, (int64_t)a.T);
-  const int t_end = min((int64_t)t0 + run, (int64_t)a.T);
-  int s = seq_of(a, t0);
+  for (int e = threadIdx.x; e <= a.E; e += kBalThreads) hist[e] = 0;
+  __syncthreads();
+  int t0 = (int)min((int64_t)blockIdx.x * run, (int64_t)a.T);
+  const int t_end = (int)min((int64_t)t0 + run, (int64_t)a.T);
+  int s = ends.of(t0);
   while (t0 < t_end && s < a.n_seq) {  // block-uniform
-    const int t1 = min(t_end, seq_end_of(a, s));
+    const int t1 = min(t_end, ends[s]);
     if (t1 > t0) {
-      for (int e = threadIdx.x; e <= a.E; e += kBalThreads) hist[e] = 0;
-      __syncthreads();
-      const int64_t i1 = (int64_t)t1 * a.k;
-      for (int64_t i = (int64_t)t0 * a.k + threadIdx.x; i < i1; i += kBalThreads) {
-        if (a.mask != nullptr && !a.mask[i / a.k]) continue;
+      const unsigned i1 = (unsigned)t1 * a.k;  // T * k < 2^31
+      for (unsigned i = (unsigned)t0 * a.k + threadIdx.x; i < i1; i += kBalThreads) {
         const int64_t e = idx[i];
+        if (a.mask != nullptr && !a.mask[i / (unsigned)a.k]) continue;
         if (e >= 0 && e < a.E) atomicAdd(&hist[e], 1);
       }
       int mine = 0;
@@ -86,9 +104,10 @@ __global__ void __launch_bounds__(kBalThreads)
       if (mine) atomicAdd(&hist[a.E], mine);
       __syncthreads();
       int32_t* row = a.counts + (int64_t)s * a.E;
-      for (int e = threadIdx.x; e < a.E; e += kBalThreads)
-        if (hist[e]) atomicAdd(&row[e], hist[e]);
-      if (threadIdx.x == 0 && hist[a.E]) atomicAdd(&a.counts[(int64_t)a.n_seq * a.E + s], hist[a.E]);
+      for (int e = threadIdx.x; e <= a.E; e += kBalThreads) {
+        if (hist[e]) atomicAdd(e < a.E ? &row[e] : &a.counts[(int64_t)a.n_seq * a.E + s], hist[e]);
+        hist[e] = 0;
+      }
       __syncthreads();
       t0 = t1;
     }
@@ -129,21 +148,58 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+__device__ __forceinline__ float exp_ftz(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.442695041f));
+  return r;
+}
+
+// Expert of value i of a lane: runs of four neighbours where a lane has four or more.
+template <int G, int V>
+__device__ __forceinline__ int expert_of(int i, int lane) {
+  return V >= 4 ? (i >> 2) * (4 * G) + lane * 4 + (i & 3) : i * G + lane;
+}
+
+// One token's row, -inf where it has no expert or is not read.
+template <int G, int V, int DT>
+__device__ __forceinline__ void load_row(const void* logits, int64_t row, int E, int lane, bool live, bool vec, float* l) {
+  const int64_t base = row * E;
+  if (V >= 4 && vec) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const int e = expert_of<G, V>(i, lane);
+      float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (live && e < E) {
+        if constexpr (DT == DMOE_F32) {
+          const float4 f = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(logits) + base + e));
+          v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        } else {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(logits) + (base + e) * 2));
+          float f[8];
+          unpack8<DT>(make_uint4(w.x, w.y, 0, 0), f);
+          v[0] = f[0], v[1] = f[1], v[2] = f[2], v[3] = f[3];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4 && i + j < V; ++j) l[i + j] = v[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = expert_of<G, V>(i, lane);
+      l[i] = live && e < E ? load_as_float(logits, base + e, DT) : -INFINITY;
+    }
+  }
+}
+
 // One token's probabilities (not yet divided by their sum) and what its loss terms need.
 template <int G, int V, bool SIGMOID>
 struct Row {
-  float p[V];     // numerators of p
-  float soft[SIGMOID ? V : 1];  // numerators of softmax(l) where p is another thing
+  float p[V];                         // numerators of p
+  float soft[SIGMOID ? V : 1];        // numerators of softmax(l) where p is another thing
+  float away[SIGMOID ? V : 1];        // 1 - sigmoid(l)
   float total, soft_total, lse;
-  bool any;       // some logit is above -inf (or is NaN)
-
-  __device__ __forceinline__ void load(const void* logits, int dt, int64_t row, int E, int lane, bool live, float* l) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = i * G + lane;
-      l[i] = live && e < E ? load_as_float(logits, row * E + e, dt) : -INFINITY;
-    }
-  }
+  bool any;                           // some logit is above -inf (or is NaN)
 
   __device__ __forceinline__ void compute(const float* l) {
     float m = l[0];
@@ -154,16 +210,27 @@ struct Row {
     float sum = 0.f, ssum = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float ex = __expf(l[i] - base);
+      const float ex = exp_ftz(l[i] - base);
       ssum += ex;
       if constexpr (SIGMOID) {
         soft[i] = ex;
-        // sigmoid(l) = exp(min(l, 0)) / (1 + exp(-|l|)), over its largest exp(min(base, 0))
-        p[i] = __fdividef(__expf(fminf(l[i], 0.f) - fminf(base, 0.f)), 1.f + __expf(-fabsf(l[i])));
+        const float e = exp_ftz(-fabsf(l[i]));
+        const float r = __fdividef(1.f, 1.f + e);
+        p[i] = (l[i] >= 0.f ? 1.f : e) * r;
+        away[i] = (l[i] >= 0.f ? e : 1.f) * r;
         sum += p[i];
-        if (l[i] != l[i]) sum = l[i];  // the minimum above prefers a number, too
       } else {
         p[i] = ex;
+      }
+    }
+    if constexpr (SIGMOID) {
+      if (base < -40.f) {  // sigmoid(l) / exp(base), 1 + e is 1
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          p[i] = soft[i];
+          sum += p[i];
+        }
       }
     }
     soft_total = group_sum<G>(ssum);
@@ -173,41 +240,74 @@ struct Row {
   }
 };
 
-template <int G, int V, bool SIGMOID>
+// The tokens [t0, t1) of a group in turn: their sequences, which of them count, and their rows, one
+// token ahead.
+template <int G, int V, int DT>
+struct Walk {
+  const BalArgs& a;
+  const Ends& ends;
+  int t, t1, s, s_end, lane;
+  bool vec;
+  // the token that comes next
+  bool live;
+  int seq;
+  float l[V];
+  __device__ __forceinline__ Walk(const BalArgs& args, const Ends& en, int first, int end, int ln)
+      : a(args), ends(en), t(first), t1(end), lane(ln) {
+    s = t < t1 ? ends.of(t) : a.n_seq;
+    s_end = s < a.n_seq ? ends[s] : a.T;
+    vec = a.E % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0;
+    fetch();
+  }
+  __device__ __forceinline__ void fetch() {
+    while (t < t1 && s < a.n_seq && t >= s_end) {
+      ++s;
+      if (s < a.n_seq) s_end = ends[s];
+    }
+    live = t < t1 && s < a.n_seq && (a.mask == nullptr || a.mask[t]);
+    seq = s;
+    load_row<G, V, DT>(a.logits, t, a.E, lane, live, vec, l);
+  }
+};
+
+template <int G, int V, bool SIGMOID, int DT>
 __global__ void __launch_bounds__(kBalThreads)
-    balance_loss_kernel(BalArgs a, int dt, int run, float* __restrict__ loss, double* __restrict__ part) {
+    balance_loss_kernel(BalArgs a, int run, float* __restrict__ loss, double* __restrict__ part) {
   __shared__ double sums[2][kBalThreads / 32];
   __shared__ int last;
+  __shared__ int32_t sh_ends[kSharedEnds];
+  const Ends ends = fetch_ends(a, sh_ends);
   int full, tokens;
-  totals(a, full, tokens);
+  totals(a, full, tokens);  // synchronises
   const int lane = threadIdx.x & (G - 1);
   const int group = blockIdx.x * (kBalThreads / G) + threadIdx.x / G;  // takes tokens [t0, t1)
   const int t0 = (int)min((int64_t)group * run, (int64_t)a.T), t1 = (int)min((int64_t)t0 + run, (int64_t)a.T);
   const int32_t* n_of = a.counts + (int64_t)a.n_seq * a.E;
-  int s = t0 < t1 ? seq_of(a, t0) : a.n_seq, loaded = -1;
-  int s_end = s < a.n_seq ? seq_end_of(a, s) : a.T;
+  Walk<G, V, DT> w(a, ends, t0, t1, lane);
+  int loaded = -1;
   float c[V], coef = 0.f;
   double bal = 0.0, zz = 0.0;
   for (int i = 0; i < run; ++i) {  // every group makes `run` steps: the shuffles span the warp
-    const int t = t0 + i;
-    while (t < t1 && s < a.n_seq && t >= s_end) {
-      ++s;
-      if (s < a.n_seq) s_end = seq_end_of(a, s);
+    const bool live = w.live;
+    const int s = w.seq;
+    float l[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) l[v] = w.l[v];
+    if (i + 1 < run) {
+      ++w.t;
+      w.fetch();
     }
-    const bool live = t < t1 && s < a.n_seq && (a.mask == nullptr || a.mask[t]);
     if (live && loaded != s) {
       loaded = s;
       const float n = (float)n_of[s];
       coef = __fdividef((float)a.E, (float)a.k * n) / (n * (float)full);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int e = v * G + lane;
+        const int e = expert_of<G, V>(v, lane);
         c[v] = e < a.E ? (float)a.counts[(int64_t)s * a.E + e] : 0.f;
       }
     }
     Row<G, V, SIGMOID> r;
-    float l[V];
-    r.load(a.logits, dt, t, a.E, lane, live, l);
     r.compute(l);
     float dot = 0.f;
 #pragma unroll
@@ -231,9 +331,9 @@ __global__ void __launch_bounds__(kBalThreads)
   __syncthreads();
   if (threadIdx.x == 0) {
     double b = 0.0, z = 0.0;
-    for (int w = 0; w < kBalThreads / 32; ++w) {
-      b += sums[0][w];
-      z += sums[1][w];
+    for (int i = 0; i < kBalThreads / 32; ++i) {
+      b += sums[0][i];
+      z += sums[1][i];
     }
     part[2 * blockIdx.x] = b;
     part[2 * blockIdx.x + 1] = z;
@@ -261,50 +361,54 @@ __global__ void __launch_bounds__(kBalThreads)
   __syncthreads();
   if (threadIdx.x == 0) {
     b = z = 0.0;
-    for (int w = 0; w < kBalThreads / 32; ++w) {
-      b += sums[0][w];
-      z += sums[1][w];
+    for (int i = 0; i < kBalThreads / 32; ++i) {
+      b += sums[0][i];
+      z += sums[1][i];
     }
     loss[0] = (float)b;
     loss[1] = tokens > 0 ? (float)(z / (double)tokens) : 0.f;
   }
 }
 
-template <int G, int V, bool SIGMOID>
+template <int G, int V, bool SIGMOID, int DT>
 __global__ void __launch_bounds__(kBalThreads)
-    balance_grad_kernel(BalArgs a, int dt, int run, const float* __restrict__ g_bal, const float* __restrict__ g_z,
+    balance_grad_kernel(BalArgs a, int run, const float* __restrict__ g_bal, const float* __restrict__ g_z,
                         void* __restrict__ grad) {
+  __shared__ int32_t sh_ends[kSharedEnds];
+  const Ends ends = fetch_ends(a, sh_ends);
   int full, tokens;
-  totals(a, full, tokens);
+  totals(a, full, tokens);  // synchronises
   const int lane = threadIdx.x & (G - 1);
   const int group = blockIdx.x * (kBalThreads / G) + threadIdx.x / G;
   const int t0 = (int)min((int64_t)group * run, (int64_t)a.T), t1 = (int)min((int64_t)t0 + run, (int64_t)a.T);
   const int32_t* n_of = a.counts + (int64_t)a.n_seq * a.E;
   const float gb = g_bal ? *g_bal : 0.f;
   const float gz = g_z && tokens > 0 ? *g_z * 2.f / (float)tokens : 0.f;
-  int s = t0 < t1 ? seq_of(a, t0) : a.n_seq, loaded = -1;
-  int s_end = s < a.n_seq ? seq_end_of(a, s) : a.T;
+  const bool vec_out = V >= 4 && a.E % 4 == 0 && (reinterpret_cast<uintptr_t>(grad) & 15u) == 0;
+  Walk<G, V, DT> w(a, ends, t0, t1, lane);
+  int loaded = -1;
   float c[V], coef = 0.f;
   for (int i = 0; i < run; ++i) {
-    const int t = t0 + i;
-    while (t < t1 && s < a.n_seq && t >= s_end) {
-      ++s;
-      if (s < a.n_seq) s_end = seq_end_of(a, s);
+    const bool live = w.live;
+    const int s = w.seq, t = w.t;
+    float l[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) l[v] = w.l[v];
+    if (i + 1 < run) {
+      ++w.t;
+      w.fetch();
     }
-    const bool live = t < t1 && s < a.n_seq && (a.mask == nullptr || a.mask[t]);
     if (live && loaded != s) {
       loaded = s;
       const float n = (float)n_of[s];
       coef = gb * (__fdividef((float)a.E, (float)a.k * n) / (n * (float)full));
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int e = v * G + lane;
+        const int e = expert_of<G, V>(v, lane);
         c[v] = e < a.E ? (float)a.counts[(int64_t)s * a.E + e] : 0.f;
       }
     }
     Row<G, V, SIGMOID> r;
-    float l[V];
-    r.load(a.logits, dt, t, a.E, lane, live, l);
     r.compute(l);
     float dot = 0.f;
 #pragma unroll
@@ -315,62 +419,92 @@ __global__ void __launch_bounds__(kBalThreads)
     if (t < t1) {
       const bool on = live && r.any;
       const float zc = on && gz != 0.f ? gz * r.lse / r.soft_total : 0.f;
+      float d[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int e = v * G + lane;
-        if (e < a.E) {
-          float d = 0.f;
-          if (on) {
-            d = coef * (r.p[v] * inv) * (c[v] - dot);
-            if constexpr (SIGMOID) {
-              const float x = __expf(-fabsf(l[v]));
-              d *= __fdividef(l[v] >= 0.f ? x : 1.f, 1.f + x);  // 1 - sigmoid(l)
-            }
-            // left out without a gradient of z: lse may be infinite where the balance is not
-            if (gz != 0.f) d += zc * (SIGMOID ? r.soft[SIGMOID ? v : 0] : r.p[v]);
-          }
-          store_from_float(grad, (int64_t)t * a.E + e, d, dt);
+        d[v] = 0.f;
+        if (on) {
+          d[v] = coef * (r.p[v] * inv) * (c[v] - dot);
+          if constexpr (SIGMOID) d[v] *= r.away[v];
+          // left out without a gradient of z: lse may be infinite where the balance is not
+          if (gz != 0.f) d[v] += zc * (SIGMOID ? r.soft[SIGMOID ? v : 0] : r.p[v]);
+        }
+      }
+      const int64_t base = (int64_t)t * a.E;
+      if (vec_out) {
+#pragma unroll
+        for (int v = 0; v + 3 < V; v += 4) {
+          const int e = expert_of<G, V>(v, lane);
+          if (e >= a.E) continue;
+          if constexpr (DT == DMOE_F32)
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(grad) + base + e) = make_float4(d[v], d[v + 1], d[v + 2], d[v + 3]);
+          else
+            *reinterpret_cast<uint2*>(reinterpret_cast<char*>(grad) + (base + e) * 2) =
+                make_uint2(pack2<DT>(d[v], d[v + 1]), pack2<DT>(d[v + 2], d[v + 3]));
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int e = expert_of<G, V>(v, lane);
+          if (e < a.E) store_from_float(grad, base + e, d[v], DT);
         }
       }
     }
   }
 }
 
-// Tokens a group takes and CTAs: up to four CTAs an SM, runs no longer than that needs.
+// Tokens a group takes and CTAs: about eight CTAs an SM, runs no longer than that needs.
 void shape(int T, int per_cta, int* run, int* grid) {
-  const int64_t groups = (int64_t)kMaxGrid / 2 * per_cta;
+  const int64_t groups = (int64_t)kMaxGrid * per_cta;
   *run = (int)((T + groups - 1) / groups);
   if (*run < 1) *run = 1;
   const int64_t g = ((int64_t)T + (int64_t)per_cta * *run - 1) / ((int64_t)per_cta * *run);
   *grid = (int)(g < 1 ? 1 : g);
 }
 
-template <int G, int V, bool SIGMOID>
-int run_balance(const BalArgs& a, int dt, float* loss, double* part, const float* gb, const float* gz, void* grad,
-                cudaStream_t st) {
+// Where the forward (grad NULL) and the backward pass write.
+struct BalOut {
+  float* loss;
+  double* part;
+  const float* gb;
+  const float* gz;
+  void* grad;
+  bool backward;
+};
+
+template <int G, int V, bool SIGMOID, int DT>
+int run_balance(const BalArgs& a, const BalOut& o, cudaStream_t st) {
   int run, grid;
   shape(a.T, kBalThreads / G, &run, &grid);
-  if (grad == nullptr)
-    balance_loss_kernel<G, V, SIGMOID><<<grid, kBalThreads, 0, st>>>(a, dt, run, loss, part);
+  if (o.backward)
+    balance_grad_kernel<G, V, SIGMOID, DT><<<grid, kBalThreads, 0, st>>>(a, run, o.gb, o.gz, o.grad);
   else
-    balance_grad_kernel<G, V, SIGMOID><<<grid, kBalThreads, 0, st>>>(a, dt, run, gb, gz, grad);
+    balance_loss_kernel<G, V, SIGMOID, DT><<<grid, kBalThreads, 0, st>>>(a, run, o.loss, o.part);
   DMOE_LAUNCH_CHECK();
   return DMOE_OK;
 }
 
+template <bool SIGMOID, int DT>
+int by_experts(const BalArgs& a, const BalOut& o, cudaStream_t st) {
+  if (a.E <= 8) return run_balance<8, 1, SIGMOID, DT>(a, o, st);
+  if (a.E <= 16) return run_balance<16, 1, SIGMOID, DT>(a, o, st);
+  if (a.E <= 32) return run_balance<32, 1, SIGMOID, DT>(a, o, st);
+  if (a.E <= 64) return run_balance<32, 2, SIGMOID, DT>(a, o, st);
+  if (a.E <= 128) return run_balance<32, 4, SIGMOID, DT>(a, o, st);
+  if (a.E <= 256) return run_balance<32, 8, SIGMOID, DT>(a, o, st);
+  if (a.E <= 512) return run_balance<32, 16, SIGMOID, DT>(a, o, st);
+  return run_balance<32, 32, SIGMOID, DT>(a, o, st);
+}
+
 template <bool SIGMOID>
-int dispatch_balance(const BalArgs& a, int dt, float* loss, double* part, const float* gb, const float* gz, void* grad,
-                     cudaStream_t st) {
-#define DMOE_BAL(G, V) return run_balance<G, V, SIGMOID>(a, dt, loss, part, gb, gz, grad, st)
-  if (a.E <= 8) DMOE_BAL(8, 1);
-  if (a.E <= 16) DMOE_BAL(16, 1);
-  if (a.E <= 32) DMOE_BAL(32, 1);
-  if (a.E <= 64) DMOE_BAL(32, 2);
-  if (a.E <= 128) DMOE_BAL(32, 4);
-  if (a.E <= 256) DMOE_BAL(32, 8);
-  if (a.E <= 512) DMOE_BAL(32, 16);
-  DMOE_BAL(32, 32);
-#undef DMOE_BAL
+int by_type(const BalArgs& a, int dt, const BalOut& o, cudaStream_t st) {
+  if (dt == DMOE_F32) return by_experts<SIGMOID, DMOE_F32>(a, o, st);
+  if (dt == DMOE_BF16) return by_experts<SIGMOID, DMOE_BF16>(a, o, st);
+  return by_experts<SIGMOID, DMOE_F16>(a, o, st);
+}
+
+int launch_balance(const BalArgs& a, int dt, int mode, const BalOut& o, cudaStream_t st) {
+  return mode == DMOE_ROUTER_SOFTMAX ? by_type<false>(a, dt, o, st) : by_type<true>(a, dt, o, st);
 }
 
 int check_balance(const char* name, const void* logits, int dtype, int T, int E, int k, int mode,
@@ -418,9 +552,8 @@ extern "C" int dmoe_balance_loss(const void* logits, int dtype, const int64_t* i
   if (run < least) run = (int)least;
   balance_count_kernel<<<(T + run - 1) / run, kBalThreads, (E + 1) * 4, st>>>(a, idx, run, dev_status);
   DMOE_LAUNCH_CHECK();
-  double* part = reinterpret_cast<double*>(workspace);
-  return mode == DMOE_ROUTER_SOFTMAX ? dispatch_balance<false>(a, dtype, loss, part, nullptr, nullptr, nullptr, st)
-                                     : dispatch_balance<true>(a, dtype, loss, part, nullptr, nullptr, nullptr, st);
+  const BalOut o{loss, reinterpret_cast<double*>(workspace), nullptr, nullptr, nullptr, false};
+  return launch_balance(a, dtype, mode, o, st);
 }
 
 extern "C" int dmoe_balance_loss_backward(const void* logits, int dtype, int T, int E, int k, int mode,
@@ -433,7 +566,6 @@ extern "C" int dmoe_balance_loss_backward(const void* logits, int dtype, int T, 
   if (T == 0) return DMOE_OK;
   DMOE_REQUIRE(grad != nullptr && (reinterpret_cast<uintptr_t>(grad) & 3u) == 0, "%s: bad gradient pointer", name);
   const BalArgs a{logits, T, E, k, seq_end, n_seq, mask, const_cast<int32_t*>(counts)};
-  cudaStream_t st = as_stream(stream);
-  return mode == DMOE_ROUTER_SOFTMAX ? dispatch_balance<false>(a, dtype, nullptr, nullptr, g_balance, g_z, grad, st)
-                                     : dispatch_balance<true>(a, dtype, nullptr, nullptr, g_balance, g_z, grad, st);
+  const BalOut o{nullptr, nullptr, g_balance, g_z, grad, true};
+  return launch_balance(a, dtype, mode, o, as_stream(stream));
 }
