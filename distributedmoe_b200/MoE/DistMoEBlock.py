@@ -576,7 +576,9 @@ class DistMoEBlock(nn.Module):
         before the gather (8-bit records cross NVLink: about half the bytes), the gate/up
         GEMM runs on 8-bit tensor cores and the down projection in bf16 (bf16 layers only;
         the reference's benchmark offers "fp8" as a whole-layer 8-bit cast,
-        src/python/MoE/benchmarks/bench.py:184-185)."""
+        src/python/MoE/benchmarks/bench.py:184-185); or "fp8_block": e4m3 with one scale for each
+        128 x 128 block of all three projections and for each 128 values of a token row, the form
+        in which 8-bit checkpoints are published (bf16 layers, hidden and inner % 16 == 0)."""
         tte = self.tensor_transfer_engine
         if not getattr(tte, "direct", False):
             raise RuntimeError("the device-driven data plane needs the NVLinkDirect backend")
@@ -590,15 +592,18 @@ class DistMoEBlock(nn.Module):
                              f"[{n_local}, I, {d}] and down [{n_local}, {d}, I]")
         if self.dtype not in (torch.bfloat16, torch.float16, torch.float32):
             raise NotImplementedError("the device-driven data plane computes in bf16, fp16 or fp32")
-        if expert_precision not in ("model", "fp8"):
-            raise ValueError(f"expert_precision {expert_precision!r}: 'model' or 'fp8'")
-        fp8 = expert_precision == "fp8"
-        if fp8 and (self.dtype != torch.bfloat16 or d % 16):
+        if expert_precision not in ("model", "fp8", "fp8_block"):
+            raise ValueError(f"expert_precision {expert_precision!r}: 'model', 'fp8' or 'fp8_block'")
+        fp8, blocks = expert_precision == "fp8", expert_precision == "fp8_block"
+        if (fp8 or blocks) and (self.dtype != torch.bfloat16 or d % 16):
             raise ValueError("8-bit experts need a bf16 layer and hidden % 16 == 0")
+        if blocks and g.shape[1] % 16:
+            raise ValueError("block-scaled experts need an inner dimension that is a multiple of 16")
+        record = N.fp8_record_bytes(d) if fp8 else N.fp8_block_record_bytes(d) if blocks else None
         dev = self.device
         with torch.cuda.device(dev):
             tte.open_window(capacity, max(max_tokens * k, 1), d, self.dtype, inst.n_inst, dev,
-                            record_bytes=N.fp8_record_bytes(d) if fp8 else None)
+                            record_bytes=record)
             descs = exchange(tte.window_descriptor())
             win = tte.attach_windows(descs, rank)
             i32 = dict(dtype=torch.int32, device=dev)
@@ -609,8 +614,12 @@ class DistMoEBlock(nn.Module):
                 "world": world, "rank": rank, "inst": inst, "win": win, "cap": capacity, "policy": policy,
                 "n_local": n_local, "stack": (g, u, dn), "max_tokens": max_tokens,
                 "fp8": N.Fp8Experts(g, u, dn) if fp8 and n_local > 0 else None, "is_fp8": fp8,
-                "records": torch.empty(max(max_tokens, 1), N.fp8_record_bytes(d), dtype=torch.uint8, device=dev)
-                if fp8 else None,
+                "blocks": N.Fp8BlockExperts(g, u, dn) if blocks and n_local > 0 else None,
+                "is_blocks": blocks,
+                "blocks_ws": torch.empty(N.ep_fp8_blocks_workspace(capacity, g.shape[1]), dtype=torch.uint8, device=dev)
+                if blocks and n_local > 0 else None,
+                "records": torch.empty(max(max_tokens, 1), record, dtype=torch.uint8, device=dev)
+                if record is not None else None,
                 "timeout_ns": int(timeout_ms) * 1_000_000,
                 "inst_rank": torch.tensor(inst.inst_rank, **i32),
                 "inst_slot": torch.tensor(inst.inst_slot, **i32),
@@ -711,8 +720,12 @@ class DistMoEBlock(nn.Module):
             counts = offsets = perm_token = perm_slot = inverse = w = None
         inst = ep["inst"]
         N.ep_plan(win, counts, E, inst.n_inst, ep["policy"], table, cap, tmo, placement + (ep["seg_expert"], ep["seg_end"]))
-        # 8-bit experts: each token row leaves as one record (e4m3 codes + its scale).
-        rows_out = N.quantize_records(x, ep["records"][:T]) if ep["is_fp8"] else x
+        # 8-bit experts: each token row leaves as one record (e4m3 codes + its scale or scales).
+        rows_out = x
+        if ep["is_fp8"]:
+            rows_out = N.quantize_records(x, ep["records"][:T])
+        elif ep["is_blocks"]:
+            rows_out = N.quantize_block_records(x, ep["records"][:T])
         N.ep_dispatch(win, rows_out, T, k, E, offsets, perm_token, perm_slot, placement, ep["inst_rank"], cap,
                       ep["ret"], ep["done"])
         # The shared expert starts on a side stream once the rows are sent: the routing kernels
@@ -729,6 +742,10 @@ class DistMoEBlock(nn.Module):
             act = ACTIVATIONS[self.config.activation]
             if ep["fp8"] is not None:
                 N.ep_expert_mlp_fp8(win, ep["fp8"], *segs, cap, act, self._direct_tile_policy(T), work_rows=rows)
+            elif ep["blocks"] is not None:
+                # Every rank sends about T tokens: the rows an instance can expect.
+                hint = max(1, -(-ep["world"] * T * k // max(1, inst.n_inst)))
+                N.ep_expert_mlp_fp8_blocks(win, ep["blocks"], *segs, cap, act, ep["blocks_ws"], hint, work_rows=rows)
             else:
                 N.ep_expert_mlp(win, g, u, dn, *segs, cap, act, self._direct_tile_policy(T), work_rows=rows)
         N.ep_signal(win, N.EP_FLAG_RESULTS, dev)

@@ -89,8 +89,8 @@ class LocalCluster:
         block must sit on the host's GPU; the blocks' stacks are concatenated (block order)
         into the one weight stack the grouped MLP reads; max_tokens (default io_buffer_size *
         number_of_io_buffers // top_k) sizes the receive window; cuda_graphs replays each
-        token count's forward from a captured CUDA graph; expert_precision "fp8" runs the
-        routed experts on 8-bit records (DistMoEBlock.setup_direct_plane)."""
+        token count's forward from a captured CUDA graph; expert_precision "fp8" or
+        "fp8_block" runs the routed experts on 8-bit records (DistMoEBlock.setup_direct_plane)."""
         nb = len(expert_blocks)
         ports = free_ports(1 + 5 * nb)
         host_port, rest = ports[0], ports[1:]

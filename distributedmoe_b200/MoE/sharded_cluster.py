@@ -111,7 +111,8 @@ class ShardedCluster:
         cuda_graphs: replay each token count's forward from a captured CUDA graph (every rank
         captures at the same step; capturing runs no kernel, so the ranks stay in step).
         expert_precision: "fp8" sends 8-bit records and runs the gate/up GEMM on e4m3 tensor
-        cores (DistMoEBlock.setup_direct_plane)."""
+        cores, "fp8_block" all three projections with a scale for each block of 128
+        (DistMoEBlock.setup_direct_plane)."""
         direct = backend == TensorTransferEngineBackend.NVLinkDirect
         if direct:
             # The task buffers only serve the metadata hand-shake: keep them small.

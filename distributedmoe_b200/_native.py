@@ -123,6 +123,9 @@ SIGNATURES = {
     "dmoe_ep_expert_mlp_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                               _vp, _vp, ctypes.c_int, _i64, ctypes.c_int, _vp, _sz, _vp, ctypes.c_int,
                                               _vp]),
+    "dmoe_ep_expert_mlp_fp8_blocks": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int,
+                                                     ctypes.c_int, _vp, _vp, ctypes.c_int, _i64, ctypes.c_int,
+                                                     ctypes.c_int, _vp, _sz, _vp, _vp]),
     "dmoe_ep_wait": (ctypes.c_int, [_vp, ctypes.c_int, _u64, _vp, _vp]),
     "dmoe_ep_signal": (ctypes.c_int, [_vp, ctypes.c_int, _vp]),
     "dmoe_ep_combine": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
@@ -753,6 +756,28 @@ def matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor
     return _product(xq, x_scale, w_q, w_scale, shape, 1, (0,), (xq.shape[0],), out, out_dtype, 0)
 
 
+def fp8_block_record_bytes(d: int) -> int:
+    """Bytes of one block-scaled receive record: d e4m3 codes, ceil(d / 128) fp32 scales, padding to
+    16."""
+    return d + (4 * _blocks(d) + 15) // 16 * 16
+
+
+def quantize_block_records(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [T, d] -> uint8 records [T, fp8_block_record_bytes(d)]: row t's codes, then its scales."""
+    dev = _one_device(x, out)
+    T, d = x.shape
+    if d == 0 or d % 16 or not x.is_contiguous():
+        raise DMoEError(f"8-bit records need a contiguous x with d % 16 == 0 (d={d})")
+    rec = fp8_block_record_bytes(d)
+    if out is None:
+        out = torch.empty(T, rec, dtype=torch.uint8, device=x.device)
+    if out.dtype != torch.uint8 or out.dim() != 2 or out.shape[0] < T or out.shape[1] != rec or not out.is_contiguous():
+        raise DMoEError(f"records must be a contiguous uint8 [T, {rec}] tensor")
+    _call(dev, "quantize_blocks_e4m3", lib().dmoe_quantize_blocks_e4m3, x.data_ptr(), dtype_code(x.dtype), 1, T, d, 1,
+          out.data_ptr(), rec, out.data_ptr() + d, rec // 4)
+    return out
+
+
 class Fp8BlockExperts:
     """An expert stack whose three projections are e4m3 with one fp32 scale for each 128 x 128
     block: quantised here from 16- or 32-bit stacks, or taken as a checkpoint holds them
@@ -1083,6 +1108,31 @@ def ep_expert_mlp_fp8(win: EpWindow, experts: Fp8Experts, seg_expert: torch.Tens
                                       int(tile_policy), _stream(dev))
     _check(rc, "dmoe_ep_expert_mlp_fp8")
     tm.done()
+
+
+def ep_expert_mlp_fp8_blocks(win: EpWindow, experts: Fp8BlockExperts, seg_expert: torch.Tensor, seg_end: torch.Tensor,
+                             cap: int, act: int, workspace: torch.Tensor, rows_hint: int = 0,
+                             work_rows: Optional[float] = None) -> None:
+    """:func:`ep_expert_mlp` for block-scaled receive records (:func:`quantize_block_records`) and
+    e4m3 stacks, down projection included; the return rows are bf16.  workspace: uint8, at least
+    ``ep_fp8_blocks_workspace(cap, I)`` bytes; rows_hint: rows an instance is expected to have."""
+    dev = _one_device(experts.wd_q, seg_expert, seg_end, workspace)
+    device = seg_expert.device
+    E, d, I = experts._ptrs[-3:]
+    with torch.cuda.device(dev):
+        st = _stream(device)
+        tm = _Timed("grouped_gated_mlp", st, device, None if work_rows is None else 6.0 * work_rows * d * I)
+        rc = lib().dmoe_ep_expert_mlp_fp8_blocks(ctypes.byref(win), *experts._ptrs, seg_expert.data_ptr(),
+                                                 seg_end.data_ptr(), seg_expert.numel(), int(cap), int(rows_hint),
+                                                 int(act), workspace.data_ptr(), workspace.numel(),
+                                                 scratch.status(device).data_ptr(), st)
+        _check(rc, "dmoe_ep_expert_mlp_fp8_blocks")
+        tm.done()
+
+
+def ep_fp8_blocks_workspace(cap: int, inner: int) -> int:
+    """Bytes of workspace of :func:`ep_expert_mlp_fp8_blocks`."""
+    return int(lib().dmoe_grouped_mlp_fp8_blocks_workspace_size(int(cap), int(inner)))
 
 
 def ep_wait(win: EpWindow, kind: int, timeout_ns: int, device: torch.device, stream: Optional[int] = None) -> None:

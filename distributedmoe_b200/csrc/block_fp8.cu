@@ -1315,3 +1315,38 @@ extern "C" int dmoe_grouped_gated_mlp_fp8_blocks(const void* Xq, int64_t x_ld, c
   return run_blk_mlp(Xq, x_ld, x_scale, xs_ld, wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale, E_stack, d, I, segs,
                      rows_hint, act, Y, nullptr, nullptr, workspace, dev_status, as_stream(stream));
 }
+
+extern "C" int dmoe_ep_expert_mlp_fp8_blocks(const dmoe_ep_window* win, const void* wg_q, const float* wg_scale,
+                                             const void* wu_q, const float* wu_scale, const void* wd_q,
+                                             const float* wd_scale, int E_stack, int d, int I,
+                                             const int32_t* seg_expert, const int32_t* seg_end, int n_seg, int64_t cap,
+                                             int rows_hint, int act, void* workspace, size_t workspace_bytes,
+                                             int32_t* dev_status, void* stream) {
+  clear_error();
+  const char* name = "dmoe_ep_expert_mlp_fp8_blocks";
+  DMOE_REQUIRE(win != nullptr && win->world >= 1 && win->world <= DMOE_EP_MAX_RANKS && win->rank >= 0 &&
+                   win->rank < win->world,
+               "%s: bad window table", name);
+  DMOE_REQUIRE(act == DMOE_ACT_RELU || act == DMOE_ACT_SILU, "%s: bad activation %d", name, act);
+  DMOE_REQUIRE(d > 0 && I > 0 && d % 16 == 0 && I % 16 == 0, "%s: d=%d and I=%d must be multiples of 16", name, d, I);
+  DMOE_REQUIRE(E_stack >= 1 && n_seg >= 0 && n_seg <= kMaxSegs && rows_hint >= 0, "%s: bad E_stack/n_seg/rows_hint", name);
+  DMOE_REQUIRE(cap >= 0 && cap < (1ll << 31), "%s: bad capacity", name);
+  if (n_seg == 0 || cap == 0) return DMOE_OK;
+  const char* X = reinterpret_cast<const char*>(win->recv[win->rank]);
+  DMOE_REQUIRE(win->back[win->rank] != nullptr, "%s: null pointer", name);
+  if (int r = check_blk_mlp(name, X, wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale, d, I, n_seg, seg_expert, seg_end,
+                            cap, workspace, workspace_bytes, dev_status))
+    return r;
+  char* base[DMOE_EP_MAX_RANKS] = {};
+  for (int g = 0; g < win->world; ++g) {
+    DMOE_REQUIRE(win->rows[g] != nullptr && aligned16(win->rows[g]), "%s: rank %d has no return rows", name, g);
+    base[g] = reinterpret_cast<char*>(win->rows[g]);
+  }
+  static thread_local BlkSegs segs;
+  if (int r = fill_blk_segs(name, segs, seg_expert, seg_end, n_seg, 1, (int)cap, E_stack)) return r;
+  const int64_t rec = d + ((blocks_of(d) * 4 + 15) & ~int64_t(15));
+  return run_blk_mlp(X, rec, reinterpret_cast<const float*>(X + d), rec / 4, wg_q, wg_scale, wu_q, wu_scale, wd_q,
+                     wd_scale, E_stack, d, I, segs, rows_hint, act, nullptr,
+                     reinterpret_cast<const int32_t*>(win->back[win->rank]), base, workspace, dev_status,
+                     as_stream(stream));
+}

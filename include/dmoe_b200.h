@@ -472,6 +472,18 @@ int dmoe_ep_expert_mlp_fp8(const dmoe_ep_window* win, const void* wg_q, const fl
                            void* workspace, size_t workspace_bytes, int32_t* dev_status, int tile_policy,
                            void* stream);
 
+/* The exchange's expert step with block scales: each receive record is d e4m3 codes, then the fp32
+ * scales of its ceil(d / 128) blocks from byte d on, padded to a multiple of 16 bytes
+ * (dmoe_quantize_blocks_e4m3 with block_rows 1, q_ld = the record's bytes, the scale pointer at q + d
+ * and scale_ld = those bytes / 4 makes them).  Stacks and scales as dmoe_grouped_gated_mlp_fp8_blocks;
+ * the return rows are bf16.  rows_hint: rows an instance is expected to have; workspace >=
+ * dmoe_grouped_mlp_fp8_blocks_workspace_size(cap, I). */
+int dmoe_ep_expert_mlp_fp8_blocks(const dmoe_ep_window* win, const void* wg_q, const float* wg_scale, const void* wu_q,
+                                  const float* wu_scale, const void* wd_q, const float* wd_scale, int E_stack, int d,
+                                  int I, const int32_t* seg_expert, const int32_t* seg_end, int n_seg, int64_t cap,
+                                  int rows_hint, int act, void* workspace, size_t workspace_bytes, int32_t* dev_status,
+                                  void* stream);
+
 /* Wait (bounded) until every other rank raised its flag of `kind` to this forward's epoch. */
 int dmoe_ep_wait(const dmoe_ep_window* win, int kind, uint64_t timeout_ns, int32_t* dev_status, void* stream);
 

@@ -123,7 +123,7 @@ def test_no_tokens():
     N = _nat()
     l, idx = _case(0, 8, 2, torch.float32, 1)
     balance, z, counts = N.balance_loss(l, idx)
-    assert float(balance) == 0 and float(z) == 0 and counts.tolist() == [[0] * 8]
+    assert float(balance.detach()) == 0 and float(z.detach()) == 0 and counts.tolist() == [[0] * 8]
     assert torch.autograd.grad(balance, l)[0].shape == (0, 8)
     l, idx = _case(4, 8, 2, torch.float32, 1)
     balance, z, counts = N.balance_loss(l, idx, seq_end=torch.empty(0, dtype=torch.int32, device=DEV))

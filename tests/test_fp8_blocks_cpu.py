@@ -123,6 +123,33 @@ def test_wrappers_take_cuda_tensors_only():
             call()
 
 
+def test_exchange_step_refuses():
+    lib = N.lib()
+    win = N.ep_window(1, 0, [4096], [4096], [4096], [4096], [4096])
+
+    def call(w=win, E=2, d=256, inner=128, n=2, cap=64, hint=0, act=1, ws=P, nbytes=1 << 20, wd=P):
+        return lib.dmoe_ep_expert_mlp_fp8_blocks(ctypes.byref(w) if w else None, P, P, P, P, wd, P, E, d, inner, P, P, n,
+                                                 cap, hint, act, ws, nbytes, P, None)
+
+    _refused(call(w=None), "window")
+    _refused(call(w=N.ep_window(0, 0, [], [], [], [], [])), "window")
+    _refused(call(act=3), "activation")
+    _refused(call(d=200), "multiples of 16")
+    _refused(call(inner=24), "multiples of 16")
+    _refused(call(E=0), "E_stack")
+    _refused(call(n=1025), "n_seg")
+    _refused(call(hint=-1), "rows_hint")
+    _refused(call(cap=1 << 31), "capacity")
+    _refused(call(wd=None), "null")
+    _refused(call(nbytes=100), "workspace")
+    _refused(call(w=N.ep_window(1, 0, [4096], [4096], [4096], [4096], [4100])), "return rows")
+    assert call(n=0) == 0 and call(cap=0) == 0
+
+
+def test_record_bytes():
+    assert [N.fp8_block_record_bytes(d) for d in (16, 256, 2064, 7168)] == [32, 272, 2064 + 80, 7168 + 224]
+
+
 def test_workspace_sizes():
     lib = N.lib()
     assert lib.dmoe_grouped_mlp_fp8_blocks_workspace_size(100, 272) >= 100 * 272 + 100 * 3 * 4

@@ -1,0 +1,123 @@
+"""Block-scaled 8-bit experts in a layer: router, plan, gather, quantiser, gated MLP and combine as they
+are used together, called one by one and inside the device-driven plane (expert_precision
+"fp8_block"), against the definition in 64 bits.
+
+Tolerance: each expert row as in the MLP's own test, rounded to bf16 (half a step, 2^-8), weighted;
+the combine adds k of them in fp32 (k 2^-23) and rounds the sum to bf16 once more."""
+
+import pytest
+import torch
+
+from test_fp8_blocks_gpu import DEV, _mlp_reference, _nat, _quantize64, _values
+
+gpu = pytest.mark.gpu
+
+
+def _weights(E, d, I, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    w = [(torch.randn(E, *s, generator=g, device=DEV) * 0.05).to(torch.bfloat16) for s in ((I, d), (I, d), (d, I))]
+    w_r = (torch.randn(E, d, generator=g, device=DEV) * 0.05).to(torch.bfloat16)
+    return w, w_r, g
+
+
+def _expected(x, idx, w, weights):
+    """(y, allowed error) of the layer for tokens x with experts idx [T, k] and weights w [T, k]."""
+    T, k = idx.shape
+    d = x.shape[1]
+    y = torch.zeros(T, d, dtype=torch.float64, device=DEV)
+    slack, size = torch.zeros_like(y), torch.zeros_like(y)
+    q, s = _quantize64(x)
+    xv = _values(q, s, 1)
+    for e in range(weights[0].shape[0]):
+        t, slot = torch.where(idx == e)
+        if t.numel() == 0:
+            continue
+        g, u, dn = (_values(*_quantize64(m[e], 128), 128) for m in weights)
+        rows, err = _mlp_reference(xv[t], g, u, dn, True)
+        share = w[t, slot].double()[:, None]
+        y.index_add_(0, t, share * rows)
+        slack.index_add_(0, t, share * err)
+        size.index_add_(0, t, share * (rows.abs() + err))
+    slack = slack + 2.0 ** -8 * size + k * 2.0 ** -23 * size
+    return y, slack + 2.0 ** -8 * (y.abs() + slack)
+
+
+@gpu
+@pytest.mark.parametrize("T,E,k,d,I", [(1, 8, 2, 256, 384), (5, 16, 4, 400, 272), (200, 8, 2, 512, 400), (700, 4, 2, 272, 528)])
+def test_operators_one_by_one(T, E, k, d, I):
+    N = _nat()
+    weights, w_r, g = _weights(E, d, I, T + E)
+    x = torch.randn(T, d, generator=g, device=DEV).to(torch.bfloat16)
+    idx, w, _ = N.router(x, w_r, k, renormalize=True, w_dtype=torch.float32)
+    plan = N.route_plan(idx, w, E)
+    rows = torch.empty(T * k, d, dtype=torch.bfloat16, device=DEV)
+    N.permute_rows(x, rows, [0], [0], [T * k], row_map=plan["perm_token"])
+    xq, xs = N.quantize_blocks_e4m3(rows)
+    Y = N.grouped_gated_mlp_fp8_blocks(xq, xs, N.Fp8BlockExperts(*weights), torch.arange(E, dtype=torch.int32, device=DEV),
+                                       plan["offsets"][1:], N.ACT_SILU)
+    out = torch.empty(T, d, dtype=torch.bfloat16, device=DEV)
+    N.combine(Y, plan["inverse"], w, out)
+    N.check_device_status(torch.device(DEV))
+    want, slack = _expected(x, idx, w, weights)
+    assert ((out.double() - want).abs() - slack).max().item() <= 0
+
+
+@gpu
+def test_records_layout():
+    """Row t's codes in bytes [0, d), its scales from byte d on; a row is a multiple of 16 bytes."""
+    N = _nat()
+    for T, d in ((50, 256), (3, 2064), (1, 16)):
+        x = torch.randn(T, d, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).to(torch.bfloat16)
+        q, s = N.quantize_blocks_e4m3(x)
+        rec = N.quantize_block_records(x)
+        nb = s.shape[1]
+        assert rec.shape == (T, N.fp8_block_record_bytes(d)) and rec.shape[1] % 16 == 0
+        assert torch.equal(rec[:, :d], q.view(torch.uint8))
+        assert torch.equal(rec[:, d:d + 4 * nb].contiguous().view(torch.float32), s)
+    with pytest.raises(N.DMoEError):
+        N.quantize_block_records(torch.zeros(2, 24, device=DEV))
+
+
+@gpu
+@pytest.mark.parametrize("graphs", [False, True])
+def test_direct_layer(graphs):
+    """The device-driven plane with replicated blocks, eagerly and from captured graphs."""
+    from distributedmoe_b200.MoE.local_cluster import LocalCluster
+    from distributedmoe_b200.TensorTransferEngine import TensorTransferEngineBackend as B
+    N = _nat()
+    E, k, d, I = 8, 2, 272, 400
+    weights, w_r, g = _weights(E, d, I, 23)
+    blocks = [[0, 1, 2, 3], [4, 5, 6, 7], [1, 6]]
+    dev = torch.device(DEV)
+    cl = LocalCluster(E, blocks, k, d, torch.bfloat16, dev, [dev] * len(blocks),
+                      stacked=[tuple(m[b].contiguous() for m in weights) for b in blocks], io_buffer_size=256,
+                      number_of_io_buffers=1, backend=B.NVLinkDirect, max_tokens=1024, cuda_graphs=graphs,
+                      expert_precision="fp8_block", activation="silu", renormalize=True)
+    outs = []
+    try:
+        with torch.no_grad():
+            cl.moe.gate.weight.copy_(w_r)
+        for T in [1, 200, 1024, 200, 1]:
+            x = torch.randn(T, d, generator=g, device=DEV).to(torch.bfloat16)
+            outs.append((x, cl.moe(x)))
+        torch.cuda.synchronize()
+        N.check_device_status(dev)
+    finally:
+        cl.close()
+    for x, y in outs:
+        idx, w, _ = N.router(x, w_r, k, renormalize=True, w_dtype=torch.float32)
+        want, slack = _expected(x, idx, w, weights)
+        assert y.dtype == torch.bfloat16 and ((y.double() - want).abs() - slack).max().item() <= 0
+
+
+@gpu
+def test_direct_layer_refusals():
+    from distributedmoe_b200.MoE.local_cluster import LocalCluster
+    from distributedmoe_b200.TensorTransferEngine import TensorTransferEngineBackend as B
+    dev = torch.device(DEV)
+    for d, I, dtype, precision in ((272, 392, torch.bfloat16, "fp8_block"), (256, 384, torch.float16, "fp8_block"),
+                                   (264, 384, torch.bfloat16, "fp8_block"), (256, 384, torch.bfloat16, "fp8_blocks")):
+        stack = tuple(torch.zeros(2, *s, dtype=dtype, device=DEV) for s in ((I, d), (I, d), (d, I)))
+        with pytest.raises(ValueError):
+            LocalCluster(2, [[0, 1]], 1, d, dtype, dev, [dev], stacked=[stack], io_buffer_size=64, number_of_io_buffers=1,
+                         backend=B.NVLinkDirect, max_tokens=16, expert_precision=precision)
