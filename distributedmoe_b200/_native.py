@@ -662,7 +662,7 @@ def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Te
         raise DMoEError(f"block_rows={block_rows}: 1, or {FP8_BLOCK} for x [..., rows, cols]")
     code = dtype_code(x.dtype)
     q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
-    scale = torch.empty(s_shape, dtype=torch.float32, device=x.device)
+    scale = torch.empty(*s_shape, dtype=torch.float32, device=x.device)
     _call(dev, "quantize_blocks_e4m3", lib().dmoe_quantize_blocks_e4m3, x.data_ptr(), code, batch, rows, cols,
           block_rows, q.data_ptr(), cols, scale.data_ptr(), nb)
     return q, scale
@@ -715,7 +715,7 @@ def _product(xq, x_scale, w_q, w_scale, w_shape, E, seg_expert, seg_end, out, ou
     Nn, K = w_shape[-2:]
     m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, K)
     if out is None:
-        out = torch.empty((m, Nn), dtype=out_dtype or torch.bfloat16, device=xq.device)
+        out = torch.empty(m, Nn, dtype=out_dtype or torch.bfloat16, device=xq.device)
         y_ld = Nn
     else:
         if out.shape != (m, Nn) or (Nn > 1 and out.stride(1) != 1) or (out_dtype is not None and out.dtype != out_dtype):
@@ -828,7 +828,7 @@ def grouped_gated_mlp_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, expert
     d, I = experts._ptrs[-2:]
     m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, d)
     if Y is None:
-        Y = torch.empty((m, d), dtype=torch.bfloat16, device=xq.device)
+        Y = torch.empty(m, d, dtype=torch.bfloat16, device=xq.device)
     elif Y.dtype != torch.bfloat16 or Y.shape != (m, d) or not Y.is_contiguous():
         raise DMoEError(f"Y must be a contiguous bf16 [{m}, {d}] tensor")
     nbytes = lib().dmoe_grouped_mlp_fp8_blocks_workspace_size(m, I)

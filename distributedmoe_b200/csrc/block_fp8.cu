@@ -204,9 +204,9 @@ __device__ __forceinline__ char* blk_out_row(const BlkArgs& a, int row, int esz)
   return base == nullptr ? nullptr : base + (int64_t)(code & 0x7ffffff) * a.ldo * esz;
 }
 
-// 32 lanes x 16 fp32 columns in two halves: the registers hold their values after the second, which
-// waits for every load this warp has started.
-__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t (&r)[16]) {
+// 32 lanes x 16 or 32 fp32 columns in two halves: the registers hold their values after the second,
+// which waits for every load this warp has started.
+__device__ __forceinline__ void tmem_ld_start(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
       "[%16];"
@@ -214,10 +214,21 @@ __device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t (&r)[16
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld_start(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : DMOE_R8(0), DMOE_R8(8), DMOE_R8(16), DMOE_R8(24)
+      : "r"(taddr)
+      : "memory");
+}
 #define BLK_RW8(b) "+r"(r[b + 0]), "+r"(r[b + 1]), "+r"(r[b + 2]), "+r"(r[b + 3]), "+r"(r[b + 4]), "+r"(r[b + 5]), \
                    "+r"(r[b + 6]), "+r"(r[b + 7])
-__device__ __forceinline__ void tmem_ld16_finish(uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_finish(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : BLK_RW8(0), BLK_RW8(8)::"memory");
+}
+__device__ __forceinline__ void tmem_ld_finish(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : BLK_RW8(0), BLK_RW8(8), BLK_RW8(16), BLK_RW8(24)::"memory");
 }
 #undef BLK_RW8
 
@@ -270,33 +281,43 @@ __device__ __forceinline__ void named_sync(int id, int threads) {
 // hands its own to the other two.
 constexpr int kN = 256;                // weight rows of a tile: gated 128 gate and 128 up rows
 constexpr int kThreadsBlk = 128 + 32 * kEpiWarps;
-constexpr int kRegsIssue = 72, kRegsSums = 216;  // 128 * 72 + 256 * 216 = 384 * 168, the registers at launch
+// Registers a thread after the hand-over; both sides of the split have to hold their own without
+// spills (the issuing warps spilled at 40: 224 -> 377 us for 4096 x 14336 x 4096).
+struct RegSplit {
+  int issue, sums;
+};
+constexpr RegSplit kWide{56, 224}, kEven{72, 216};
+static_assert(128 * kWide.issue + 256 * kWide.sums == kThreadsBlk * 168 &&
+                  128 * kEven.issue + 256 * kEven.sums == kThreadsBlk * 168,
+              "a split hands out the registers the block was launched with");
 constexpr int kOpBytes = 128 * kBlk;             // one step of 128 operand rows
 constexpr int kBarBytes = 256;
 constexpr int kXchBytes = 2 * 2 * 128 * 4;
 constexpr int kOutBytes = kEpiWarps * 32 * 128;  // 128 bytes of 32 rows for each epilogue warp
 
 template <bool GATED>
-__device__ __forceinline__ int tmem_col(int half, int j) {  // first of the 16 columns of chunk j
-  return GATED ? (j < 4 ? half * 64 + j * 16 : 128 + half * 64 + (j - 4) * 16) : half * 128 + j * 16;
+__device__ __forceinline__ int tmem_col(int half, int c) {  // column c of this warp's 128
+  return GATED ? (c < 64 ? half * 64 + c : 64 + half * 64 + c) : half * 128 + c;
 }
 
 // Reads back this warp's 32 rows and 128 columns of an accumulator and adds them, scaled; `release`
 // hands the accumulator back as soon as the last columns are in registers.
-template <bool GATED, class F>
+// C columns are loaded at a time, the next C while these are added: 32 where the registers allow it.
+template <bool GATED, int C, class F>
 __device__ __forceinline__ void add_step(uint64_t (&sum)[64], uint32_t tbase, int half, float s0, float s1, F&& release) {
   const uint64_t s0p = pack_f2(s0, s0), s1p = pack_f2(s1, s1);
-  uint32_t v[2][16];  // the next 16 columns come while these are added
-  tmem_ld16_start(tbase + tmem_col<GATED>(half, 0), v[0]);
+  uint32_t v[2][C];
+  tmem_ld_start(tbase + tmem_col<GATED>(half, 0), v[0]);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    tmem_ld16_finish(v[j & 1]);
-    if (j < 7)
-      tmem_ld16_start(tbase + tmem_col<GATED>(half, j + 1), v[(j + 1) & 1]);
+  for (int j = 0; j < 128 / C; ++j) {
+    tmem_ld_finish(v[j & 1]);
+    if (j < 128 / C - 1)
+      tmem_ld_start(tbase + tmem_col<GATED>(half, (j + 1) * C), v[(j + 1) & 1]);
     else
       release();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) fma2(sum[j * 8 + i], v[j & 1][2 * i], v[j & 1][2 * i + 1], j < 4 ? s0p : s1p);
+    for (int i = 0; i < C / 2; ++i)
+      fma2(sum[j * (C / 2) + i], v[j & 1][2 * i], v[j & 1][2 * i + 1], j * C < 64 ? s0p : s1p);
   }
 }
 
@@ -443,6 +464,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     blk_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w0,
                     const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ BlkSegs segs,
                     const __grid_constant__ BlkArgs args) {
+  constexpr RegSplit kSplit = GATED ? kEven : kWide;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* out_buf = smem + kPStages * kPStageBytes;
@@ -500,7 +522,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
   const int nk = args.k_blk;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSplit.issue));
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
@@ -579,7 +601,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
   }
   } else {
     // ------------------------------------------------------------------ epilogue (both CTAs)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSums));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSplit.sums));
     const int q = warp & 3;  // TMEM lane quadrant this warp may access
     const int half = (warp - 4) >> 2;
     const uint32_t acce_leader0 = map_to_cta(smem_u32(&acce[0]), 0);
@@ -603,7 +625,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        add_step<GATED>(sum, tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN), half, s0, s1, [&] {
+        add_step<GATED, 32>(sum, tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN), half, s0, s1, [&] {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_remote(acce_leader0 + (uint32_t)(acc * sizeof(uint64_t)));
@@ -666,6 +688,8 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     blk_single_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w0,
                       const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ BlkSegs segs,
                       const __grid_constant__ BlkArgs args, const int tile_m, const int stages, const int ranks) {
+  constexpr RegSplit kSplit = GATED || SPLIT ? kEven : kWide;
+  constexpr int kCols = GATED || SPLIT ? 16 : 32;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   // Rows of x first: an MMA reads 128 of them from the start of a stage's tile_m.
@@ -728,7 +752,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
   // Every role walks the same tiles; with SPLIT all warps of the cluster's CTAs meet twice a tile
   // (sums written; sums read), which also keeps the next tile's operands off the sums.
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSplit.issue));
     int stage = 0, acc = 0;
     uint32_t ph = 0, acc_ph = 0, armed = 0, armed_ph = 0;
     bool ok = true;
@@ -825,7 +849,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     }
   } else {
     // ------------------------------------------------------------------ epilogue
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSums));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSplit.sums));
     if (early) wait_for_previous_kernel();
     const int q = warp & 3, half = (warp - 4) >> 2;
     uint4* st = reinterpret_cast<uint4*>(out_buf + (warp - 4) * 32 * 128);
@@ -851,7 +875,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
         if (!ok) break;
         if (active) {
           tc_fence_after();
-          add_step<GATED>(sum, tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN), half, s0, s1, [&] {
+          add_step<GATED, kCols>(sum, tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN), half, s0, s1, [&] {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acce[acc]);
@@ -878,7 +902,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
 #pragma unroll
           for (int v = 0; v < 32; ++v) {
             const float2 x = unpack_f2(sum[2 * v]), y = unpack_f2(sum[2 * v + 1]);
-            const int unit = (tmem_col<GATED>(half, v >> 2) >> 2) + (v & 3);
+            const int unit = tmem_col<GATED>(half, v * 4) >> 2;
             red[(q * 32 + lane) * 64 + (unit ^ (lane & 7))] = make_float4(x.x, x.y, y.x, y.y);
           }
         }
