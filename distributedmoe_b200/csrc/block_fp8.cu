@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
 // Row tiles of tile_m rows (32, 64 or 128) x 256 weight rows.  The MMA's M is 128: the rows past the
 // tile come from whatever lies behind it in shared memory, give rows of D that nobody reads, and
 // the warps of their quadrants only pass the accumulators on.
-// With SPLIT the CTAs of a cluster take parts of the reduction of the same tile; each leaves its sums
+// With SPLIT the CTAs of a cluster may take parts of the reduction of the same tile; each leaves its sums
 // in its own shared memory (where the operands were) and finishes some of the rows, adding the
 // ranks' sums in order.
 __host__ __device__ constexpr int single_stage_bytes(int tile_m) { return tile_m * kBlk + 2 * kOpBytes; }
@@ -707,9 +707,6 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int rank = SPLIT ? (int)cluster_ctarank() : 0;
-  const int group = SPLIT ? (int)blockIdx.x / ranks : (int)blockIdx.x;
-  const int n_groups = SPLIT ? (int)gridDim.x / ranks : (int)gridDim.x;
 
   if (threadIdx.x == 64) {
     tma_prefetch_map(&tm_w0);
@@ -746,10 +743,25 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int total = tab.tile[segs.n_seg] * args.n_tiles_n;
-  const int kb0 = SPLIT ? (int)((int64_t)args.k_blk * rank / ranks) : 0;
-  const int kb1 = SPLIT ? (int)((int64_t)args.k_blk * (rank + 1) / ranks) : args.k_blk;
+  int group = blockIdx.x, n_groups = gridDim.x, rank = 0, kb0 = 0, kb1 = args.k_blk;
+  bool split = false;
+  if constexpr (SPLIT) {
+    // The host split for the tiles it expected; here they are known.  A tile costs its steps and
+    // about two more, a split one its part of them and about eight for the two meetings.
+    const int clusters = (int)gridDim.x / ranks;
+    const int64_t in_parts = (int64_t)((total + clusters - 1) / clusters) * (args.k_blk / ranks + 8);
+    const int64_t whole = (int64_t)((total + (int)gridDim.x - 1) / (int)gridDim.x) * (args.k_blk + 2);
+    split = in_parts <= whole;
+    if (split) {
+      rank = (int)cluster_ctarank();
+      group = (int)blockIdx.x / ranks;
+      n_groups = clusters;
+      kb0 = (int)((int64_t)args.k_blk * rank / ranks);
+      kb1 = (int)((int64_t)args.k_blk * (rank + 1) / ranks);
+    }
+  }
 
-  // Every role walks the same tiles; with SPLIT all warps of the cluster's CTAs meet twice a tile
+  // Every role walks the same tiles; split, all warps of the cluster's CTAs meet twice a tile
   // (sums written; sums read), which also keeps the next tile's operands off the sums.
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSplit.issue));
@@ -826,7 +838,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
           if (acc == 0) acc_ph ^= 1u;
         }
       }
-      if constexpr (SPLIT) {
+      if (SPLIT && split) {
         __syncwarp();
         cluster_sync_all();
         cluster_sync_all();
@@ -887,7 +899,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
         if (acc == 0) acc_ph ^= 1u;
       }
       // After a wait that ran out nothing is stored, but warps that meet below still do.
-      if constexpr (!SPLIT) {
+      if (!(SPLIT && split)) {
         if (active) {
           if constexpr (GATED)
             store_codes(sum, args, row, ti.row0 + rows, ok, ti.nt, half, q, xch + flip * 256, st);
