@@ -677,9 +677,12 @@ static_assert(32 * kN * 4 <= single_stages(32) * single_stage_bytes(32) &&
                   128 * kN * 4 <= single_stages(128) * single_stage_bytes(128),
               "sums of a split tile");
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -921,42 +924,60 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
         __syncwarp();
         cluster_sync_all();
         const uint32_t red0 = smem_u32(smem);
-        auto total_of = [&](int r, int col) {  // the ranks' sums of one element, in order
-          const uint32_t at = red0 + (uint32_t)((r * 64 + ((col >> 2) ^ (r & 7))) * 16 + (col & 3) * 4);
-          float part[8], v = 0.f;
+        auto total_of = [&](int r, int unit) {  // the ranks' sums of four columns, in order
+          const uint32_t at = red0 + (uint32_t)((r * 64 + (unit ^ (r & 7))) * 16);
+          float4 part[8];
 #pragma unroll
-          for (int g = 0; g < 8; ++g) part[g] = g < ranks ? ld_cluster(map_to_cta(at, (uint32_t)g)) : 0.f;
+          for (int g = 0; g < 8; ++g)
+            part[g] = g < ranks ? ld_cluster(map_to_cta(at, (uint32_t)g)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          float4 v = part[0];
 #pragma unroll
-          for (int g = 0; g < 8; ++g) v += part[g];
+          for (int g = 1; g < 8; ++g) {
+            v.x += part[g].x;
+            v.y += part[g].y;
+            v.z += part[g].z;
+            v.w += part[g].w;
+          }
           return v;
         };
-        const int c = (threadIdx.x - 128) & 127;
-        if constexpr (GATED) {
-          // Rank g finishes rows g, g + ranks, ...; 128 threads a row, one h each.
-          for (int r = rank + half * ranks; r < rows; r += 2 * ranks) {
-            const float g = total_of(r, c);
-            float h = (args.act == DMOE_ACT_SILU ? blk_act<DMOE_ACT_SILU>(g) : blk_act<DMOE_ACT_RELU>(g)) * total_of(r, 128 + c);
-            const float top = finite_abs(h);  // non-negative floats order as their bits
-            const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-            uint32_t* at = xch + (flip * 2 + half) * 4;
-            flip ^= 1;
-            if (lane == 0) at[q] = most;
-            named_sync(1 + half, 128);
-            const float s = block_scale(__uint_as_float(max(max(at[0], at[1]), max(at[2], at[3]))));
-            if (fabsf(h) > kFinite) h = __int_as_float(0x7fffffff);
-            const int col = ti.nt * 128 + c;
+        // Rank g finishes rows g, g + ranks, ... of the tile, a warp a row.
+        for (int r = rank + ranks * (warp - 4); r < rows; r += ranks * kEpiWarps) {
+          const int orow = ti.row0 + r;
+          if constexpr (GATED) {
+            const float4 g4 = total_of(r, lane), u4 = total_of(r, 32 + lane);
+            float h[4] = {g4.x, g4.y, g4.z, g4.w};
+            const float u[4] = {u4.x, u4.y, u4.z, u4.w};
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              h[i] = (args.act == DMOE_ACT_SILU ? blk_act<DMOE_ACT_SILU>(h[i]) : blk_act<DMOE_ACT_RELU>(h[i])) * u[i];
+              top = fmaxf(top, finite_abs(h[i]));
+              if (fabsf(h[i]) > kFinite) h[i] = __int_as_float(0x7fffffff);
+            }
+            // non-negative floats order as their bits
+            const float s = block_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+            const int col = ti.nt * 128 + lane * 4;
             if (ok && col < args.n_out)
-              reinterpret_cast<uint8_t*>(args.out)[(int64_t)(ti.row0 + r) * args.ldo + col] =
-                  __nv_cvt_float_to_fp8(h * __frcp_rn(s), __NV_SATFINITE, __NV_E4M3);
-            if (ok && c == 0) args.out_scale[(int64_t)(ti.row0 + r) * args.os_ld + ti.nt] = s;
-          }
-        } else {
-          const int esz = args.out_dtype == DMOE_F32 ? 4 : 2;
-          const int col = ti.nt * kN + half * 128 + c;
-          for (int r = rank; r < rows; r += ranks) {
-            const float v = total_of(r, half * 128 + c);
-            char* dst = blk_out_row(args, ti.row0 + r, esz);
-            if (ok && dst != nullptr && col < args.n_out) store_from_float(dst, col, v, args.out_dtype);
+              *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(args.out) + (int64_t)orow * args.ldo + col) =
+                  codes4(h, __frcp_rn(s));
+            if (ok && lane == 0) args.out_scale[(int64_t)orow * args.os_ld + ti.nt] = s;
+          } else {
+            const bool f32 = args.out_dtype == DMOE_F32;
+            const float4 y[2] = {total_of(r, lane), total_of(r, 32 + lane)};
+            char* dst = blk_out_row(args, orow, f32 ? 4 : 2);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int col = ti.nt * kN + i * 128 + lane * 4;
+              if (!ok || dst == nullptr || col >= args.n_out) continue;
+              if (f32)
+                *reinterpret_cast<float4*>(dst + (int64_t)col * 4) = y[i];
+              else if (args.out_dtype == DMOE_BF16)
+                *reinterpret_cast<uint2*>(dst + (int64_t)col * 2) =
+                    make_uint2(pack2<DMOE_BF16>(y[i].x, y[i].y), pack2<DMOE_BF16>(y[i].z, y[i].w));
+              else
+                *reinterpret_cast<uint2*>(dst + (int64_t)col * 2) =
+                    make_uint2(pack2<DMOE_F16>(y[i].x, y[i].y), pack2<DMOE_F16>(y[i].z, y[i].w));
+            }
           }
         }
         // The next tile's copies write where the sums were read.
