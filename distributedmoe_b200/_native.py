@@ -94,7 +94,7 @@ SIGNATURES = {
                                                          ctypes.c_int, _vp, _vp, _sz, _vp, _vp]),
     "dmoe_balance_loss_workspace_size": (_sz, []),
     "dmoe_balance_loss": (ctypes.c_int, [_vp, ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
-                                         ctypes.c_int, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+                                         ctypes.c_int, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
     "dmoe_balance_loss_backward": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                   ctypes.c_int, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp]),
     "dmoe_router_logits": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp,
@@ -797,7 +797,7 @@ class Fp8BlockExperts:
         return self
 
     def _set(self, wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale) -> None:
-        self.dev = _one_device(wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale)
+        _one_device(wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale)
         shape = wg_q.shape
         if len(shape) != 3 or wu_q.shape != shape or wd_q.shape != (shape[0], shape[2], shape[1]):
             raise DMoEError("expert stacks must be gate/up [E, I, d] and down [E, d, I]")
@@ -809,8 +809,12 @@ class Fp8BlockExperts:
         _check_weight_blocks(wd_q, wd_scale, (E, d, I), "down")
         self.wg_q, self.wg_scale, self.wu_q, self.wu_scale = wg_q, wg_scale, wu_q, wu_scale
         self.wd_q, self.wd_scale = wd_q, wd_scale
-        self._ptrs = (wg_q.data_ptr(), wg_scale.data_ptr(), wu_q.data_ptr(), wu_scale.data_ptr(), wd_q.data_ptr(),
-                      wd_scale.data_ptr(), E, d, I)
+
+    def _args(self):
+        """Pointers and sizes as the library calls take them."""
+        E, I, d = self.wg_q.shape
+        return (self.wg_q.data_ptr(), self.wg_scale.data_ptr(), self.wu_q.data_ptr(), self.wu_scale.data_ptr(),
+                self.wd_q.data_ptr(), self.wd_scale.data_ptr(), E, d, I)
 
     @property
     def shape(self):
@@ -825,7 +829,8 @@ def grouped_gated_mlp_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, expert
     (rows may be strided); segments and rows_hint as :func:`grouped_matmul_fp8_blocks`; rows outside
     the segments are not written.  Returns Y [rows, d] (a new tensor if not given)."""
     dev = _one_device(xq, x_scale, experts.wg_q, Y)
-    d, I = experts._ptrs[-2:]
+    stacks = experts._args()
+    d, I = stacks[-2:]
     m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, d)
     if Y is None:
         Y = torch.empty(m, d, dtype=torch.bfloat16, device=xq.device)
@@ -835,7 +840,7 @@ def grouped_gated_mlp_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, expert
     ws = torch.empty(nbytes, dtype=torch.uint8, device=xq.device)
     se, sn, n_seg, on_dev, _keep = _segments(seg_expert, seg_end, dev)
     _call(dev, "grouped_gated_mlp_fp8_blocks", lib().dmoe_grouped_gated_mlp_fp8_blocks, xq.data_ptr(), x_ld,
-          x_scale.data_ptr(), xs_ld, *experts._ptrs, se, sn, n_seg, on_dev, m, int(rows_hint), int(act), Y.data_ptr(),
+          x_scale.data_ptr(), xs_ld, *stacks, se, sn, n_seg, on_dev, m, int(rows_hint), int(act), Y.data_ptr(),
           ws.data_ptr(), nbytes, scratch.status(xq.device).data_ptr())
     return Y
 
@@ -850,16 +855,16 @@ class _BalanceLoss(torch.autograd.Function):
         S = 1 if seq_end is None else seq_end.numel()
         code = dtype_code(logits.dtype)
         counts = torch.empty(S * (E + 1) + 1, dtype=torch.int32, device=device)
+        per_expert = torch.empty(S, E, dtype=torch.int32, device=device)  # the caller's own, who may add other ranks' to it
         loss = torch.empty(2, dtype=torch.float32, device=device)
         nbytes = lib().dmoe_balance_loss_workspace_size()
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         _call(dev, "balance_loss", lib().dmoe_balance_loss, logits.data_ptr(), code, idx.data_ptr(), T, E, k, mode,
-              _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes,
+              _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), per_expert.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes,
               scratch.status(device).data_ptr())
         ctx.save_for_backward(logits, seq_end, mask, counts)
         ctx.args = (dev, code, T, E, k, mode, S)
         ctx.set_materialize_grads(False)
-        per_expert = counts.as_strided((S, E), (E, 1))
         ctx.mark_non_differentiable(per_expert)
         balance, z = loss.unbind()
         return balance, z, per_expert
@@ -1118,11 +1123,12 @@ def ep_expert_mlp_fp8_blocks(win: EpWindow, experts: Fp8BlockExperts, seg_expert
     ``ep_fp8_blocks_workspace(cap, I)`` bytes; rows_hint: rows an instance is expected to have."""
     dev = _one_device(experts.wd_q, seg_expert, seg_end, workspace)
     device = seg_expert.device
-    E, d, I = experts._ptrs[-3:]
+    stacks = experts._args()
+    E, d, I = stacks[-3:]
     with torch.cuda.device(dev):
         st = _stream(device)
         tm = _Timed("grouped_gated_mlp", st, device, None if work_rows is None else 6.0 * work_rows * d * I)
-        rc = lib().dmoe_ep_expert_mlp_fp8_blocks(ctypes.byref(win), *experts._ptrs, seg_expert.data_ptr(),
+        rc = lib().dmoe_ep_expert_mlp_fp8_blocks(ctypes.byref(win), *stacks, seg_expert.data_ptr(),
                                                  seg_end.data_ptr(), seg_expert.numel(), int(cap), int(rows_hint),
                                                  int(act), workspace.data_ptr(), workspace.numel(),
                                                  scratch.status(device).data_ptr(), st)

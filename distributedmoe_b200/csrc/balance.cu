@@ -272,13 +272,18 @@ struct Walk {
 
 template <int G, int V, bool SIGMOID, int DT>
 __global__ void __launch_bounds__(kBalThreads)
-    balance_loss_kernel(BalArgs a, int run, float* __restrict__ loss, double* __restrict__ part) {
+    balance_loss_kernel(BalArgs a, int run, float* __restrict__ loss, double* __restrict__ part,
+                        int32_t* __restrict__ counts_out) {
   __shared__ double sums[2][kBalThreads / 32];
   __shared__ int last;
   __shared__ int32_t sh_ends[kSharedEnds];
   const Ends ends = fetch_ends(a, sh_ends);
   int full, tokens;
   totals(a, full, tokens);  // synchronises
+  if (counts_out != nullptr)
+    for (int64_t i = (int64_t)blockIdx.x * kBalThreads + threadIdx.x; i < (int64_t)a.n_seq * a.E;
+         i += (int64_t)gridDim.x * kBalThreads)
+      counts_out[i] = a.counts[i];
   const int lane = threadIdx.x & (G - 1);
   const int group = blockIdx.x * (kBalThreads / G) + threadIdx.x / G;  // takes tokens [t0, t1)
   const int t0 = (int)min((int64_t)group * run, (int64_t)a.T), t1 = (int)min((int64_t)t0 + run, (int64_t)a.T);
@@ -466,6 +471,7 @@ void shape(int T, int per_cta, int* run, int* grid) {
 struct BalOut {
   float* loss;
   double* part;
+  int32_t* counts_out;
   const float* gb;
   const float* gz;
   void* grad;
@@ -479,7 +485,7 @@ int run_balance(const BalArgs& a, const BalOut& o, cudaStream_t st) {
   if (o.backward)
     balance_grad_kernel<G, V, SIGMOID, DT><<<grid, kBalThreads, 0, st>>>(a, run, o.gb, o.gz, o.grad);
   else
-    balance_loss_kernel<G, V, SIGMOID, DT><<<grid, kBalThreads, 0, st>>>(a, run, o.loss, o.part);
+    balance_loss_kernel<G, V, SIGMOID, DT><<<grid, kBalThreads, 0, st>>>(a, run, o.loss, o.part, o.counts_out);
   DMOE_LAUNCH_CHECK();
   return DMOE_OK;
 }
@@ -530,8 +536,8 @@ using namespace dmoe;
 extern "C" size_t dmoe_balance_loss_workspace_size(void) { return kMaxGrid * 2 * sizeof(double); }
 
 extern "C" int dmoe_balance_loss(const void* logits, int dtype, const int64_t* idx, int T, int E, int k, int mode,
-                                 const int32_t* seq_end, int n_seq, const uint8_t* mask, int32_t* counts, float* loss,
-                                 void* workspace, size_t workspace_bytes, int32_t* dev_status, void* stream) {
+                                 const int32_t* seq_end, int n_seq, const uint8_t* mask, int32_t* counts,
+                                 int32_t* counts_out, float* loss, void* workspace, size_t workspace_bytes, int32_t* dev_status, void* stream) {
   clear_error();
   const char* name = "dmoe_balance_loss";
   if (int r = check_balance(name, logits, dtype, T, E, k, mode, seq_end, n_seq, counts)) return r;
@@ -543,6 +549,7 @@ extern "C" int dmoe_balance_loss(const void* logits, int dtype, const int64_t* i
   DMOE_CUDA(cudaMemsetAsync(counts, 0, ((size_t)n_seq * (E + 1) + 1) * 4, st));
   if (T == 0 || n_seq == 0) {
     DMOE_CUDA(cudaMemsetAsync(loss, 0, 8, st));
+    if (counts_out != nullptr && n_seq > 0) DMOE_CUDA(cudaMemsetAsync(counts_out, 0, (size_t)n_seq * E * 4, st));
     return DMOE_OK;
   }
   const BalArgs a{logits, T, E, k, seq_end, n_seq, mask, counts};
@@ -552,7 +559,7 @@ extern "C" int dmoe_balance_loss(const void* logits, int dtype, const int64_t* i
   if (run < least) run = (int)least;
   balance_count_kernel<<<(T + run - 1) / run, kBalThreads, (E + 1) * 4, st>>>(a, idx, run, dev_status);
   DMOE_LAUNCH_CHECK();
-  const BalOut o{loss, reinterpret_cast<double*>(workspace), nullptr, nullptr, nullptr, false};
+  const BalOut o{loss, reinterpret_cast<double*>(workspace), counts_out, nullptr, nullptr, nullptr, false};
   return launch_balance(a, dtype, mode, o, st);
 }
 
@@ -566,6 +573,6 @@ extern "C" int dmoe_balance_loss_backward(const void* logits, int dtype, int T, 
   if (T == 0) return DMOE_OK;
   DMOE_REQUIRE(grad != nullptr && (reinterpret_cast<uintptr_t>(grad) & 3u) == 0, "%s: bad gradient pointer", name);
   const BalArgs a{logits, T, E, k, seq_end, n_seq, mask, const_cast<int32_t*>(counts)};
-  const BalOut o{nullptr, nullptr, g_balance, g_z, grad, true};
+  const BalOut o{nullptr, nullptr, nullptr, g_balance, g_z, grad, true};
   return launch_balance(a, dtype, mode, o, as_stream(stream));
 }

@@ -793,6 +793,8 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
       }
       wait_for_previous_kernel();
       let_next_kernel_start();
+    } else if (early && warp == 1) {
+      wait_for_previous_kernel();  // before its waits for x are timed
     }
     for (int tile = group; tile < total; tile += n_groups) {
       const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
@@ -1194,6 +1196,7 @@ int run_product(Product& p, const BlkSegs& segs, int hint, cudaStream_t stream) 
   // segment that needs a second tile reads its weights twice.
   const int tile_m = rows <= 20 ? 32 : rows <= 40 ? 64 : 128;
   const int m_tiles = row_tiles(segs, tile_m);
+  if (m_tiles == 0) return DMOE_OK;  // a host table without rows
   const int64_t likely = (int64_t)(segs.dev_end ? used * ((rows + tile_m - 1) / tile_m) : m_tiles) * n_tiles;
   const int sms = gemm_usable_sms();
   if (likely * 2 <= sms) {
@@ -1242,6 +1245,13 @@ int fill_blk_segs(const char* name, BlkSegs& s, const int32_t* seg_expert, const
     prev = seg_end[i];
   }
   return DMOE_OK;
+}
+
+// Row and tile numbers are 32-bit: rows leave room for a tile past the last one, tiles for a step of
+// the grid.
+constexpr int64_t kMostRows = INT32_MAX - 1024;
+bool too_many_tiles(int64_t rows, int64_t n_seg, int64_t N) {
+  return (rows / 32 + n_seg) * ((N + 127) / 128) > INT32_MAX - 1024;
 }
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
@@ -1308,7 +1318,7 @@ extern "C" int dmoe_grouped_matmul_fp8_blocks(const void* Xq, int64_t x_ld, cons
   DMOE_REQUIRE(Xq && x_scale && w_q && w_scale && Y && dev_status && seg_expert && seg_end, "%s: null pointer", name);
   DMOE_REQUIRE(aligned16(Xq) && aligned16(w_q) && aligned16(Y), "%s: tensors must be 16-byte aligned", name);
   DMOE_REQUIRE(aligned4(x_scale) && aligned4(w_scale), "%s: scales must be 4-byte aligned", name);
-  DMOE_REQUIRE(((int64_t)m_rows + n_seg) * blocks_of(N) < INT32_MAX, "%s: too many tiles", name);
+  DMOE_REQUIRE(m_rows <= kMostRows && !too_many_tiles(m_rows, n_seg, N), "%s: too many rows or tiles", name);
   static thread_local BlkSegs segs;
   if (int r = fill_blk_segs(name, segs, seg_expert, seg_end, n_seg, seg_on_device, m_rows, E_stack)) return r;
   Product p{Xq, x_ld, w_q, nullptr, E_stack, N, K, {}};
@@ -1340,7 +1350,7 @@ int check_blk_mlp(const char* name, const void* x, const void* wg, const float* 
   DMOE_REQUIRE(aligned4(gs) && aligned4(us) && aligned4(ds), "%s: scales must be 4-byte aligned", name);
   DMOE_REQUIRE(workspace_bytes >= dmoe_grouped_mlp_fp8_blocks_workspace_size((int)m_rows, I), "%s: workspace %zu < %zu bytes",
                name, workspace_bytes, dmoe_grouped_mlp_fp8_blocks_workspace_size((int)m_rows, I));
-  DMOE_REQUIRE((m_rows + n_seg) * blocks_of(d > I ? d : I) < INT32_MAX, "%s: too many tiles", name);
+  DMOE_REQUIRE(m_rows <= kMostRows && !too_many_tiles(m_rows, n_seg, d > I ? d : I), "%s: too many rows or tiles", name);
   return DMOE_OK;
 }
 }  // namespace

@@ -339,8 +339,7 @@ int run_quantize_blocks(const void* x, int64_t batch, int64_t rows, int cols, in
   if (block_rows == 1) {
     const int parts = (cols + kRowLoads<DT> * 256 - 1) / (kRowLoads<DT> * 256);
     const int64_t grid = (batch * rows + kQuantWarps - 1) / kQuantWarps;
-    DMOE_REQUIRE(grid <= INT32_MAX && parts <= 65535, "dmoe_quantize_blocks_e4m3: %lld rows of %d", (long long)(batch * rows),
-                 cols);
+    DMOE_REQUIRE(grid <= INT32_MAX, "dmoe_quantize_blocks_e4m3: %lld rows", (long long)(batch * rows));
     quantize_row_blocks_kernel<DT><<<dim3((unsigned)grid, parts), kQuantWarps * 32, 0, s>>>(x, batch * rows, cols, q,
                                                                                             q_ld, scale, scale_ld);
   } else {
@@ -364,8 +363,8 @@ extern "C" int dmoe_quantize_blocks_e4m3(const void* x, int dtype, int64_t batch
   const char* name = "dmoe_quantize_blocks_e4m3";
   DMOE_REQUIRE(dtype_ok(dtype), "%s: dtype must be f32, f16 or bf16", name);
   DMOE_REQUIRE(block_rows == 1 || block_rows == 128, "%s: block_rows=%d must be 1 or 128", name, block_rows);
-  DMOE_REQUIRE(batch >= 0 && rows >= 0 && cols > 0 && cols % 16 == 0, "%s: cols=%d must be a multiple of 16", name,
-               cols);
+  DMOE_REQUIRE(batch >= 0 && rows >= 0 && cols > 0 && cols <= (1 << 26) && cols % 16 == 0,
+               "%s: cols=%d must be a multiple of 16 up to 2^26", name, cols);
   if (batch == 0 || rows == 0) return DMOE_OK;
   DMOE_REQUIRE(batch <= (INT64_MAX >> 24) / rows, "%s: %lld x %lld rows", name, (long long)batch, (long long)rows);
   DMOE_REQUIRE(x && q && scale, "%s: null pointer", name);

@@ -277,6 +277,7 @@ int dmoe_grouped_gated_mlp_fp8_blocks(const void* Xq, int64_t x_ld, const float*
  *  mask    [T] bytes, 0: the token does not count and its logits are not read; NULL: all count
  *  counts  [n_seq * (E + 1) + 1] int32, written: C [n_seq, E], then the counted tokens n [n_seq],
  *          then a scratch word; the backward call takes it as the forward call left it
+ *  counts_out [n_seq, E] int32 or NULL: C once more, for a caller that goes on to change it
  *  loss    [2] fp32: balance = mean over sequences with tokens of
  *            sum_e (E C[s,e] / (k n[s])) (sum_t p[t,e] / n[s]),
  *          z = mean over counted tokens of logsumexp(l)^2; both 0 without tokens.
@@ -289,8 +290,8 @@ int dmoe_grouped_gated_mlp_fp8_blocks(const void* Xq, int64_t x_ld, const float*
  */
 size_t dmoe_balance_loss_workspace_size(void);
 int dmoe_balance_loss(const void* logits, int dtype, const int64_t* idx, int T, int E, int k, int mode,
-                      const int32_t* seq_end, int n_seq, const uint8_t* mask, int32_t* counts, float* loss,
-                      void* workspace, size_t workspace_bytes, int32_t* dev_status, void* stream);
+                      const int32_t* seq_end, int n_seq, const uint8_t* mask, int32_t* counts, int32_t* counts_out,
+                      float* loss, void* workspace, size_t workspace_bytes, int32_t* dev_status, void* stream);
 int dmoe_balance_loss_backward(const void* logits, int dtype, int T, int E, int k, int mode, const int32_t* seq_end,
                                int n_seq, const uint8_t* mask, const int32_t* counts, const float* g_balance,
                                const float* g_z, void* grad, void* stream);

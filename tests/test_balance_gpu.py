@@ -290,3 +290,26 @@ def test_wrapper_refusals():
         with pytest.raises(N.DMoEError):
             call()
     assert N.balance_loss(l, idx, seq_end=torch.tensor([20], **i32))[2].shape == (1, 8)
+
+
+@gpu
+def test_differentiable_once():
+    N = _nat()
+    l, idx = _case(20, 8, 2, torch.float32, 1)
+    balance, z, _ = N.balance_loss(l, idx)
+    grad, = torch.autograd.grad(balance + z, l, create_graph=True)
+    plain, = torch.autograd.grad(sum(N.balance_loss(l, idx)[:2]), l)
+    assert torch.equal(grad.detach(), plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(grad.sum(), l)
+
+
+@gpu
+def test_counts_are_the_callers():
+    """Adding to the returned counts (other ranks' selections) leaves the gradient as it was."""
+    N = _nat()
+    l, idx = _case(50, 8, 2, torch.float32, 3)
+    want, = torch.autograd.grad(N.balance_loss(l, idx)[0], l)
+    balance, _, counts = N.balance_loss(l, idx)
+    counts += 1000
+    assert torch.equal(torch.autograd.grad(balance, l)[0], want)

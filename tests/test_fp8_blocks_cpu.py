@@ -23,7 +23,7 @@ def _quantize(x=P, dtype=2, batch=1, rows=4, cols=256, block=1, q=P, q_ld=256, s
 
 
 @pytest.mark.parametrize("kw,words", [
-    (dict(dtype=3), "dtype"), (dict(block=64), "block_rows"), (dict(cols=24), "multiple of 16"), (dict(cols=0), "multiple"),
+    (dict(dtype=3), "dtype"), (dict(block=64), "block_rows"), (dict(cols=24), "multiple of 16"), (dict(cols=0), "multiple"), (dict(cols=1 << 27, q_ld=1 << 27, s_ld=1 << 20), "2^26"),
     (dict(rows=-1), "multiple of 16"), (dict(x=None), "null"), (dict(q=None), "null"), (dict(s=None), "null"),
     (dict(x=ODD), "aligned"), (dict(q=ODD), "aligned"), (dict(s=NINE), "aligned"), (dict(q_ld=240), "q_ld"),
     (dict(q_ld=264), "q_ld"), (dict(s_ld=1), "scale_ld"), (dict(block=128, q_ld=272), "packed"),
@@ -54,7 +54,7 @@ def _matmul(x=P, x_ld=256, xs=P, xs_ld=2, w=P, ws=P, E=2, Nn=64, K=256, experts=
     (dict(ws=None), "null"), (dict(y=None), "null"), (dict(status=None), "null"), (dict(x=ODD), "aligned"),
     (dict(w=ODD), "aligned"), (dict(y=ODD), "aligned"), (dict(ws=NINE), "aligned"), (dict(ends=(5, 3)), "segment 1 end"),
     (dict(ends=(3, 9)), "segment 1 end"), (dict(experts=(0, 2)), "expert 2"), (dict(experts=(-1, 0)), "expert -1"),
-    (dict(n=257), "257"), (dict(n=1025, dev=1), "1025"), (dict(m=2**31 - 1, Nn=1 << 20, y_ld=1 << 20), "tiles"),
+    (dict(n=257), "257"), (dict(n=1025, dev=1), "1025"), (dict(m=2**31 - 1), "rows or tiles"), (dict(m=2**30, Nn=1 << 20, y_ld=1 << 20), "tiles"),
 ])
 def test_matmul_refuses(kw, words):
     _refused(_matmul(**kw), words)
@@ -86,9 +86,9 @@ def test_empty_requests_are_fine():
     assert N.lib().dmoe_balance_loss_backward(None, 0, 0, 8, 2, 0, None, 1, None, P, None, None, None, None) == 0
 
 
-def _balance(logits=P, dt=0, idx=P, T=16, E=8, k=2, mode=0, seq=None, n=1, mask=None, counts=P, loss=P, ws=P,
+def _balance(logits=P, dt=0, idx=P, T=16, E=8, k=2, mode=0, seq=None, n=1, mask=None, counts=P, out=None, loss=P, ws=P,
              ws_bytes=1 << 20, status=P):
-    return N.lib().dmoe_balance_loss(logits, dt, idx, T, E, k, mode, seq, n, mask, counts, loss, ws, ws_bytes, status,
+    return N.lib().dmoe_balance_loss(logits, dt, idx, T, E, k, mode, seq, n, mask, counts, out, loss, ws, ws_bytes, status,
                                      None)
 
 

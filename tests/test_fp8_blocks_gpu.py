@@ -255,7 +255,7 @@ def test_matmul_strided_rows(rows):
     N = _nat()
     Nn, K = 264, 400
     xq, xs, wq, ws = _operands(11, rows, 1, Nn, K)
-    wide_q = torch.zeros(rows, K + 48, dtype=torch.uint8, device=DEV)
+    wide_q = torch.full((rows, K + 48), 0x7F, dtype=torch.uint8, device=DEV)  # NaN codes behind each row
     wide_q[:, :K] = xq.view(torch.uint8)
     wide_s = torch.full((rows, 9), float("nan"), device=DEV)
     wide_s[:, 2:2 + xs.shape[1]] = xs
@@ -523,3 +523,31 @@ def test_same_bits_every_time():
         first = N.matmul_fp8_blocks(xq, xs, wq[0], ws[0], out_dtype=torch.float32)
         for _ in range(5):
             assert torch.equal(first, N.matmul_fp8_blocks(xq, xs, wq[0], ws[0], out_dtype=torch.float32))
+
+
+@gpu
+def test_no_rows_and_no_segments():
+    N = _nat()
+    xq, xs, wq, ws = _operands(8, 4, 2, 136, 256)
+    assert N.quantize_blocks_e4m3(torch.empty(0, 256, device=DEV))[0].shape == (0, 256)
+    assert N.matmul_fp8_blocks(xq[:0], xs[:0], wq[0], ws[0]).shape == (0, 136)
+    out = torch.full((4, 136), 2.0, dtype=torch.bfloat16, device=DEV)
+    N.grouped_matmul_fp8_blocks(xq, xs, wq, ws, [], [], out)
+    N.grouped_matmul_fp8_blocks(xq, xs, wq, ws, [0, 1], [0, 0], out)
+    zero = torch.zeros(2, dtype=torch.int32, device=DEV)
+    for hint in (1, 200):
+        N.grouped_matmul_fp8_blocks(xq, xs, wq, ws, zero, zero, out, rows_hint=hint)
+    assert bool((out == 2.0).all())
+    N.check_device_status(torch.device(DEV))
+
+
+@gpu
+def test_replaced_weights_are_used():
+    """An expert stack whose tensors are exchanged is read as it is then."""
+    N = _nat()
+    xq, xs, gq, gs = _operands(1, 6, 1, 272, 256)
+    _, _, dq, dsc = _operands(3, 1, 1, 256, 272)
+    ex = N.Fp8BlockExperts.from_quantized(gq, gs, gq, gs, dq, dsc)
+    first = N.grouped_gated_mlp_fp8_blocks(xq, xs, ex, [0], [6], N.ACT_SILU)
+    ex.wd_scale = dsc * 2
+    assert torch.equal(N.grouped_gated_mlp_fp8_blocks(xq, xs, ex, [0], [6], N.ACT_SILU), first * 2)
