@@ -672,7 +672,9 @@ def _check_weight_blocks(q: torch.Tensor, scale: torch.Tensor, shape: Sequence[i
     """A stack q of this shape [E, N, K] (or [N, K]) and its scales."""
     if q.dtype is not torch.float8_e4m3fn or scale.dtype is not torch.float32:
         raise DMoEError(f"{what} must be float8_e4m3fn with fp32 scales")
-    if scale.shape != (*shape[:-2], -(-shape[-2] // FP8_BLOCK), -(-shape[-1] // FP8_BLOCK)):
+    got = scale.shape
+    if len(got) != len(shape) or got[-1] != -(-shape[-1] // FP8_BLOCK) or got[-2] != -(-shape[-2] // FP8_BLOCK) \
+            or (len(shape) == 3 and got[0] != shape[0]):
         raise DMoEError(f"{what} must be [..., N, K] with scales [..., ceil(N / 128), ceil(K / 128)]")
     if not (q.is_contiguous() and scale.is_contiguous()):
         raise DMoEError("dmoe kernels take contiguous weights")
@@ -709,7 +711,12 @@ def _segments(seg_expert, seg_end, dev: int):
     return ctypes.addressof(a1), ctypes.addressof(a2), n, 0, (a1, a2)
 
 
-def _product(xq, x_scale, w_q, w_scale, w_shape, E, seg_expert, seg_end, out, out_dtype, rows_hint) -> torch.Tensor:
+_Int32 = ctypes.c_int32 * 1
+_FIRST_EXPERT = _Int32(0)
+
+
+def _product(xq, x_scale, w_q, w_scale, w_shape, E, table, out, out_dtype, rows_hint) -> torch.Tensor:
+    """table: (seg_expert, seg_end), or None for one segment of all rows."""
     dev = _one_device(xq, x_scale, w_q, w_scale, out)
     _check_weight_blocks(w_q, w_scale, w_shape, "w_q")
     Nn, K = w_shape[-2:]
@@ -721,7 +728,11 @@ def _product(xq, x_scale, w_q, w_scale, w_shape, E, seg_expert, seg_end, out, ou
         if out.shape != (m, Nn) or (Nn > 1 and out.stride(1) != 1) or (out_dtype is not None and out.dtype != out_dtype):
             raise DMoEError(f"out must be [{m}, {Nn}] with contiguous columns, in out_dtype where that is given")
         y_ld = out.stride(0) if m > 1 else Nn
-    se, sn, n_seg, on_dev, _keep = _segments(seg_expert, seg_end, dev)
+    if table is None:
+        end = _Int32(m)
+        se, sn, n_seg, on_dev = ctypes.addressof(_FIRST_EXPERT), ctypes.addressof(end), 1, 0
+    else:
+        se, sn, n_seg, on_dev, _keep = _segments(*table, dev)
     _call(dev, "grouped_matmul_fp8_blocks", lib().dmoe_grouped_matmul_fp8_blocks, xq.data_ptr(), x_ld,
           x_scale.data_ptr(), xs_ld, w_q.data_ptr(), w_scale.data_ptr(), E, Nn, K, se, sn, n_seg, on_dev, m,
           int(rows_hint), out.data_ptr(), y_ld, dtype_code(out.dtype), scratch.status(xq.device).data_ptr())
@@ -743,7 +754,7 @@ def grouped_matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torc
     shape = w_q.shape
     if len(shape) != 3:
         raise DMoEError("w_q must be [E, N, K]")
-    return _product(xq, x_scale, w_q, w_scale, shape, shape[0], seg_expert, seg_end, out, out_dtype, rows_hint)
+    return _product(xq, x_scale, w_q, w_scale, shape, shape[0], (seg_expert, seg_end), out, out_dtype, rows_hint)
 
 
 def matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
@@ -753,7 +764,7 @@ def matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor
     shape = w_q.shape
     if len(shape) != 2:
         raise DMoEError("w_q must be [N, K]")
-    return _product(xq, x_scale, w_q, w_scale, shape, 1, (0,), (xq.shape[0],), out, out_dtype, 0)
+    return _product(xq, x_scale, w_q, w_scale, shape, 1, None, out, out_dtype, 0)
 
 
 def fp8_block_record_bytes(d: int) -> int:

@@ -270,29 +270,18 @@ struct Walk {
   }
 };
 
+// The loss terms of a group's tokens [t0, t1), in lane 0 of the group; every group of a warp makes
+// `run` steps, since the shuffles span the warp.
 template <int G, int V, bool SIGMOID, int DT>
-__global__ void __launch_bounds__(kBalThreads)
-    balance_loss_kernel(BalArgs a, int run, float* __restrict__ loss, double* __restrict__ part,
-                        int32_t* __restrict__ counts_out) {
-  __shared__ double sums[2][kBalThreads / 32];
-  __shared__ int last;
-  __shared__ int32_t sh_ends[kSharedEnds];
-  const Ends ends = fetch_ends(a, sh_ends);
-  int full, tokens;
-  totals(a, full, tokens);  // synchronises
-  if (counts_out != nullptr)
-    for (int64_t i = (int64_t)blockIdx.x * kBalThreads + threadIdx.x; i < (int64_t)a.n_seq * a.E;
-         i += (int64_t)gridDim.x * kBalThreads)
-      counts_out[i] = a.counts[i];
+__device__ __forceinline__ void token_losses(const BalArgs& a, const Ends& ends, int full, int t0, int t1, int run,
+                                             double& bal, double& zz) {
   const int lane = threadIdx.x & (G - 1);
-  const int group = blockIdx.x * (kBalThreads / G) + threadIdx.x / G;  // takes tokens [t0, t1)
-  const int t0 = (int)min((int64_t)group * run, (int64_t)a.T), t1 = (int)min((int64_t)t0 + run, (int64_t)a.T);
   const int32_t* n_of = a.counts + (int64_t)a.n_seq * a.E;
   Walk<G, V, DT> w(a, ends, t0, t1, lane);
   int loaded = -1;
   float c[V], coef = 0.f;
-  double bal = 0.0, zz = 0.0;
-  for (int i = 0; i < run; ++i) {  // every group makes `run` steps: the shuffles span the warp
+  bal = zz = 0.0;
+  for (int i = 0; i < run; ++i) {
     const bool live = w.live;
     const int s = w.seq;
     float l[V];
@@ -324,36 +313,11 @@ __global__ void __launch_bounds__(kBalThreads)
       zz += (double)r.lse * (double)r.lse;
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    bal += __shfl_xor_sync(0xffffffffu, bal, o);
-    zz += __shfl_xor_sync(0xffffffffu, zz, o);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    sums[0][threadIdx.x >> 5] = bal;
-    sums[1][threadIdx.x >> 5] = zz;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double b = 0.0, z = 0.0;
-    for (int i = 0; i < kBalThreads / 32; ++i) {
-      b += sums[0][i];
-      z += sums[1][i];
-    }
-    part[2 * blockIdx.x] = b;
-    part[2 * blockIdx.x + 1] = z;
-    __threadfence();
-    last = atomicAdd(&a.counts[(int64_t)a.n_seq * (a.E + 1)], 1) == (int)gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  // The last CTA joins the parts, each warp-strided run of them in order, then the warps.
-  double b = 0.0, z = 0.0;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += kBalThreads) {
-    b += __ldcg(&part[2 * i]);
-    z += __ldcg(&part[2 * i + 1]);
-  }
+}
+
+// Sums of two values over the CTA, in a fixed order, by thread 0; `sums` is used again by the next
+// call only after a synchronisation.
+__device__ __forceinline__ void cta_sums(double& b, double& z, double (*sums)[kBalThreads / 32]) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     b += __shfl_xor_sync(0xffffffffu, b, o);
@@ -369,6 +333,133 @@ __global__ void __launch_bounds__(kBalThreads)
     for (int i = 0; i < kBalThreads / 32; ++i) {
       b += sums[0][i];
       z += sums[1][i];
+    }
+  }
+}
+
+template <int G, int V, bool SIGMOID, int DT>
+__global__ void __launch_bounds__(kBalThreads)
+    balance_loss_kernel(BalArgs a, int run, float* __restrict__ loss, double* __restrict__ part,
+                        int32_t* __restrict__ counts_out) {
+  __shared__ double sums[2][kBalThreads / 32];
+  __shared__ int last;
+  __shared__ int32_t sh_ends[kSharedEnds];
+  const Ends ends = fetch_ends(a, sh_ends);
+  int full, tokens;
+  totals(a, full, tokens);  // synchronises
+  if (counts_out != nullptr)
+    for (int64_t i = (int64_t)blockIdx.x * kBalThreads + threadIdx.x; i < (int64_t)a.n_seq * a.E;
+         i += (int64_t)gridDim.x * kBalThreads)
+      counts_out[i] = a.counts[i];
+  const int group = blockIdx.x * (kBalThreads / G) + threadIdx.x / G;
+  const int t0 = (int)min((int64_t)group * run, (int64_t)a.T), t1 = (int)min((int64_t)t0 + run, (int64_t)a.T);
+  double b, z;
+  token_losses<G, V, SIGMOID, DT>(a, ends, full, t0, t1, run, b, z);
+  cta_sums(b, z, sums);
+  if (threadIdx.x == 0) {
+    part[2 * blockIdx.x] = b;
+    part[2 * blockIdx.x + 1] = z;
+    __threadfence();
+    last = atomicAdd(&a.counts[(int64_t)a.n_seq * (a.E + 1)], 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  // The last CTA joins the parts, each thread its strided run of them in order, then the warps.
+  b = z = 0.0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kBalThreads) {
+    b += __ldcg(&part[2 * i]);
+    z += __ldcg(&part[2 * i + 1]);
+  }
+  cta_sums(b, z, sums);
+  if (threadIdx.x == 0) {
+    loss[0] = (float)b;
+    loss[1] = tokens > 0 ? (float)(z / (double)tokens) : 0.f;
+  }
+}
+
+// The whole forward pass in one launch, for problems whose three launches cost more than their work:
+// a cluster of eight CTAs counts its tokens' selections in shared memory, adds the ranks' counts through
+// distributed shared memory and goes on to the losses.
+constexpr int kSmallRanks = 8;
+constexpr int kSmallCounts = 1024;        // n_seq * (E + 1) at most
+constexpr int64_t kSmallLogits = 1 << 15;  // T * E at most: 4096 x 8 takes 12 us against 11 in three launches
+
+__device__ __forceinline__ uint32_t in_rank(const void* p, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void meet_cluster() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int G, int V, bool SIGMOID, int DT>
+__global__ void __launch_bounds__(kBalThreads)
+    balance_small_kernel(BalArgs a, const int64_t* __restrict__ idx, int run, float* __restrict__ loss,
+                         int32_t* __restrict__ counts_out, int32_t* __restrict__ status) {
+  __shared__ double sums[2][kBalThreads / 32];
+  __shared__ double parts[2][kSmallRanks];
+  __shared__ int32_t sh_ends[kSharedEnds];
+  __shared__ int32_t mine[kSmallCounts], all[kSmallCounts];
+  const int rank = blockIdx.x;  // one cluster
+  const Ends ends = fetch_ends(a, sh_ends);
+  const int n = a.n_seq * (a.E + 1);
+  for (int i = threadIdx.x; i < n; i += kBalThreads) mine[i] = 0;
+  __syncthreads();
+  if (rank == 0 && a.seq_end != nullptr) {
+    int bad = 0;
+    for (int s = threadIdx.x; s < a.n_seq; s += kBalThreads) {
+      const int en = a.seq_end[s], before = s > 0 ? a.seq_end[s - 1] : 0;
+      bad |= en < before || en > a.T;
+    }
+    if (bad) atomicOr(status, DMOE_DEVERR_BAD_SEGMENT);
+  }
+  constexpr int kGroups = kBalThreads / G;
+  const int first = min(rank * kGroups * run, a.T), end = min(first + kGroups * run, a.T);
+  for (int i = first * a.k + threadIdx.x; i < end * a.k; i += kBalThreads) {
+    const int t = i / a.k;
+    const int64_t e = idx[i];
+    if (a.mask != nullptr && !a.mask[t]) continue;
+    const int s = ends.of(t);
+    if (s >= a.n_seq) continue;
+    if (e >= 0 && e < a.E) atomicAdd(&mine[s * a.E + (int)e], 1);
+    if (i == t * a.k) atomicAdd(&mine[a.n_seq * a.E + s], 1);  // the token itself, once
+  }
+  meet_cluster();
+  for (int i = threadIdx.x; i < n; i += kBalThreads) {
+    int v[kSmallRanks], sum = 0;
+#pragma unroll
+    for (int r = 0; r < kSmallRanks; ++r)
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[r]) : "r"(in_rank(&mine[i], r)) : "memory");
+#pragma unroll
+    for (int r = 0; r < kSmallRanks; ++r) sum += v[r];
+    all[i] = sum;
+    if (rank == 0) {
+      a.counts[i] = sum;
+      if (counts_out != nullptr && i < a.n_seq * a.E) counts_out[i] = sum;
+    }
+  }
+  BalArgs here = a;
+  here.counts = all;
+  __syncthreads();
+  int full, tokens;
+  totals(here, full, tokens);
+  const int t0 = min(first + (int)(threadIdx.x / G) * run, a.T), t1 = min(t0 + run, end);
+  double b, z;
+  token_losses<G, V, SIGMOID, DT>(here, ends, full, t0, t1, run, b, z);
+  cta_sums(b, z, sums);
+  if (threadIdx.x == 0) {
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_rank(&parts[0][rank], 0)), "d"(b) : "memory");
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_rank(&parts[1][rank], 0)), "d"(z) : "memory");
+  }
+  __syncwarp();
+  meet_cluster();
+  if (rank == 0 && threadIdx.x == 0) {
+    b = z = 0.0;
+    for (int r = 0; r < kSmallRanks; ++r) {
+      b += parts[0][r];
+      z += parts[1][r];
     }
     loss[0] = (float)b;
     loss[1] = tokens > 0 ? (float)(z / (double)tokens) : 0.f;
@@ -469,6 +560,8 @@ void shape(int T, int per_cta, int* run, int* grid) {
 
 // Where the forward (grad NULL) and the backward pass write.
 struct BalOut {
+  const int64_t* small;  // the selections, where one launch does the whole forward pass
+  int32_t* status;
   float* loss;
   double* part;
   int32_t* counts_out;
@@ -481,6 +574,25 @@ struct BalOut {
 template <int G, int V, bool SIGMOID, int DT>
 int run_balance(const BalArgs& a, const BalOut& o, cudaStream_t st) {
   int run, grid;
+  if (o.small != nullptr) {
+    const int per_step = kSmallRanks * (kBalThreads / G);
+    run = (a.T + per_step - 1) / per_step;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kSmallRanks;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(kSmallRanks);
+    cfg.blockDim = dim3(kBalThreads);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    DMOE_CUDA(cudaLaunchKernelEx(&cfg, balance_small_kernel<G, V, SIGMOID, DT>, a, o.small, run, o.loss, o.counts_out,
+                                 o.status));
+    DMOE_LAUNCH_CHECK();
+    return DMOE_OK;
+  }
   shape(a.T, kBalThreads / G, &run, &grid);
   if (o.backward)
     balance_grad_kernel<G, V, SIGMOID, DT><<<grid, kBalThreads, 0, st>>>(a, run, o.gb, o.gz, o.grad);
@@ -546,20 +658,25 @@ extern "C" int dmoe_balance_loss(const void* logits, int dtype, const int64_t* i
                "%s: workspace %zu < %zu bytes or not 8-byte aligned", name, workspace_bytes,
                dmoe_balance_loss_workspace_size());
   cudaStream_t st = as_stream(stream);
+  const BalArgs a{logits, T, E, k, seq_end, n_seq, mask, counts};
+  if (T > 0 && n_seq > 0 && (int64_t)T * E <= kSmallLogits && (int64_t)n_seq * (E + 1) <= kSmallCounts &&
+      n_seq <= kSharedEnds) {
+    const BalOut o{idx, dev_status, loss, nullptr, counts_out, nullptr, nullptr, nullptr, false};
+    return launch_balance(a, dtype, mode, o, st);
+  }
   DMOE_CUDA(cudaMemsetAsync(counts, 0, ((size_t)n_seq * (E + 1) + 1) * 4, st));
   if (T == 0 || n_seq == 0) {
     DMOE_CUDA(cudaMemsetAsync(loss, 0, 8, st));
     if (counts_out != nullptr && n_seq > 0) DMOE_CUDA(cudaMemsetAsync(counts_out, 0, (size_t)n_seq * E * 4, st));
     return DMOE_OK;
   }
-  const BalArgs a{logits, T, E, k, seq_end, n_seq, mask, counts};
   // Runs of at least 1024 selections a CTA: shorter ones spend their time on the histogram.
   int run = (1024 + k - 1) / k;
   const int64_t least = ((int64_t)T + kMaxGrid - 1) / kMaxGrid;
   if (run < least) run = (int)least;
   balance_count_kernel<<<(T + run - 1) / run, kBalThreads, (E + 1) * 4, st>>>(a, idx, run, dev_status);
   DMOE_LAUNCH_CHECK();
-  const BalOut o{loss, reinterpret_cast<double*>(workspace), counts_out, nullptr, nullptr, nullptr, false};
+  const BalOut o{nullptr, nullptr, loss, reinterpret_cast<double*>(workspace), counts_out, nullptr, nullptr, nullptr, false};
   return launch_balance(a, dtype, mode, o, st);
 }
 
@@ -573,6 +690,6 @@ extern "C" int dmoe_balance_loss_backward(const void* logits, int dtype, int T, 
   if (T == 0) return DMOE_OK;
   DMOE_REQUIRE(grad != nullptr && (reinterpret_cast<uintptr_t>(grad) & 3u) == 0, "%s: bad gradient pointer", name);
   const BalArgs a{logits, T, E, k, seq_end, n_seq, mask, const_cast<int32_t*>(counts)};
-  const BalOut o{nullptr, nullptr, nullptr, g_balance, g_z, grad, true};
+  const BalOut o{nullptr, nullptr, nullptr, nullptr, nullptr, g_balance, g_z, grad, true};
   return launch_balance(a, dtype, mode, o, as_stream(stream));
 }
