@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&accf[a], 1);
-      mbar_init(&acce[a], kEpiWarps);
+      mbar_init(&acce[a], tile_m / 32 * 2);  // the warps of the quadrants that a tile can reach
     }
     mbar_init(fin, 1);
     *abort_flag = 0;
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     for (int tile = group; tile < total; tile += n_groups) {
       const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
       const int rows = min(tile_m, ti.row_end - ti.row0);
-      const bool active = q * 32 < rows;  // some row of this quadrant belongs to the tile
+      const bool reached = q * 32 < tile_m, active = q * 32 < rows;  // some row of this quadrant belongs to the tile
       const int row = ti.row0 + q * 32 + lane;
       const bool valid = q * 32 + lane < rows;
       StepScales sc;
@@ -884,7 +884,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
       uint64_t sum[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) sum[i] = 0;
-      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+      for (int kb = kb0; kb < kb1 && ok && reached; ++kb) {
         float s0, s1;
         if (active) sc.take<GATED>(kb, kb1, s0, s1);
         ok = wait_in_line(&accf[acc], acc_ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_EPILOGUE);
