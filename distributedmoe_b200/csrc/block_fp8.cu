@@ -21,7 +21,15 @@
 //           distributed shared memory, in the order of the ranks.
 // The weights are never the M operand, although they have more rows than a decode batch: an MMA takes
 // 123 cycles to load its 128 rows of M whatever N is (128 for N = 256), so 256 weight rows a step
-// cost 4 x 128 cycles as N and 8 x 123 as M.
+// cost 4 x 128 cycles as N and 8 x 123 as M.  For the same reason an accumulator is 256 columns, and
+// TMEM holds two: a step's MMAs (512 cycles) and its way through the epilogue (about 1,000: commit, wake,
+// 128 columns a warp read and added, hand-back) overlap with the next step's and no further.
+//
+// What bounds them, measured on a B200: many rows, a step takes about 720 cycles of 512 (4096 x 14336
+// x 4096 in 216-224 us, 2.2 PFLOP/s, against 174 us for the same loop without scales, one read-back a
+// tile) and the power cap holds the clock at 1.3-1.6 GHz meanwhile; few rows, HBM (512 rows over 32
+// experts of 7168/2048: gate/up 939 MB in 160 us, down 470 MB in 85 us, 5.5-5.9 TB/s); one token
+// through 14336 x 4096, 59 MB in 16 us: 1.3 us to set up, 11 us of memory, 2.7 us to join and leave.
 #include <cuda_fp8.h>
 
 #include "dmoe_common.cuh"
