@@ -210,19 +210,20 @@ struct Raw8 {
 // 1 x 128: a warp takes kRowLoads x 256 consecutive columns of one row, two blocks per load, with all
 // its loads in flight at once.  A scale costs two divisions, some 35 instructions: lane i of each
 // half-warp does those of load i and hands them round, rather than all lanes for every load (8192 x
-// 7168 bf16: 36 us, 5.0 TB/s, against 44; f32 46 us, 6.4 TB/s, HBM's rate).
+// 7168 bf16: 34 us, 5.2 TB/s, against 44; f32 46 us, 6.4 TB/s, HBM's rate).
 template <int DT>
 constexpr int kRowLoads = DT == DMOE_F32 ? 4 : 8;
+constexpr int kRowWarps = 4, kRowCtas = 8;  // warps of a CTA, CTAs an SM: 32 warps at 64 registers (24 at 72: 36 us)
 
 template <int DT>
-__global__ void __launch_bounds__(kQuantWarps * 32)
+__global__ void __launch_bounds__(kRowWarps * 32, kRowCtas)
     quantize_row_blocks_kernel(const void* __restrict__ x, int64_t rows, int cols, uint8_t* __restrict__ q,
                                int64_t q_ld, float* __restrict__ scale, int64_t scale_ld) {
   // The product that follows may set itself up meanwhile; it waits for this kernel's end.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int NL = kRowLoads<DT>;
   const int lane = threadIdx.x & 31, at = lane & 15;
-  const int64_t row = (int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
+  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int c0 = blockIdx.y * (NL * 256) + lane * 8;
   Raw8<DT> raw[NL];
@@ -339,9 +340,9 @@ int run_quantize_blocks(const void* x, int64_t batch, int64_t rows, int cols, in
                         float* scale, int64_t scale_ld, cudaStream_t s) {
   if (block_rows == 1) {
     const int parts = (cols + kRowLoads<DT> * 256 - 1) / (kRowLoads<DT> * 256);
-    const int64_t grid = (batch * rows + kQuantWarps - 1) / kQuantWarps;
+    const int64_t grid = (batch * rows + kRowWarps - 1) / kRowWarps;
     DMOE_REQUIRE(grid <= INT32_MAX, "dmoe_quantize_blocks_e4m3: %lld rows", (long long)(batch * rows));
-    quantize_row_blocks_kernel<DT><<<dim3((unsigned)grid, parts), kQuantWarps * 32, 0, s>>>(x, batch * rows, cols, q,
+    quantize_row_blocks_kernel<DT><<<dim3((unsigned)grid, parts), kRowWarps * 32, 0, s>>>(x, batch * rows, cols, q,
                                                                                             q_ld, scale, scale_ld);
   } else {
     const int64_t row_blocks = (rows + 127) / 128;
