@@ -670,9 +670,9 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
 // Row tiles of tile_m rows (32, 64 or 128) x 256 weight rows.  The MMA's M is 128: the rows past the
 // tile come from whatever lies behind it in shared memory, give rows of D that nobody reads, and
 // the warps of their quadrants only pass the accumulators on.
-// With SPLIT the CTAs of a cluster may take parts of the reduction of the same tile; each leaves its sums
-// in its own shared memory (where the operands were) and finishes some of the rows, adding the
-// ranks' sums in order.
+// With SPLIT the CTAs of a cluster take parts of the reduction of the same tile where whole tiles would
+// leave SMs idle (few tiles, or the last wave of many); each leaves its sums in its own shared memory
+// (where the operands were) and finishes some of the rows, adding the ranks' sums in order.
 __host__ __device__ constexpr int single_stage_bytes(int tile_m) { return tile_m * kBlk + 2 * kOpBytes; }
 constexpr int kSingleFixed = 1024 + kOutBytes + kBarBytes + kXchBytes + kSegTableBytes;
 __host__ __device__ constexpr int single_stages(int tile_m) {
@@ -754,26 +754,30 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int total = tab.tile[segs.n_seg] * args.n_tiles_n;
-  int group = blockIdx.x, n_groups = gridDim.x, rank = 0, kb0 = 0, kb1 = args.k_blk;
-  bool split = false;
+  // Tiles [0, whole) go to one CTA each, in waves of the grid; with SPLIT the last ones, where they
+  // would leave SMs idle, go to a cluster each.  A tile costs its steps and about two more, a split
+  // one its part of them, about eight for the two meetings and more with its rows.
+  const int grid = (int)gridDim.x;
+  int whole = total, rank = 0;
   if constexpr (SPLIT) {
-    // The host split for the tiles it expected; here they are known.  A tile costs its steps and
-    // about two more, a split one its part of them and about eight for the two meetings.
-    const int clusters = (int)gridDim.x / ranks;
-    const int64_t in_parts = (int64_t)((total + clusters - 1) / clusters) * (args.k_blk / ranks + 8);
-    const int64_t whole = (int64_t)((total + (int)gridDim.x - 1) / (int)gridDim.x) * (args.k_blk + 2);
-    split = in_parts <= whole;
-    if (split) {
-      rank = (int)cluster_ctarank();
-      group = (int)blockIdx.x / ranks;
-      n_groups = clusters;
-      kb0 = (int)((int64_t)args.k_blk * rank / ranks);
-      kb1 = (int)((int64_t)args.k_blk * (rank + 1) / ranks);
-    }
+    const int clusters = grid / ranks, left = total % grid;
+    const int part = args.k_blk / ranks + 8 + tile_m / 8;
+    if (left > 0 && (int64_t)((left + clusters - 1) / clusters) * part <= args.k_blk + 2) whole = total - left;
+    rank = (int)cluster_ctarank();
   }
+  const int whole_here = whole > (int)blockIdx.x ? (whole - (int)blockIdx.x + grid - 1) / grid : 0;
+  struct Item {
+    int tile, kb0, kb1;
+    bool parts;
+  };
+  auto item = [&](int it) {  // tile >= total: no more
+    if (!SPLIT || it < whole_here) return Item{it < whole_here ? (int)blockIdx.x + it * grid : total, 0, args.k_blk, false};
+    return Item{whole + (int)blockIdx.x / ranks + (it - whole_here) * (grid / ranks),
+                (int)((int64_t)args.k_blk * rank / ranks), (int)((int64_t)args.k_blk * (rank + 1) / ranks), true};
+  };
 
-  // Every role walks the same tiles; split, all warps of the cluster's CTAs meet twice a tile
-  // (sums written; sums read), which also keeps the next tile's operands off the sums.
+  // Every role walks the same tiles; at a split one all warps of the cluster's CTAs meet twice (sums
+  // written; sums read), which also keeps the next tile's operands off the sums.
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSplit.issue));
     int stage = 0, acc = 0;
@@ -792,11 +796,12 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     };
     int ahead = 0;  // steps of the first tile whose weights were asked for early
     if (early && warp == 0) {
-      if (group < total) {
-        const BlkTile ti = blk_tile(group, args.n_tiles_n, segs.n_seg, tile_m, tab);
-        ahead = min(stages, kb1 - kb0);
+      const Item first = item(0);
+      if (first.tile < total) {
+        const BlkTile ti = blk_tile(first.tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
+        ahead = min(stages, first.kb1 - first.kb0);
         if (elect_one())
-          for (int i = 0; i < ahead; ++i) load_w(ti, kb0 + i, i);
+          for (int i = 0; i < ahead; ++i) load_w(ti, first.kb0 + i, i);
         __syncwarp();
       }
       wait_for_previous_kernel();
@@ -804,8 +809,11 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     } else if (early && warp == 1) {
       wait_for_previous_kernel();  // before its waits for x are timed
     }
-    for (int tile = group; tile < total; tile += n_groups) {
-      const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
+    for (int it = 0;; ++it) {
+      const Item now = item(it);
+      if (now.tile >= total) break;
+      const int kb0 = now.kb0, kb1 = now.kb1;
+      const BlkTile ti = blk_tile(now.tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
       if (warp == 0) {
         // -------------------------------------------------------------- TMA producer
         for (int kb = kb0; kb < kb1 && ok; ++kb) {
@@ -851,7 +859,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
           if (acc == 0) acc_ph ^= 1u;
         }
       }
-      if (SPLIT && split) {
+      if (SPLIT && now.parts) {
         __syncwarp();
         cluster_sync_all();
         cluster_sync_all();
@@ -881,8 +889,11 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
     int acc = 0, flip = 0;
     uint32_t acc_ph = 0;
     bool ok = true;
-    for (int tile = group; tile < total; tile += n_groups) {
-      const BlkTile ti = blk_tile(tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
+    for (int it = 0;; ++it) {
+      const Item now = item(it);
+      if (now.tile >= total) break;
+      const int kb0 = now.kb0, kb1 = now.kb1;
+      const BlkTile ti = blk_tile(now.tile, args.n_tiles_n, segs.n_seg, tile_m, tab);
       const int rows = min(tile_m, ti.row_end - ti.row0);
       const bool reached = q * 32 < tile_m, active = q * 32 < rows;  // some row of this quadrant belongs to the tile
       const int row = ti.row0 + q * 32 + lane;
@@ -912,7 +923,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
         if (acc == 0) acc_ph ^= 1u;
       }
       // After a wait that ran out nothing is stored, but warps that meet below still do.
-      if (!(SPLIT && split)) {
+      if (!(SPLIT && now.parts)) {
         if (active) {
           if constexpr (GATED)
             store_codes(sum, args, row, ti.row0 + rows, ok, ti.nt, half, q, xch + flip * 256, st);
@@ -1228,6 +1239,10 @@ int run_product(Product& p, const BlkSegs& segs, int hint, cudaStream_t stream) 
   const int64_t by_pair = segs.dev_end ? (int64_t)(rows + kPM / 2) * used : (int64_t)row_tiles(segs, kPM) * kPM;
   const int64_t by_single = segs.dev_end ? (int64_t)(rows + 64) * used : (int64_t)row_tiles(segs, 128) * 128;
   if (tile_m == 128 && by_pair * 93 < by_single * 100) return launch_pair<GATED>(p, segs, row_tiles(segs, kPM), stream);
+  // Long reductions: the tiles of a last, partly empty wave are split over two SMs each (1002 rows over
+  // 8 experts at 4096 x 14336: 125 -> 112 us; 8192 over 32 at 2048 x 7168: 172 -> 168).  Short ones lose
+  // more by the cluster launch (500 rows over 8 at 4096 x 4096: 29.8 -> 30.5 us).
+  if (p.args.k_blk >= 48) return launch_single<GATED, true>(p, segs, tile_m, m_tiles, 2, stream);
   return launch_single<GATED, false>(p, segs, tile_m, m_tiles, 1, stream);
 }
 
