@@ -543,10 +543,11 @@ def run_ours(args, dist, rank, world, local_rank):
     graphs = args.cuda_graphs == "on" or (args.cuda_graphs == "auto" and w.name.endswith("decode-moe-layer"))
     graphs = graphs and args.data_plane == "direct"
     fp8 = args.expert_precision == "fp8"
-    if fp8 and args.data_plane != "direct":
-        raise SystemExit("--expert-precision fp8 runs on the direct data plane")
+    blocks = args.expert_precision == "fp8_block"
+    if (fp8 or blocks) and args.data_plane != "direct":
+        raise SystemExit(f"--expert-precision {args.expert_precision} runs on the direct data plane")
     layer = Layer(w, dev, world, rank, parallel, args.data_plane, cuda_graphs=graphs,
-                  expert_precision="fp8" if fp8 else "model")
+                  expert_precision=args.expert_precision if fp8 or blocks else "model")
     moe, x, T, D = layer.moe, layer.x, layer.T, w.d
     x_host = x.cpu().pin_memory()
     y_host = torch.empty(T, D, dtype=torch.bfloat16).pin_memory()
@@ -658,8 +659,10 @@ def run_ours(args, dist, rank, world, local_rank):
         n_act = T * w.k
         movers = {
             "router": (T * D * 2 + w.E * D * 2 + n_act * 12, "x read + router weights + indices/weights out"),
-            "ep_dispatch": (2 * n_act * ((D + 16) if fp8 else D * 2) + n_act * 8,
-                            "routed rows read + written, indices" + (" (8-bit records, d + 16 bytes)" if fp8 else "")),
+            "ep_dispatch": (2 * n_act * ((D + 16) if fp8 else N.fp8_block_record_bytes(D) if blocks else D * 2) + n_act * 8,
+                            "routed rows read + written, indices" + (" (8-bit records, d + 16 bytes)" if fp8 else
+                                                                      " (block-scaled records)" if blocks else "")),
+            "quantize_blocks_e4m3": (T * D * 2 + T * N.fp8_block_record_bytes(D), "tokens read (bf16), records written"),
             "quantize_rows_e4m3": (T * D * 2 + T * (D + 16), "tokens read (bf16), records written"),
             "ep_combine": (n_act * D * 2 + T * D * 2 + n_act * 12, "routed rows read, tokens written, indices"),
             "permute_rows": (None, "task-plane gathers"),
@@ -688,9 +691,10 @@ def run_ours(args, dist, rank, world, local_rank):
         "metric": METRIC, "value": total_tokens / (ms * 1e-3), "unit": "tokens/s", "n_gpus": world,
         "steps": steps, "warmup": args.warmup, "ms_per_step": ms, "higher_is_better": True,
         "scaling": "strong" if (w.strong and parallel == "experts") else "weak",
-        "vs_baseline": None, "dtype": "e4m3 gate/up, bf16 down and combine" if fp8 else "bf16", "data": "synthetic",
+        "vs_baseline": None, "dtype": "e4m3 gate/up, bf16 down and combine" if fp8 else "e4m3 experts (block scales), bf16 combine" if blocks
+        else "bf16", "data": "synthetic",
         "config": dict(w.config(world, parallel, args.data_plane), cuda_graphs=graphs,
-                       **({"expert_precision": "fp8"} if fp8 else {})), "impl": "ours",
+                       **({"expert_precision": args.expert_precision} if fp8 or blocks else {})), "impl": "ours",
         "e2e": {"value": total_tokens / (e2e_ms * 1e-3), "unit": "tokens/s", "ms_per_step": e2e_ms,
                 "h2d_bytes_per_step": total_tokens * D * 2, "d2h_bytes_per_step": total_tokens * D * 2,
                 "copies": "pinned host in/out every step; H2D of step i+1 and D2H of step i-1 on two copy "
@@ -733,12 +737,18 @@ def run_gemm_only(args):
         ends = [min(rows, max(0, c)) for c in cuts]
         ends[-1] = rows
     fp8 = args.expert_precision == "fp8"
+    blocks = args.expert_precision == "fp8_block"
     if fp8:  # operands quantised once, outside the timed region: the GEMM pair alone is timed
         xq, xs = N.quantize_rows_e4m3(X)
         ex = N.Fp8Experts(wg, wu, wd)
+    if blocks:
+        xq, xs = N.quantize_blocks_e4m3(X)
+        ex = N.Fp8BlockExperts(wg, wu, wd)
 
     def launch():
-        if fp8:
+        if blocks:
+            N.grouped_gated_mlp_fp8_blocks(xq, xs, ex, list(range(Eg)), ends, N.ACT_SILU, Y)
+        elif fp8:
             N.grouped_gated_mlp_fp8(xq, xs, ex, list(range(Eg)), ends, N.ACT_SILU, Y)
         else:
             N.grouped_gated_mlp(X, wg, wu, wd, list(range(Eg)), ends, N.ACT_SILU, Y)
@@ -756,7 +766,7 @@ def run_gemm_only(args):
     ms = a.elapsed_time(b) / args.steps
     print(json.dumps({"mode": "gemm", "workload": w.name, "rows": rows, "experts": Eg, "ms_per_launch_pair": ms,
                       "segment_rows": [b - a for a, b in zip([0] + ends[:-1], ends)] if args.gemm_ragged else None,
-                      "precision": "e4m3 gate/up, bf16 down" if fp8 else "bf16",
+                      "precision": "e4m3 gate/up, bf16 down" if fp8 else "e4m3, block scales" if blocks else "bf16",
                       "tflops": 6.0 * rows * D * w.I / (ms * 1e-3) / 1e12}), flush=True)
 
 
@@ -845,8 +855,9 @@ def main():
     ap.add_argument("--mode", default="layer", choices=["layer", "gemm", "movers"],
                     help="gemm: time only the grouped expert MLP; movers: only the router, plan, gather and "
                          "combine (for kernel profiling)")
-    ap.add_argument("--expert-precision", default="bf16", choices=["bf16", "fp8"],
-                    help="fp8: routed experts on 8-bit records and e4m3 gate/up GEMMs (not the headline "
+    ap.add_argument("--expert-precision", default="bf16", choices=["bf16", "fp8", "fp8_block"],
+                    help="fp8: routed experts on 8-bit records and e4m3 gate/up GEMMs; fp8_block: all three "
+                         "projections in e4m3 with a scale for each block of 128 (neither is the headline "
                          "precision: the headline line is bf16)")
     ap.add_argument("--gemm-rows", type=int, default=4096)
     ap.add_argument("--gemm-experts", type=int, default=2)
