@@ -238,13 +238,17 @@ def _one_device(*ts: Optional[torch.Tensor]) -> int:
     return dev
 
 
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _call(dev: int, name: str, fn, *args) -> None:
     """One library call on the current stream of device `dev` (which is its last argument), with
     that device current."""
-    if torch._C._cuda_getDevice() != dev:
+    if _current_device() != dev:
         with torch.cuda.device(dev):
             return _call(dev, name, fn, *args)
-    st = torch._C._cuda_getCurrentRawStream(dev)
+    st = _raw_stream(dev)
     if _timing is not None:
         tm = _Timed(name, st, torch.device("cuda", dev))
         _check(fn(*args, st), "dmoe_" + name)
@@ -650,10 +654,11 @@ def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Te
     cols = shape[-1] if shape else 0
     if cols == 0 or cols % 16:
         raise DMoEError("x must be [..., cols] ([..., rows, cols] for 128 x 128 blocks) with cols a multiple of 16")
-    nb = _blocks(cols)
+    nb = -(-cols // FP8_BLOCK)
     if block_rows == 1:
         batch, rows = 1, x.numel() // cols
-        s_shape = (*shape[:-1], nb)
+        # slices of a torch.Size are slow: the common case does without
+        s_shape = (rows, nb) if len(shape) == 2 else (*shape[:-1], nb)
     elif block_rows == FP8_BLOCK and len(shape) >= 2:
         rows = shape[-2]
         batch = x.numel() // (rows * cols) if rows else 0
@@ -668,13 +673,12 @@ def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Te
     return q, scale
 
 
-def _check_weight_blocks(q: torch.Tensor, scale: torch.Tensor, shape: Sequence[int], what: str) -> None:
-    """A stack q of this shape [E, N, K] (or [N, K]) and its scales."""
+def _check_weight_blocks(q: torch.Tensor, scale: torch.Tensor, E: Optional[int], n: int, k: int, what: str) -> None:
+    """A stack q [E, n, k] (E None: one matrix [n, k]) and its scales."""
     if q.dtype is not torch.float8_e4m3fn or scale.dtype is not torch.float32:
         raise DMoEError(f"{what} must be float8_e4m3fn with fp32 scales")
-    got = scale.shape
-    if len(got) != len(shape) or got[-1] != -(-shape[-1] // FP8_BLOCK) or got[-2] != -(-shape[-2] // FP8_BLOCK) \
-            or (len(shape) == 3 and got[0] != shape[0]):
+    nb, kb = -(-n // FP8_BLOCK), -(-k // FP8_BLOCK)
+    if scale.shape != ((nb, kb) if E is None else (E, nb, kb)):
         raise DMoEError(f"{what} must be [..., N, K] with scales [..., ceil(N / 128), ceil(K / 128)]")
     if not (q.is_contiguous() and scale.is_contiguous()):
         raise DMoEError("dmoe kernels take contiguous weights")
@@ -715,11 +719,10 @@ _Int32 = ctypes.c_int32 * 1
 _FIRST_EXPERT = _Int32(0)
 
 
-def _product(xq, x_scale, w_q, w_scale, w_shape, E, table, out, out_dtype, rows_hint) -> torch.Tensor:
-    """table: (seg_expert, seg_end), or None for one segment of all rows."""
+def _product(xq, x_scale, w_q, w_scale, E, Nn, K, table, out, out_dtype, rows_hint) -> torch.Tensor:
+    """table: (seg_expert, seg_end), or None for one segment of all rows and one matrix w_q (E None)."""
     dev = _one_device(xq, x_scale, w_q, w_scale, out)
-    _check_weight_blocks(w_q, w_scale, w_shape, "w_q")
-    Nn, K = w_shape[-2:]
+    _check_weight_blocks(w_q, w_scale, E, Nn, K, "w_q")
     m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, K)
     if out is None:
         out = torch.empty(m, Nn, dtype=out_dtype or torch.bfloat16, device=xq.device)
@@ -734,7 +737,7 @@ def _product(xq, x_scale, w_q, w_scale, w_shape, E, table, out, out_dtype, rows_
     else:
         se, sn, n_seg, on_dev, _keep = _segments(*table, dev)
     _call(dev, "grouped_matmul_fp8_blocks", lib().dmoe_grouped_matmul_fp8_blocks, xq.data_ptr(), x_ld,
-          x_scale.data_ptr(), xs_ld, w_q.data_ptr(), w_scale.data_ptr(), E, Nn, K, se, sn, n_seg, on_dev, m,
+          x_scale.data_ptr(), xs_ld, w_q.data_ptr(), w_scale.data_ptr(), E or 1, Nn, K, se, sn, n_seg, on_dev, m,
           int(rows_hint), out.data_ptr(), y_ld, dtype_code(out.dtype), scratch.status(xq.device).data_ptr())
     return out
 
@@ -751,20 +754,18 @@ def grouped_matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torc
     f16 or f32; bf16 if not said); rows outside the segments are not written.  rows_hint: rows
     expected per segment where that is not rows / segments (a capacity-sized buffer); it only picks
     the tile shape."""
-    shape = w_q.shape
-    if len(shape) != 3:
+    if w_q.dim() != 3 or w_q.shape[0] == 0:
         raise DMoEError("w_q must be [E, N, K]")
-    return _product(xq, x_scale, w_q, w_scale, shape, shape[0], (seg_expert, seg_end), out, out_dtype, rows_hint)
+    return _product(xq, x_scale, w_q, w_scale, *w_q.shape, (seg_expert, seg_end), out, out_dtype, rows_hint)
 
 
 def matmul_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
                       out: Optional[torch.Tensor] = None, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """xq [rows, K] times the transpose of w_q [N, K], both e4m3 with fp32 scales for each 1 x 128
     and 128 x 128 block: :func:`grouped_matmul_fp8_blocks` with one segment."""
-    shape = w_q.shape
-    if len(shape) != 2:
+    if w_q.dim() != 2:
         raise DMoEError("w_q must be [N, K]")
-    return _product(xq, x_scale, w_q, w_scale, shape, 1, None, out, out_dtype, 0)
+    return _product(xq, x_scale, w_q, w_scale, None, *w_q.shape, None, out, out_dtype, 0)
 
 
 def fp8_block_record_bytes(d: int) -> int:
@@ -815,9 +816,9 @@ class Fp8BlockExperts:
         E, I, d = shape
         if d % 16 or I % 16:
             raise DMoEError(f"8-bit experts need d % 16 == 0 and I % 16 == 0 (d={d}, I={I})")
-        _check_weight_blocks(wg_q, wg_scale, shape, "gate")
-        _check_weight_blocks(wu_q, wu_scale, shape, "up")
-        _check_weight_blocks(wd_q, wd_scale, (E, d, I), "down")
+        _check_weight_blocks(wg_q, wg_scale, E, I, d, "gate")
+        _check_weight_blocks(wu_q, wu_scale, E, I, d, "up")
+        _check_weight_blocks(wd_q, wd_scale, E, d, I, "down")
         self.wg_q, self.wg_scale, self.wu_q, self.wu_scale = wg_q, wg_scale, wu_q, wu_scale
         self.wd_q, self.wd_scale = wd_q, wd_scale
 
