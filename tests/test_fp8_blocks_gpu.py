@@ -230,6 +230,58 @@ def test_product(case, dtype, device_table):
     N.check_device_status(torch.device(DEV))
 
 
+# Rows of three or more segments over 40 tiles of weights and a reduction of 49 blocks: 160 or 200 tiles
+# on 148 SMs, whose last wave is split over pairs of SMs, and 240, whose last wave is too full for it.
+_LAST_WAVES = [[33, 20, 1], [65, 20, 30], [129, 0, 259], [33, 33, 1, 1]]
+
+
+@gpu
+@pytest.mark.parametrize("device_table", [False, True])
+@pytest.mark.parametrize("sizes", _LAST_WAVES, ids=lambda s: "r" + "_".join(map(str, s)))
+def test_product_last_wave(sizes, device_table):
+    """Whole tiles first, then parts of the last ones: twice the same bits, rows behind untouched."""
+    N = _nat()
+    E, Nn, K, rows = 2, 10232, 6160, sum(sizes) + 3
+    xq, xs, wq, ws = _operands(3, rows, E, Nn, K)
+    experts, ends = [i % E for i in range(len(sizes))], _table(sizes)
+    table = (torch.tensor(experts, dtype=torch.int32, device=DEV), torch.tensor(ends, dtype=torch.int32, device=DEV)) \
+        if device_table else (experts, ends)
+    out = torch.full((rows, Nn), 7.0, dtype=torch.float32, device=DEV)
+    N.grouped_matmul_fp8_blocks(xq, xs, wq, ws, *table, out)
+    x, w = _values(xq, xs, 1), _values(wq, ws, 128)
+    a = 0
+    for e, b in zip(experts, ends):
+        if b > a:
+            _check(out[a:b], x[a:b] @ w[e].T, _product_slack(x[a:b].abs(), w[e].abs()), 2.0 ** -23)
+        a = b
+    assert bool((out[a:] == 7.0).all()), "rows behind the last segment stay as they were"
+    assert torch.equal(N.grouped_matmul_fp8_blocks(xq, xs, wq, ws, *table, out_dtype=torch.float32)[:a], out[:a])
+    N.check_device_status(torch.device(DEV))
+
+
+@gpu
+@pytest.mark.parametrize("sizes", _LAST_WAVES, ids=lambda s: "r" + "_".join(map(str, s)))
+def test_gated_mlp_last_wave(sizes):
+    N = _nat()
+    E, d, I, rows = 2, 6160, 5120, sum(sizes)
+    xq, xs, gq, gs = _operands(4, rows, E, I, d)
+    _, _, uq, us = _operands(5, 1, E, I, d)
+    _, _, dq, dsc = _operands(6, 1, E, d, I)
+    ex = N.Fp8BlockExperts.from_quantized(gq, gs, uq, us, dq, dsc)
+    experts, ends = [i % E for i in range(len(sizes))], _table(sizes)
+    Y = N.grouped_gated_mlp_fp8_blocks(xq, xs, ex, experts, ends, N.ACT_SILU)
+    assert torch.equal(Y, N.grouped_gated_mlp_fp8_blocks(xq, xs, ex, experts, ends, N.ACT_SILU))
+    x = _values(xq, xs, 1)
+    wg, wu, wd = _values(gq, gs, 128), _values(uq, us, 128), _values(dq, dsc, 128)
+    a = 0
+    for e, b in zip(experts, ends):
+        if b > a:
+            want, slack = _mlp_reference(x[a:b], wg[e], wu[e], wd[e], True)
+            _check(Y[a:b], want, slack, 2.0 ** -7)
+        a = b
+    N.check_device_status(torch.device(DEV))
+
+
 @gpu
 @pytest.mark.parametrize("hint", [1, 17, 40, 100, 200])
 def test_product_any_tile_shape_for_any_rows(hint):
