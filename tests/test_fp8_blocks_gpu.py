@@ -453,6 +453,31 @@ def test_gated_mlp_what_is_not_finite_stays_in_its_row():
 
 
 @gpu
+@pytest.mark.parametrize("silu", [True, False])
+@pytest.mark.parametrize("rows,d", [(5, 256), (3, 4096), (200, 256), (600, 256)],
+                         ids=["whole", "split", "single", "pair"])
+def test_gated_mlp_nan_in_the_gate_stack_alone(rows, d, silu):
+    """A NaN gate is a NaN h whatever the activation, although the up value is finite: a code of one
+    expert's gate stack and a scale of another's, each kernel and a split tile; the third expert's rows are
+    as without them."""
+    N = _nat()
+    I = 272
+    xq, xs, gq, gs = _operands(1, 3 * rows, 3, I, d)
+    _, _, uq, us = _operands(2, 1, 3, I, d)
+    _, _, dq, dsc = _operands(3, 1, 3, d, I)
+    ex = N.Fp8BlockExperts.from_quantized(gq, gs, uq, us, dq, dsc)
+    act = N.ACT_SILU if silu else N.ACT_RELU
+    table = ([0, 1, 2], [rows, 2 * rows, 3 * rows])
+    clean = N.grouped_gated_mlp_fp8_blocks(xq, xs, ex, *table, act)
+    gq.view(torch.uint8)[0, 5, 7] = 0x7F
+    gs[1, 2, 0] = float("nan")
+    Y = N.grouped_gated_mlp_fp8_blocks(xq, xs, ex, *table, act)
+    assert bool(clean.isfinite().all())
+    assert bool(Y[:2 * rows].isnan().all())
+    assert torch.equal(Y[2 * rows:], clean[2 * rows:])
+
+
+@gpu
 def test_experts_quantised_from_bf16():
     """The whole path a user takes: a bf16 stack quantised once, rows quantised per call, close to
     the bf16 experts within the rounding of e4m3 (half a step, 2^-4, in each of three operands)."""
