@@ -179,13 +179,10 @@ constexpr float kFinite = 3.402823466e38f;
 
 // silu(g) = g / (1 + 2^(-g log2 e)) or relu(g), by the two approximate instructions (2 ulp each; a
 // sigmoid below 2^-126 is 0).  Without flushing, the subnormals that cannot matter here cost as many
-// instructions again.  A NaN gate stays NaN (fmaxf would make it 0).
+// instructions again.
 template <int ACT>
 __device__ __forceinline__ float blk_act(float g) {
-  if constexpr (ACT != DMOE_ACT_SILU) {
-    asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(g));
-    return g;
-  }
+  if constexpr (ACT != DMOE_ACT_SILU) return relu_fn(g);
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.442695041f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));

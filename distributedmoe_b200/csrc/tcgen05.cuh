@@ -213,8 +213,14 @@ __host__ __device__ constexpr uint32_t operand_format() {
   return DT == DMOE_BF16 ? 1u : (DT == DMOE_F32 ? 2u : 0u);
 }
 
+// max(g, 0), NaN for a NaN g (fmaxf would give 0).
+__device__ __forceinline__ float relu_fn(float g) {
+  asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(g));
+  return g;
+}
+
 __device__ __forceinline__ float act_fn(float g, int act) {
-  return act == DMOE_ACT_SILU ? g / (1.f + __expf(-g)) : fmaxf(g, 0.f);
+  return act == DMOE_ACT_SILU ? g / (1.f + __expf(-g)) : relu_fn(g);
 }
 
 // ------------------------------------------------------------------------- CTA pairs and clusters

@@ -518,3 +518,29 @@ def test_layer_with_a_nan_token_keeps_other_tokens_finite():
     assert torch.isnan(y[17]).all()
     rest = torch.cat([y[:17], y[18:]])
     assert torch.isfinite(rest).all()
+
+
+@gpu
+@pytest.mark.parametrize("act", [O.ACT_RELU, O.ACT_SILU])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows", [5, 300, 1030])
+def test_grouped_mlp_nan_in_the_gate_stack_alone(rows, dtype, act):
+    """A NaN gate is a NaN h whatever the activation, although the up value is finite; the other
+    expert's rows are as without it."""
+    N = _nat()
+    X, wg, wu, wd, _, _ = _mlp_case(3, 2, 256, 384, [rows, rows], dtype, act)
+    X, wg, wu, wd = (t.to(DEV) for t in (X[:2 * rows], wg, wu, wd))
+    clean = torch.empty_like(X)
+    N.grouped_gated_mlp(X, wg, wu, wd, [0, 1], [rows, 2 * rows], act, clean)
+    wg[0, 3, 5] = float("nan")
+    Y = torch.empty_like(X)
+    N.grouped_gated_mlp(X, wg, wu, wd, [0, 1], [rows, 2 * rows], act, Y)
+    _status_ok()
+    assert bool(Y[:rows].isnan().all()) and torch.equal(Y[rows:], clean[rows:])
+    if dtype == torch.bfloat16:  # e4m3 gate and up stacks with row scales
+        xq, xs = N.quantize_rows_e4m3(X)
+        ex = N.Fp8Experts(wg.nan_to_num(0.0), wu, wd)
+        ex.wg_q.view(torch.uint8)[0, 3, 5] = 0x7F
+        N.grouped_gated_mlp_fp8(xq, xs, ex, [0, 1], [rows, 2 * rows], act, Y)
+        _status_ok()
+        assert bool(Y[:rows].isnan().all()) and bool(Y[rows:].isfinite().all())
