@@ -245,12 +245,15 @@ __host__ __device__ constexpr uint32_t blk_idesc(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// mbar_wait without a call: the sums held in registers would be spilled around one.
+// mbar_wait without a call: the sums held in registers would be spilled around one.  REMOTE: the
+// arrivals come from the other CTA too, by mbar_arrive_remote.
+template <bool REMOTE = false>
 __device__ __forceinline__ bool wait_in_line(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status,
                                              int code) {
-  if (mbar_try_wait(bar, parity)) return true;
+  auto done = [&] { return REMOTE ? mbar_try_wait_remote(bar, parity) : mbar_try_wait(bar, parity); };
+  if (done()) return true;
   const uint64_t t0 = global_timer_ns();
-  while (!mbar_try_wait(bar, parity)) {
+  while (!done()) {
     if (*abort_flag) return false;
     if (global_timer_ns() - t0 > kWaitTimeoutNs) {
       *abort_flag = 1;
@@ -579,7 +582,7 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
       for (int tile = pair; tile < total && ok; tile += n_pairs) {
         for (int kb = 0; kb < nk; ++kb) {
           ok = wait_in_line(&full[stage], ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA) &&
-               wait_in_line(&acce[acc], acc_ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA);
+               wait_in_line<true>(&acce[acc], acc_ph ^ 1u, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_MMA);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();

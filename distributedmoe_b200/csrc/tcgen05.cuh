@@ -244,11 +244,26 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// Arrive on another CTA's barrier without a cluster-scope release, for a thread that hands over
-// nothing but TMEM columns it has read (its loads have completed): the release waits for all of the
+// Arrive on another CTA's barrier at cluster scope without a release, for a thread that hands over
+// nothing but TMEM columns it has read: tcgen05.wait::ld has completed its loads and
+// tcgen05.fence::before_thread_sync orders them before this arrive.  A release waits for all of the
 // thread's memory operations, more than a thousand cycles in a loop that also loads from memory.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// The other side of it: the arrivals come from both CTAs of a pair, so the wait has cluster scope;
+// tcgen05.fence::after_thread_sync follows before the columns are written again.
+__device__ __forceinline__ bool mbar_try_wait_remote(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {

@@ -603,6 +603,21 @@ def test_same_bits_every_time():
 
 
 @gpu
+def test_pair_products_repeat_and_match():
+    """Several tiles a pair of SMs, each accumulator handed back by both CTAs many times: repeated calls
+    agree bit for bit, and with the definition."""
+    N = _nat()
+    for rows, Nn, K in ((2048, 4104, 2064), (5000, 1032, 400)):
+        xq, xs, wq, ws = _operands(rows, rows, 1, Nn, K)
+        first = N.matmul_fp8_blocks(xq, xs, wq[0], ws[0], out_dtype=torch.float32)
+        x, w = _values(xq, xs, 1), _values(wq, ws, 128)[0]
+        _check(first, x @ w.T, _product_slack(x.abs(), w.abs()), 2.0 ** -23)
+        for _ in range(20):
+            assert torch.equal(first, N.matmul_fp8_blocks(xq, xs, wq[0], ws[0], out_dtype=torch.float32))
+    N.check_device_status(torch.device(DEV))
+
+
+@gpu
 def test_no_rows_and_no_segments():
     N = _nat()
     xq, xs, wq, ws = _operands(8, 4, 2, 136, 256)
