@@ -635,6 +635,13 @@ def grouped_gated_mlp_fp8(Xq: torch.Tensor, x_scale: torch.Tensor, experts: Fp8E
 FP8_BLOCK = 128
 
 
+def _int32(*sizes: int) -> None:
+    """Refuse numbers that the library takes as 32-bit ones and ctypes would wrap."""
+    for n in sizes:
+        if not -0x80000000 <= n <= 0x7FFFFFFF:
+            raise DMoEError(f"{n} is past the 2^31 - 1 that the library takes")
+
+
 def _blocks(n: int) -> int:
     return -(-n // FP8_BLOCK)
 
@@ -654,6 +661,7 @@ def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Te
     cols = shape[-1] if shape else 0
     if cols == 0 or cols % 16:
         raise DMoEError("x must be [..., cols] ([..., rows, cols] for 128 x 128 blocks) with cols a multiple of 16")
+    _int32(cols)
     nb = -(-cols // FP8_BLOCK)
     if block_rows == 1:
         batch, rows = 1, x.numel() // cols
@@ -675,6 +683,7 @@ def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Te
 
 def _check_weight_blocks(q: torch.Tensor, scale: torch.Tensor, E: Optional[int], n: int, k: int, what: str) -> None:
     """A stack q [E, n, k] (E None: one matrix [n, k]) and its scales."""
+    _int32(E or 1, n, k)
     if q.dtype is not torch.float8_e4m3fn or scale.dtype is not torch.float32:
         raise DMoEError(f"{what} must be float8_e4m3fn with fp32 scales")
     nb, kb = -(-n // FP8_BLOCK), -(-k // FP8_BLOCK)
@@ -691,6 +700,7 @@ def _check_row_blocks(xq: torch.Tensor, x_scale: torch.Tensor, K: int) -> Tuple[
     shape, nb = xq.shape, -(-K // FP8_BLOCK)
     if len(shape) != 2 or shape[1] != K or x_scale.shape != (shape[0], nb):
         raise DMoEError(f"xq must be [rows, {K}] with scales [rows, {nb}]")
+    _int32(shape[0])
     a, b = xq.stride(), x_scale.stride()
     if (K > 1 and a[1] != 1) or (nb > 1 and b[1] != 1):
         raise DMoEError("the columns of xq and of its scales must be contiguous")
@@ -705,12 +715,14 @@ def _segments(seg_expert, seg_end, dev: int):
             raise DMoEError("a segment table on the device is two contiguous int32 tensors of one length")
         if seg_expert.get_device() != dev or seg_end.get_device() != dev:
             raise DMoEError(f"the segment table must be on cuda:{dev}")
+        _int32(seg_expert.numel())
         return seg_expert.data_ptr(), seg_end.data_ptr(), seg_expert.numel(), 1, None
     if isinstance(seg_expert, torch.Tensor) or isinstance(seg_end, torch.Tensor):
         raise DMoEError("a segment table is two int32 CUDA tensors or two sequences of numbers")
     n = len(seg_expert)
     if n != len(seg_end):
         raise DMoEError("seg_expert and seg_end differ in length")
+    _int32(n, *map(int, seg_expert), *map(int, seg_end))
     a1, a2 = _i32_array(seg_expert), _i32_array(seg_end)
     return ctypes.addressof(a1), ctypes.addressof(a2), n, 0, (a1, a2)
 
@@ -722,6 +734,7 @@ _FIRST_EXPERT = _Int32(0)
 def _product(xq, x_scale, w_q, w_scale, E, Nn, K, table, out, out_dtype, rows_hint) -> torch.Tensor:
     """table: (seg_expert, seg_end), or None for one segment of all rows and one matrix w_q (E None)."""
     dev = _one_device(xq, x_scale, w_q, w_scale, out)
+    _int32(rows_hint)
     _check_weight_blocks(w_q, w_scale, E, Nn, K, "w_q")
     m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, K)
     if out is None:
@@ -780,6 +793,7 @@ def quantize_block_records(x: torch.Tensor, out: Optional[torch.Tensor] = None) 
     T, d = x.shape
     if d == 0 or d % 16 or not x.is_contiguous():
         raise DMoEError(f"8-bit records need a contiguous x with d % 16 == 0 (d={d})")
+    _int32(d)
     rec = fp8_block_record_bytes(d)
     if out is None:
         out = torch.empty(T, rec, dtype=torch.uint8, device=x.device)
@@ -841,6 +855,7 @@ def grouped_gated_mlp_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, expert
     (rows may be strided); segments and rows_hint as :func:`grouped_matmul_fp8_blocks`; rows outside
     the segments are not written.  Returns Y [rows, d] (a new tensor if not given)."""
     dev = _one_device(xq, x_scale, experts.wg_q, Y)
+    _int32(rows_hint, act)
     stacks = experts._args()
     d, I = stacks[-2:]
     m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, d)
@@ -926,6 +941,7 @@ def balance_loss(logits: torch.Tensor, idx: torch.Tensor, *, mode: int = ROUTER_
         raise DMoEError("seq_end must be an int32 vector")
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != logits.shape[:1]):
         raise DMoEError("mask must be bool [T]")
+    _int32(*logits.shape, idx.shape[1], int(mode), 0 if seq_end is None else seq_end.numel())
     return _BalanceLoss.apply(logits, idx, int(mode), seq_end, mask, dev)
 
 
@@ -1134,6 +1150,7 @@ def ep_expert_mlp_fp8_blocks(win: EpWindow, experts: Fp8BlockExperts, seg_expert
     e4m3 stacks, down projection included; the return rows are bf16.  workspace: uint8, at least
     ``ep_fp8_blocks_workspace(cap, I)`` bytes; rows_hint: rows an instance is expected to have."""
     dev = _one_device(experts.wd_q, seg_expert, seg_end, workspace)
+    _int32(rows_hint, act, seg_expert.numel())
     device = seg_expert.device
     stacks = experts._args()
     E, d, I = stacks[-3:]

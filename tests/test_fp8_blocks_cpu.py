@@ -155,3 +155,42 @@ def test_workspace_sizes():
     assert lib.dmoe_grouped_mlp_fp8_blocks_workspace_size(100, 272) >= 100 * 272 + 100 * 3 * 4
     assert lib.dmoe_grouped_mlp_fp8_blocks_workspace_size(0, 272) > 0
     assert lib.dmoe_balance_loss_workspace_size() % 8 == 0
+
+
+def _huge(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")  # sizes without memory
+
+
+_F8, _F32, _I32, _I64 = torch.float8_e4m3fn, torch.float32, torch.int32, torch.int64
+_PAST = 2**32 + 256  # what a 32-bit argument would take for 256
+
+
+@pytest.mark.parametrize("call", [
+    lambda: N.quantize_blocks_e4m3(_huge(1, _PAST)),
+    lambda: N.quantize_blocks_e4m3(_huge(128, _PAST), 128),
+    lambda: N.quantize_block_records(_huge(1, _PAST)),
+    lambda: N.matmul_fp8_blocks(_huge(_PAST, 16, dtype=_F8), _huge(_PAST, 1, dtype=_F32), _huge(8, 16, dtype=_F8), _huge(1, 1, dtype=_F32)),
+    lambda: N.matmul_fp8_blocks(_huge(4, 16, dtype=_F8), _huge(4, 1, dtype=_F32), _huge(_PAST, 16, dtype=_F8), _huge(_PAST // 128, 1, dtype=_F32)),
+    lambda: N.matmul_fp8_blocks(_huge(4, _PAST, dtype=_F8), _huge(4, _PAST // 128, dtype=_F32), _huge(8, _PAST, dtype=_F8),
+                                _huge(1, _PAST // 128, dtype=_F32)),
+    lambda: N.grouped_matmul_fp8_blocks(_huge(4, 16, dtype=_F8), _huge(4, 1, dtype=_F32), _huge(_PAST, 8, 16, dtype=_F8),
+                                        _huge(_PAST, 1, 1, dtype=_F32), [0], [4]),
+    lambda: N.grouped_matmul_fp8_blocks(_huge(4, 16, dtype=_F8), _huge(4, 1, dtype=_F32), _huge(1, 8, 16, dtype=_F8),
+                                        _huge(1, 1, 1, dtype=_F32), [0], [2**32 + 4]),
+    lambda: N.grouped_matmul_fp8_blocks(_huge(4, 16, dtype=_F8), _huge(4, 1, dtype=_F32), _huge(1, 8, 16, dtype=_F8),
+                                        _huge(1, 1, 1, dtype=_F32), [-2**32], [4]),
+    lambda: N.grouped_matmul_fp8_blocks(_huge(4, 16, dtype=_F8), _huge(4, 1, dtype=_F32), _huge(1, 8, 16, dtype=_F8),
+                                        _huge(1, 1, 1, dtype=_F32), _huge(2**32 + 1, dtype=_I32), _huge(2**32 + 1, dtype=_I32)),
+    lambda: N.balance_loss(_huge(_PAST, 8, dtype=_F32), _huge(_PAST, 2, dtype=_I64)),
+    lambda: N.balance_loss(_huge(4, 2**32 + 8, dtype=_F32), _huge(4, 2, dtype=_I64)),
+    lambda: N.balance_loss(_huge(4, 8, dtype=_F32), _huge(4, 2**32 + 2, dtype=_I64)),
+    lambda: N.balance_loss(_huge(4, 8, dtype=_F32), _huge(4, 2, dtype=_I64), seq_end=_huge(2**32 + 1, dtype=_I32)),
+    lambda: N.balance_loss(_huge(4, 8, dtype=_F32), _huge(4, 2, dtype=_I64), mode=2**32),
+])
+def test_wrappers_refuse_sizes_past_32_bits(call, monkeypatch):
+    """Sizes that the library takes as 32-bit numbers are refused before they would wrap to others."""
+    monkeypatch.setattr(N, "_one_device", lambda *t: 0)
+    monkeypatch.setattr(N, "_call", lambda *a: pytest.fail("a wrapped size reached the library"))
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    with pytest.raises(N.DMoEError, match="2\\^"):
+        call()
