@@ -342,6 +342,7 @@ int run_quantize_blocks(const void* x, int64_t batch, int64_t rows, int cols, in
     const int parts = (cols + kRowLoads<DT> * 256 - 1) / (kRowLoads<DT> * 256);
     const int64_t grid = (batch * rows + kRowWarps - 1) / kRowWarps;
     DMOE_REQUIRE(grid <= INT32_MAX, "dmoe_quantize_blocks_e4m3: %lld rows", (long long)(batch * rows));
+    DMOE_REQUIRE(parts <= 65535, "dmoe_quantize_blocks_e4m3: cols=%d, at most 2^26 - 1024 f32 columns", cols);  // grid.y
     quantize_row_blocks_kernel<DT><<<dim3((unsigned)grid, parts), kRowWarps * 32, 0, s>>>(x, batch * rows, cols, q,
                                                                                             q_ld, scale, scale_ld);
   } else {

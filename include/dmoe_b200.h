@@ -230,7 +230,7 @@ int dmoe_grouped_gated_mlp_fp8(const void* Xq, const float* x_scale, const void*
  *   becomes a NaN code and does not enter amax.
  *   block_rows 1: q rows q_ld bytes apart, scale[row * scale_ld + col / 128] (batch * rows rows);
  *   block_rows 128: q packed, scale [batch, ceil(rows / 128), ceil(cols / 128)].
- *   cols % 16 == 0, q_ld % 16 == 0; x and q 16-byte aligned.
+ *   cols % 16 == 0, cols <= 2^26 (2^26 - 1024 for f32 rows), q_ld % 16 == 0; x and q 16-byte aligned.
  *
  * dmoe_grouped_matmul_fp8_blocks: for the rows r of segment i (as dmoe_grouped_gated_mlp), with
  *   e = seg_expert[i],

@@ -194,3 +194,8 @@ def test_wrappers_refuse_sizes_past_32_bits(call, monkeypatch):
     monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
     with pytest.raises(N.DMoEError, match="2\\^"):
         call()
+
+
+def test_quantize_refuses_rows_wider_than_a_grid():
+    """2^26 columns of f32 are 65,536 CTAs along the row, one more than a grid's y axis has."""
+    _refused(_quantize(dtype=0, rows=1, cols=1 << 26, q_ld=1 << 26, s_ld=1 << 19), "f32 columns")

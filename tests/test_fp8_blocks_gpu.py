@@ -168,6 +168,22 @@ def test_quantize_past_32_bit_offsets():
     del x, q, q2
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantize_widest_row(dtype):
+    N = _nat()
+    cols = 65535 * 1024 if dtype == torch.float32 else 2**26
+    x = torch.zeros(2, cols, dtype=dtype, device=DEV)
+    tail = torch.randn(2, 512, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(dtype)
+    x[:, -512:] = tail
+    q, s = N.quantize_blocks_e4m3(x)
+    rq, rs = _quantize64(tail)
+    assert torch.equal(q[:, -512:].double(), rq) and torch.equal(s[:, -4:].double(), rs)
+    assert int(q[:, :-512].view(torch.uint8).count_nonzero()) == 0 and bool((s[:, :-4] == 1).all())
+    with pytest.raises(N.DMoEError, match="columns|2.26"):
+        N.quantize_blocks_e4m3(torch.zeros(1, cols + 16, dtype=dtype, device=DEV))
+
+
 # ------------------------------------------------------------------------------- products
 def _operands(seed, rows, E, Nn, K):
     g = torch.Generator(device=DEV).manual_seed(seed)
