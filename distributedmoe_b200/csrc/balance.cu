@@ -97,7 +97,8 @@ __global__ void __launch_bounds__(kBalThreads)
       }
       int mine = 0;
       if (a.mask != nullptr) {
-        for (int t = t0 + threadIdx.x; t < t1; t += kBalThreads) mine += a.mask[t] != 0;
+        // unsigned, as i above: a step past t1 may pass 2^31
+        for (unsigned t = (unsigned)t0 + threadIdx.x; t < (unsigned)t1; t += kBalThreads) mine += a.mask[t] != 0;
       } else if (threadIdx.x == 0) {
         mine = t1 - t0;
       }
@@ -259,6 +260,10 @@ struct Walk {
     vec = a.E % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0;
     fetch();
   }
+  __device__ __forceinline__ void next() {
+    if (t < t1) ++t;  // no further: behind the last token t + run may pass 2^31
+    fetch();
+  }
   __device__ __forceinline__ void fetch() {
     while (t < t1 && s < a.n_seq && t >= s_end) {
       ++s;
@@ -287,10 +292,7 @@ __device__ __forceinline__ void token_losses(const BalArgs& a, const Ends& ends,
     float l[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) l[v] = w.l[v];
-    if (i + 1 < run) {
-      ++w.t;
-      w.fetch();
-    }
+    if (i + 1 < run) w.next();
     if (live && loaded != s) {
       loaded = s;
       const float n = (float)n_of[s];
@@ -490,10 +492,7 @@ __global__ void __launch_bounds__(kBalThreads)
     float l[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) l[v] = w.l[v];
-    if (i + 1 < run) {
-      ++w.t;
-      w.fetch();
-    }
+    if (i + 1 < run) w.next();
     if (live && loaded != s) {
       loaded = s;
       const float n = (float)n_of[s];
@@ -674,7 +673,7 @@ extern "C" int dmoe_balance_loss(const void* logits, int dtype, const int64_t* i
   int run = (1024 + k - 1) / k;
   const int64_t least = ((int64_t)T + kMaxGrid - 1) / kMaxGrid;
   if (run < least) run = (int)least;
-  balance_count_kernel<<<(T + run - 1) / run, kBalThreads, (E + 1) * 4, st>>>(a, idx, run, dev_status);
+  balance_count_kernel<<<(unsigned)(((int64_t)T + run - 1) / run), kBalThreads, (E + 1) * 4, st>>>(a, idx, run, dev_status);
   DMOE_LAUNCH_CHECK();
   const BalOut o{nullptr, nullptr, loss, reinterpret_cast<double*>(workspace), counts_out, nullptr, nullptr, nullptr, false};
   return launch_balance(a, dtype, mode, o, st);

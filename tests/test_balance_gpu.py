@@ -313,3 +313,37 @@ def test_counts_are_the_callers():
     balance, _, counts = N.balance_loss(l, idx)
     counts += 1000
     assert torch.equal(torch.autograd.grad(balance, l)[0], want)
+
+
+@gpu
+@pytest.mark.parametrize("masked", [False, True])
+def test_as_many_tokens_as_there_may_be(masked):
+    """T * k = 2^31 - 2: the grid, the last CTA's steps and every index at the limit that is stated.  With
+    one expert the balance is 1 and z the mean of the squared logits."""
+    N = _nat()
+    T = 2**31 - 2
+    g = torch.Generator(device=DEV).manual_seed(3)
+    idx = torch.zeros(T, 1, dtype=torch.int64, device=DEV)
+    l = torch.empty(T, 1, dtype=torch.bfloat16, device=DEV).normal_(generator=g).requires_grad_(True)
+    mask = None
+    if masked:
+        mask = torch.ones(T, dtype=torch.uint8, device=DEV)
+        mask[::3] = 0
+    balance, z, counts = N.balance_loss(l, idx, mask=mask)
+    grad, = torch.autograd.grad(z, l)
+    kept, total = 0, 0.0
+    for a in range(0, T, 2**28):
+        b = min(T, a + 2**28)
+        v = l.detach()[a:b, 0].double() ** 2
+        if masked:
+            v *= mask[a:b]
+        total += float(v.sum())
+        kept += int(mask[a:b].sum()) if masked else b - a
+    N.check_device_status(torch.device(DEV))
+    assert counts.tolist() == [[kept]]
+    assert abs(float(balance.detach()) - 1.0) <= 2.0 ** -18 and abs(float(z.detach()) - total / kept) <= 2.0 ** -18 * (total / kept + 1)
+    for part in (slice(0, 1000), slice(T - 1000, T)):
+        want = 2.0 / kept * l.detach()[part].double()
+        if masked:
+            want *= mask[part, None]
+        assert bool(((grad[part].double() - want).abs() <= (2.0 ** -18 + 2.0 ** -8) * want.abs()).all())
