@@ -893,8 +893,9 @@ class _BalanceLoss(torch.autograd.Function):
         ctx.args = (dev, code, T, E, k, mode, S)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(per_expert)
-        balance, z = loss.unbind()
-        return balance, z, per_expert
+        # The two halves as tensors for themselves: views of `loss` could not be changed in place.
+        balance, z = loss.unsafe_split(1)
+        return balance.squeeze_(), z.squeeze_(), per_expert
 
     @staticmethod
     def backward(ctx, g_balance, g_z, _counts):

@@ -347,3 +347,27 @@ def test_as_many_tokens_as_there_may_be(masked):
         if masked:
             want *= mask[part, None]
         assert bool(((grad[part].double() - want).abs() <= (2.0 ** -18 + 2.0 ** -8) * want.abs()).all())
+
+
+@gpu
+def test_losses_are_the_callers():
+    """Each loss may be changed in place, by itself or for logging, without touching the other one or the
+    gradient that its new value has."""
+    N = _nat()
+    l, idx = _case(50, 8, 2, torch.float32, 3)
+    want_b, want_z, _ = (t.detach().clone() for t in N.balance_loss(l, idx))
+    both, = torch.autograd.grad(sum(N.balance_loss(l, idx)[:2]), l)
+    balance, z, _ = N.balance_loss(l, idx)
+    assert balance.shape == () and z.shape == ()
+    balance *= 0.5
+    assert torch.equal(balance.detach(), want_b * 0.5) and torch.equal(z.detach(), want_z)
+    z *= 0.25
+    balance += z
+    assert torch.equal(balance.detach(), want_b * 0.5 + want_z * 0.25) and torch.equal(z.detach(), want_z * 0.25)
+    grad, = torch.autograd.grad(balance, l)
+    up = [torch.tensor(v, device=DEV) for v in (0.5, 0.25)]
+    assert torch.equal(grad, torch.autograd.grad(N.balance_loss(l, idx)[:2], l, up)[0])
+    balance, z, _ = N.balance_loss(l, idx)
+    balance.detach().zero_()
+    assert float(balance.detach()) == 0 and torch.equal(z.detach(), want_z)
+    assert torch.equal(torch.autograd.grad(balance + z, l)[0], both)
