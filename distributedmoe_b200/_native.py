@@ -238,17 +238,13 @@ def _one_device(*ts: Optional[torch.Tensor]) -> int:
     return dev
 
 
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 def _call(dev: int, name: str, fn, *args) -> None:
     """One library call on the current stream of device `dev` (which is its last argument), with
     that device current."""
-    if _current_device() != dev:
+    if torch._C._cuda_getDevice() != dev:
         with torch.cuda.device(dev):
             return _call(dev, name, fn, *args)
-    st = _raw_stream(dev)
+    st = torch._C._cuda_getCurrentRawStream(dev)
     if _timing is not None:
         tm = _Timed(name, st, torch.device("cuda", dev))
         _check(fn(*args, st), "dmoe_" + name)

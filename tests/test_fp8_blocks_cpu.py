@@ -2,6 +2,8 @@
 is turned down with DMOE_ERR_INVALID and a message before anything reaches a GPU."""
 
 import ctypes
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -199,3 +201,11 @@ def test_wrappers_refuse_sizes_past_32_bits(call, monkeypatch):
 def test_quantize_refuses_rows_wider_than_a_grid():
     """2^26 columns of f32 are 65,536 CTAs along the row, one more than a grid's y axis has."""
     _refused(_quantize(dtype=0, rows=1, cols=1 << 26, q_ld=1 << 26, s_ld=1 << 19), "f32 columns")
+
+
+def test_import_without_cuda_in_torch():
+    """A torch that was built without CUDA lacks these names; the module is imported all the same."""
+    names = ("_cuda_getDevice", "_cuda_getCurrentRawStream")
+    code = f"import torch\nfor n in {names!r}:\n    delattr(torch._C, n)\nimport distributedmoe_b200._native"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
