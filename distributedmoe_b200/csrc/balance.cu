@@ -624,6 +624,8 @@ int launch_balance(const BalArgs& a, int dt, int mode, const BalOut& o, cudaStre
   return mode == DMOE_ROUTER_SOFTMAX ? by_type<false>(a, dt, o, st) : by_type<true>(a, dt, o, st);
 }
 
+uintptr_t value_size(int dtype) { return dtype == DMOE_F32 ? 4 : 2; }
+
 int check_balance(const char* name, const void* logits, int dtype, int T, int E, int k, int mode,
                   const int32_t* seq_end, int n_seq, const void* counts) {
   DMOE_REQUIRE(dtype_ok(dtype), "%s: logits must be f32, f16 or bf16", name);
@@ -634,8 +636,9 @@ int check_balance(const char* name, const void* logits, int dtype, int T, int E,
   DMOE_REQUIRE((int64_t)T * k < INT32_MAX && (int64_t)n_seq * (E + 1) < INT32_MAX, "%s: too many tokens or sequences",
                name);
   DMOE_REQUIRE(counts != nullptr && (T == 0 || logits != nullptr), "%s: null pointer", name);
-  DMOE_REQUIRE((reinterpret_cast<uintptr_t>(logits) & 3u) == 0 && (reinterpret_cast<uintptr_t>(counts) & 3u) == 0,
-               "%s: logits and counts must be 4-byte aligned", name);
+  DMOE_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (value_size(dtype) - 1)) == 0 &&
+                   (reinterpret_cast<uintptr_t>(counts) & 3u) == 0,
+               "%s: logits must be aligned to their type, counts 4-byte aligned", name);
   return DMOE_OK;
 }
 
@@ -687,7 +690,8 @@ extern "C" int dmoe_balance_loss_backward(const void* logits, int dtype, int T, 
   const char* name = "dmoe_balance_loss_backward";
   if (int r = check_balance(name, logits, dtype, T, E, k, mode, seq_end, n_seq, counts)) return r;
   if (T == 0) return DMOE_OK;
-  DMOE_REQUIRE(grad != nullptr && (reinterpret_cast<uintptr_t>(grad) & 3u) == 0, "%s: bad gradient pointer", name);
+  DMOE_REQUIRE(grad != nullptr && (reinterpret_cast<uintptr_t>(grad) & (value_size(dtype) - 1)) == 0,
+               "%s: bad gradient pointer", name);
   const BalArgs a{logits, T, E, k, seq_end, n_seq, mask, const_cast<int32_t*>(counts)};
   const BalOut o{nullptr, nullptr, nullptr, nullptr, nullptr, g_balance, g_z, grad, true};
   return launch_balance(a, dtype, mode, o, as_stream(stream));

@@ -371,3 +371,17 @@ def test_losses_are_the_callers():
     balance.detach().zero_()
     assert float(balance.detach()) == 0 and torch.equal(z.detach(), want_z)
     assert torch.equal(torch.autograd.grad(balance + z, l)[0], both)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E", [(6, 5), (300, 33), (6, 128), (4000, 12)])
+def test_logits_that_start_at_any_value(T, E, dtype):
+    """A contiguous slice whose first value is aligned to its type and to nothing more, small and large."""
+    l, idx = _case(T, E, 2, dtype, E)
+    wide = torch.full((T * E + 9,), float("nan"), dtype=dtype, device=DEV)
+    for at in (1, 3, 4):
+        part = wide[at:at + T * E].view(T, E)
+        part.copy_(l.detach())
+        _check(part.detach().requires_grad_(True), idx, SIGMOID)
+        wide[at:at + T * E] = float("nan")

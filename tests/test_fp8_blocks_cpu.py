@@ -209,3 +209,9 @@ def test_import_without_cuda_in_torch():
     code = f"import torch\nfor n in {names!r}:\n    delattr(torch._C, n)\nimport distributedmoe_b200._native"
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_balance_refuses_logits_off_their_type():
+    for dt, at in ((0, 4098), (1, 4099), (2, 4097)):
+        _refused(_balance(logits=ctypes.c_void_p(at), dt=dt), "aligned")
+        _refused(N.lib().dmoe_balance_loss_backward(P, dt, 4, 8, 2, 0, None, 1, None, P, P, P, ctypes.c_void_p(at), None), "gradient")
