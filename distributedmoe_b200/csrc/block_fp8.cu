@@ -332,6 +332,57 @@ __device__ __forceinline__ void add_step(uint64_t (&sum)[64], uint32_t tbase, in
   }
 }
 
+__device__ __forceinline__ bool normal(float s) { return fabsf(s) >= 1.17549435e-38f && fabsf(s) <= kFinite; }
+
+// x = significand * 2^e with 1 <= |significand| < 2, x finite and not 0.
+__device__ __forceinline__ float significand(float x, int& e) {
+  const bool sub = !normal(x);
+  const int b = __float_as_int(sub ? x * 16777216.f : x);
+  e = ((b >> 23) & 255) - (sub ? 127 + 24 : 127);
+  return __int_as_float((b & 0x807fffff) | 0x3f800000);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+
+// Factors c1 * c2 = x * w where the product is no normal number (else 0 * 0), although the sum of a step's
+// codes (a multiple of 2^-18 below 2^26) times it may be one: c1 has the significands and as much of the
+// exponent as keeps sum * c1 normal, c2 is a power of two (past its range every result is 0 or infinite in
+// fp32).  Zeros, infinities and NaN are taken as they are.
+__device__ __forceinline__ float2 two_factors(float x, float w) {
+  const float s = x * w;
+  if (normal(s)) return make_float2(0.f, 0.f);
+  if (!(fabsf(x) <= kFinite && fabsf(w) <= kFinite) || x == 0.f || w == 0.f) return make_float2(s, 1.f);
+  int ex, ew;
+  const float m = significand(x, ex) * significand(w, ew);
+  const int e = ex + ew, e1 = min(max(e, -96), 96);
+  return make_float2(m * power_of_two(e1), power_of_two(min(max(e - e1, -126), 127)));
+}
+
+// add_step where the product of two scales is no normal number in some lane: sums times the normal products
+// as there, then the others as (sum * c1) * c2.  x, w0, w1: the step's scales, read once more.
+template <bool GATED, class F>
+__device__ __forceinline__ void add_step_any(uint64_t (&sum)[64], uint32_t tbase, int half, const float* x, const float* w0,
+                                             const float* w1, F&& release) {
+  const float xs = __ldg(x);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float w = __ldg(!GATED || j < 4 ? w0 : w1), s = normal(xs * w) ? xs * w : 0.f;
+    const float2 c = two_factors(xs, w);
+    const uint64_t sp = pack_f2(s, s), p1 = pack_f2(c.x, c.x), p2 = pack_f2(c.y, c.y);
+    uint32_t v[16];
+    tmem_ld_start(tbase + tmem_col<GATED>(half, j * 16), v);
+    tmem_ld_finish(v);
+    if (j == 7) release();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint64_t t = 0;
+      fma2(t, v[2 * i], v[2 * i + 1], p1);
+      const float2 f = unpack_f2(t);
+      fma2(sum[j * 8 + i], v[2 * i], v[2 * i + 1], sp);
+      fma2(sum[j * 8 + i], __float_as_uint(f.x), __float_as_uint(f.y), p2);
+    }
+  }
+}
+
 // Results of a tile, the row `row` in each lane.  They go through shared memory (`st`: this warp's
 // 4 KB), so that a store instruction writes runs of 64 or 128 bytes of a few rows rather than 16
 // bytes of 32: 6,300 cycles a tile before, at 256 columns of bf16.
@@ -632,15 +683,23 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
       for (int kb = 0; kb < nk && ok; ++kb) {
         float s0, s1;
         sc.take<GATED>(kb, nk, s0, s1);
-        ok = wait_in_line(&accf[acc], acc_ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_EPILOGUE);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        add_step<GATED, 32>(sum, tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN), half, s0, s1, [&] {
+        const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN);
+        auto release = [&] {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_remote(acce_leader0 + (uint32_t)(acc * sizeof(uint64_t)));
-        });
+        };
+        ok = wait_in_line(&accf[acc], acc_ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_EPILOGUE);
+        // One vote for the wait and the scales: of a large product it costs 2 %, a vote and a branch more 5 %.
+        if (__all_sync(0xffffffffu, ok && normal(s0) && (!GATED || normal(s1)))) {
+          tc_fence_after();
+          add_step<GATED, 32>(sum, at, half, s0, s1, release);
+        } else {
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          add_step_any<GATED>(sum, at, half, sc.x + kb, sc.w0 + kb, sc.w1 + kb, release);
+        }
         acc ^= 1;
         if (acc == 0) acc_ph ^= 1u;
       }
@@ -907,20 +966,27 @@ __global__ void __launch_bounds__(kThreadsBlk, 1)
 #pragma unroll
       for (int i = 0; i < 64; ++i) sum[i] = 0;
       for (int kb = kb0; kb < kb1 && ok && reached; ++kb) {
-        float s0, s1;
+        float s0 = 0.f, s1 = 0.f;
         if (active) sc.take<GATED>(kb, kb1, s0, s1);
+        const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN);
+        auto release = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acce[acc]);
+        };
         ok = wait_in_line(&accf[acc], acc_ph, abort_flag, args.status, DMOE_DEVERR_TIMEOUT_EPILOGUE);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (active) {
+        if (__all_sync(0xffffffffu, ok && active && normal(s0) && (!GATED || normal(s1)))) {  // one vote, as above
           tc_fence_after();
-          add_step<GATED, kCols>(sum, tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kN), half, s0, s1, [&] {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acce[acc]);
-          });
-        } else if (lane == 0) {
-          mbar_arrive(&acce[acc]);
+          add_step<GATED, kCols>(sum, at, half, s0, s1, release);
+        } else {
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (active) {
+            tc_fence_after();
+            add_step_any<GATED>(sum, at, half, sc.x + kb, sc.w0 + kb, sc.w1 + kb, release);
+          } else if (lane == 0) {
+            mbar_arrive(&acce[acc]);
+          }
         }
         acc ^= 1;
         if (acc == 0) acc_ph ^= 1u;

@@ -237,7 +237,8 @@ int dmoe_grouped_gated_mlp_fp8(const void* Xq, const float* x_scale, const void*
  *     Y[r, n] = sum_b x_scale[r, b] * w_scale[e, n / 128, b] * sum_{j in b} Xq[r, j] * w_q[e, n, j]
  *   over the 128-wide blocks b of K.  Xq: rows x_ld bytes apart, x_scale rows xs_ld floats apart;
  *   w_q [E_stack, N, K], w_scale [E_stack, ceil(N / 128), ceil(K / 128)]; Y rows y_ld elements apart
- *   in out_dtype (DMOE_BF16, DMOE_F16, DMOE_F32).  Sums in fp32.  Rows outside the segments are not
+ *   in out_dtype (DMOE_BF16, DMOE_F16, DMOE_F32).  Sums in fp32; the product of two scales may leave fp32's
+ *   normal range where its step's sum brings it back.  Rows outside the segments are not
  *   written.  One segment with E_stack = 1 is a plain linear layer.
  *   N % 8 == 0, K % 16 == 0, x_ld % 16 == 0, y_ld % 8 == 0; codes and Y 16-byte aligned.
  *   rows_hint: rows a segment is expected to have (0: m_rows / n_seg), which picks the tile shape

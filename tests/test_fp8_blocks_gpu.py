@@ -336,6 +336,66 @@ def test_matmul_strided_rows(rows):
     _check(y, x @ w.T, _product_slack(x.abs(), w.abs()), 2.0 ** -7)
 
 
+# Rows, output columns and K that reach each kernel and a split tile.
+_KERNELS = {"whole": (5, 264, 400), "split": (3, 512, 4096), "single": (200, 264, 400), "pair": (600, 264, 400)}
+
+
+@gpu
+@pytest.mark.parametrize("rows,Nn,K", _KERNELS.values(), ids=_KERNELS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_product_of_scales_out_of_range(rows, Nn, K, dtype):
+    """The product of two scales may be below the smallest normal number or past the largest while a step's
+    sum times it is neither: codes reach from 2^-18 to 2^25 a step.  What fp32 holds of a result below
+    2^-126 is a multiple of 2^-149, for each addition."""
+    N = _nat()
+    xq, xs, wq, ws = _operands(3, rows, 1, Nn, K)
+    wq, ws = wq[0], ws[0].clone()
+    xs = torch.full_like(xs, 2.0 ** -70) * (1 + torch.rand(xs.shape, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV))
+    ws[:] = 1.3 * 2.0 ** -66
+    ws[1] = 1.7 * 2.0 ** -75        # results that are subnormal themselves
+    ws[-1, 1:] = 1.1 * 2.0 ** -40   # a column block with both kinds of steps
+    xs[0] = 3e38
+    xq.view(torch.uint8)[0] = 0     # the largest scale over nothing but zeros
+    xs[1] = 2.0 ** 110              # past the largest number times ws[0] ..
+    xq.view(torch.uint8)[1] = 0
+    xq.view(torch.uint8)[1, 3] = 1  # .. the smallest code (2^-9) alone,
+    wq.view(torch.uint8)[:, 3] = 1  # on both sides
+    for scale in (ws, ws * 2.0 ** 100):
+        x, w = _values(xq, xs, 1), _values(wq, scale, 128)
+        y = N.matmul_fp8_blocks(xq, xs, wq, scale, out_dtype=dtype)
+        want, slack = x @ w.T, _product_slack(x.abs(), w.abs()) + (_blocks(K) + 1) * 2.0 ** -149
+        assert bool((y[0] == 0).all())
+        small = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # a step of the output's subnormals
+        _check(y, want, slack + small / 2, torch.finfo(dtype).eps)
+    N.check_device_status(torch.device(DEV))
+
+
+@gpu
+@pytest.mark.parametrize("rows,I,d", _KERNELS.values(), ids=_KERNELS)
+@pytest.mark.parametrize("silu", [True, False])
+def test_gated_mlp_product_of_scales_out_of_range(rows, I, d, silu):
+    """Gate sums near 2^-118, whose products of scales are below 2^-126, and up sums near 2^67 with one
+    such step: h is an ordinary number."""
+    N = _nat()
+    I = I // 16 * 16
+    xq, xs, gq, gs = _operands(1, rows, 1, I, d)
+    _, _, uq, us = _operands(2, 1, 1, I, d)
+    _, _, dq, dsc = _operands(3, 1, 1, d, I)
+    xs[:] = 2.0 ** -70 * (1 + torch.rand(xs.shape, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV))
+    gs[:] = 1.3 * 2.0 ** -64
+    us[:] = 1.1 * 2.0 ** 120
+    us[:, 0, 0] = 1.2 * 2.0 ** -60  # a block that adds next to nothing
+    xs[1] = 2.0 ** 40               # this row's up scales pass the largest number, over zeros
+    xq.view(torch.uint8)[1] = 0
+    ex = N.Fp8BlockExperts.from_quantized(gq, gs, uq, us, dq, dsc)
+    Y = N.grouped_gated_mlp_fp8_blocks(xq, xs, ex, [0], [rows], N.ACT_SILU if silu else N.ACT_RELU)
+    x = _values(xq, xs, 1)
+    want, slack = _mlp_reference(x, _values(gq, gs, 128)[0], _values(uq, us, 128)[0], _values(dq, dsc, 128)[0], silu)
+    assert bool((Y[1] == 0).all())
+    _check(Y, want, slack, 2.0 ** -7)
+    N.check_device_status(torch.device(DEV))
+
+
 @gpu
 @pytest.mark.parametrize("rows", [3, 40, 200])
 def test_product_keeps_nan_in_its_row(rows):
