@@ -1251,7 +1251,7 @@ int launch_single(const Product& p, const BlkSegs& segs, int tile_m, int m_tiles
 // Rows of x that a segment is expected to have: what the caller says, else the mean over the
 // segments that can have any.
 int expected_rows(const BlkSegs& segs, int hint) {
-  if (hint > 0) return hint;
+  if (hint > 0) return hint < segs.m_rows ? hint : segs.m_rows;
   const int used = segs.n_seg < segs.m_rows ? segs.n_seg : segs.m_rows;
   return used > 0 ? (segs.m_rows + used - 1) / used : 0;
 }

@@ -317,6 +317,24 @@ def test_product_any_tile_shape_for_any_rows(hint):
 
 
 @gpu
+@pytest.mark.parametrize("device_table", [False, True])
+def test_product_of_the_largest_hint(device_table):
+    """rows_hint may be any number: one past the rows is as good as the rows."""
+    N = _nat()
+    xq, xs, wq, ws = _operands(5, 90, 2, 520, 784)
+    table = ([1, 0], [40, 90])
+    if device_table:
+        table = tuple(torch.tensor(v, dtype=torch.int32, device=DEV) for v in table)
+    want = N.grouped_matmul_fp8_blocks(xq, xs, wq, ws, *table, rows_hint=90, out_dtype=torch.float32)
+    for hint in (91, 2**30, 2**31 - 1):
+        assert torch.equal(want, N.grouped_matmul_fp8_blocks(xq, xs, wq, ws, *table, rows_hint=hint, out_dtype=torch.float32))
+    x, w = _values(xq, xs, 1), _values(wq, ws, 128)
+    for part, e in ((slice(0, 40), 1), (slice(40, 90), 0)):
+        _check(want[part], x[part] @ w[e].T, _product_slack(x[part].abs(), w[e].abs()), 2.0 ** -23)
+    N.check_device_status(torch.device(DEV))
+
+
+@gpu
 @pytest.mark.parametrize("rows", [1, 16, 100, 200])
 def test_matmul_strided_rows(rows):
     """Codes, scales and output whose rows are parts of wider rows."""
