@@ -800,10 +800,27 @@ def quantize_block_records(x: torch.Tensor, out: Optional[torch.Tensor] = None) 
     return out
 
 
+def _replaceable(slot: str) -> property:
+    """A tensor of a stack, which may be exchanged for one of the same shape, type and device: calls take
+    its pointer as it is then."""
+
+    def put(self, t: torch.Tensor) -> None:
+        old = getattr(self, slot)
+        if t.shape != old.shape or t.dtype is not old.dtype or t.get_device() != old.get_device() or not t.is_contiguous():
+            raise DMoEError(f"{slot[1:]} may be replaced by a contiguous {old.dtype} tensor of shape {list(old.shape)} on its device")
+        setattr(self, slot, t)
+
+    return property(lambda self: getattr(self, slot), put)
+
+
 class Fp8BlockExperts:
     """An expert stack whose three projections are e4m3 with one fp32 scale for each 128 x 128
     block: quantised here from 16- or 32-bit stacks, or taken as a checkpoint holds them
     (:meth:`from_quantized`)."""
+
+    wg_q, wg_scale = _replaceable("_wg_q"), _replaceable("_wg_scale")
+    wu_q, wu_scale = _replaceable("_wu_q"), _replaceable("_wu_scale")
+    wd_q, wd_scale = _replaceable("_wd_q"), _replaceable("_wd_scale")
 
     def __init__(self, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> None:
         self._set(*quantize_blocks_e4m3(w_gate.contiguous(), FP8_BLOCK),
@@ -829,14 +846,14 @@ class Fp8BlockExperts:
         _check_weight_blocks(wg_q, wg_scale, E, I, d, "gate")
         _check_weight_blocks(wu_q, wu_scale, E, I, d, "up")
         _check_weight_blocks(wd_q, wd_scale, E, d, I, "down")
-        self.wg_q, self.wg_scale, self.wu_q, self.wu_scale = wg_q, wg_scale, wu_q, wu_scale
-        self.wd_q, self.wd_scale = wd_q, wd_scale
+        self._wg_q, self._wg_scale, self._wu_q, self._wu_scale = wg_q, wg_scale, wu_q, wu_scale
+        self._wd_q, self._wd_scale = wd_q, wd_scale
 
     def _args(self):
         """Pointers and sizes as the library calls take them."""
-        E, I, d = self.wg_q.shape
-        return (self.wg_q.data_ptr(), self.wg_scale.data_ptr(), self.wu_q.data_ptr(), self.wu_scale.data_ptr(),
-                self.wd_q.data_ptr(), self.wd_scale.data_ptr(), E, d, I)
+        E, I, d = self._wg_q.shape
+        return (self._wg_q.data_ptr(), self._wg_scale.data_ptr(), self._wu_q.data_ptr(), self._wu_scale.data_ptr(),
+                self._wd_q.data_ptr(), self._wd_scale.data_ptr(), E, d, I)
 
     @property
     def shape(self):

@@ -215,3 +215,22 @@ def test_balance_refuses_logits_off_their_type():
     for dt, at in ((0, 4098), (1, 4099), (2, 4097)):
         _refused(_balance(logits=ctypes.c_void_p(at), dt=dt), "aligned")
         _refused(N.lib().dmoe_balance_loss_backward(P, dt, 4, 8, 2, 0, None, 1, None, P, P, P, ctypes.c_void_p(at), None), "gradient")
+
+
+def test_replaced_weights_are_checked(monkeypatch):
+    """Calls take the stacks' pointers as they are then, so what replaces one has to be like it."""
+    monkeypatch.setattr(N, "_one_device", lambda *t: 0)
+
+    def stack(*shape):
+        return torch.zeros(*shape, dtype=_F8), torch.ones(shape[0], -(-shape[1] // 128), -(-shape[2] // 128))
+
+    (gq, gs), (dq, ds) = stack(2, 272, 256), stack(2, 256, 272)
+    ex = N.Fp8BlockExperts.from_quantized(gq, gs, gq, gs, dq, ds)
+    for name, t in (("wd_scale", torch.ones(2, 2, 2)), ("wd_scale", ds.double()), ("wg_q", gq.float()), ("wu_q", gq[:1]),
+                    ("wd_q", gq), ("wg_scale", torch.ones(2, 2, 3).transpose(1, 2)), ("wu_scale", gs.to("meta"))):
+        if t.is_meta:
+            monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1 if t.is_meta else -1)
+        with pytest.raises(N.DMoEError, match=name):
+            setattr(ex, name, t)
+    ex.wd_scale = ds * 2
+    assert torch.equal(ex.wd_scale, ds * 2) and ex._args()[5] == ex.wd_scale.data_ptr()
