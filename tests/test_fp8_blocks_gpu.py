@@ -530,6 +530,35 @@ def test_gated_mlp(case, silu):
 
 
 @gpu
+@pytest.mark.parametrize("hint", [0, 17, 100, 200])
+@pytest.mark.parametrize("case", list(_mlp_cases()), ids=lambda c: f"E{c[0]}d{c[1]}I{c[2]}r{sum(c[3])}s{len(c[3])}")
+def test_gated_mlp_device_table(case, hint):
+    """A table on the device has its own choice of tiles: each element against the definition, as a host
+    table's."""
+    N = _nat()
+    E, d, I, sizes, behind = case
+    rows = sum(sizes) + behind
+    xq, xs, gq, gs = _operands(d + I, rows, E, I, d)
+    _, _, uq, us = _operands(d + I + 1, 1, E, I, d)
+    _, _, dq, dsc = _operands(d + I + 2, 1, E, d, I)
+    ex = N.Fp8BlockExperts.from_quantized(gq, gs, uq, us, dq, dsc)
+    experts, ends = [(3 * i + 1) % E for i in range(len(sizes))], _table(sizes)
+    Y = torch.full((rows, d), 7.0, dtype=torch.bfloat16, device=DEV)
+    N.grouped_gated_mlp_fp8_blocks(xq, xs, ex, torch.tensor(experts, dtype=torch.int32, device=DEV),
+                                   torch.tensor(ends, dtype=torch.int32, device=DEV), N.ACT_SILU, Y, rows_hint=hint)
+    x = _values(xq, xs, 1)
+    wg, wu, wd = _values(gq, gs, 128), _values(uq, us, 128), _values(dq, dsc, 128)
+    a = 0
+    for e, b in zip(experts, ends):
+        if b > a:
+            want, slack = _mlp_reference(x[a:b], wg[e], wu[e], wd[e], True)
+            _check(Y[a:b], want, slack, 2.0 ** -7)
+        a = b
+    assert bool((Y[a:] == 7.0).all()), "rows behind the last segment stay as they were"
+    N.check_device_status(torch.device(DEV))
+
+
+@gpu
 def test_gated_mlp_what_is_not_finite_stays_in_its_row():
     N = _nat()
     for rows in (5, 200):
@@ -606,6 +635,33 @@ def test_bad_device_table_is_reported():
             assert (out[:10].double() - good[:10].double()).abs().max() <= 0.01 * good.double().abs().max()
             assert (out[first:].double() - good[first:].double()).abs().max() <= 0.01 * good.double().abs().max()
             assert bool((out[10:first] == 3.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("hint", [1, 30, 200])
+@pytest.mark.parametrize("experts,ends,parts", [
+    ([0, 5, 1], [10, 10, 40], [(0, 0, 10), (1, 10, 40)]),
+    ([0, 1], [10, 4000], [(0, 0, 10), (1, 10, 40)]),
+    ([0, 1, 1], [10, 5, 40], [(0, 0, 10), (1, 10, 40)]),
+    ([0, -3, 1], [10, 12, 40], [(0, 0, 10), (1, 12, 40)]),
+    ([1, 0], [-7, 40], [(0, 0, 40)]),
+    ([2, 1], [2**31 - 1, 40], []),
+])
+def test_what_a_bad_device_table_leaves(experts, ends, parts, hint):
+    """The rows that remain after clamping, each against the definition; all others as they were."""
+    N = _nat()
+    xq, xs, wq, ws = _operands(8, 40, 2, 136, 256)
+    x, w = _values(xq, xs, 1), _values(wq, ws, 128)
+    out = torch.full((40, 136), 3.0, dtype=torch.bfloat16, device=DEV)
+    N.grouped_matmul_fp8_blocks(xq, xs, wq, ws, torch.tensor(experts, dtype=torch.int32, device=DEV),
+                                torch.tensor(ends, dtype=torch.int32, device=DEV), out, rows_hint=hint)
+    with pytest.raises(N.DMoEError, match="segment"):
+        N.check_device_status(torch.device(DEV))
+    left = torch.ones(40, dtype=torch.bool, device=DEV)
+    for e, a, b in parts:
+        _check(out[a:b], x[a:b] @ w[e].T, _product_slack(x[a:b].abs(), w[e].abs()), 2.0 ** -7)
+        left[a:b] = False
+    assert bool((out[left] == 3.0).all())
 
 
 @gpu
