@@ -20,6 +20,7 @@ import torch.nn as nn
 import zmq
 import zmq.asyncio
 
+from distributedmoe_b200 import _native as N
 from distributedmoe_b200.MoE.DistMoE import P2PHeaders
 from distributedmoe_b200.MoE.DistMoEBlock import ACTIVATIONS, DistMoEBlockConfig
 from distributedmoe_b200.MoE.PipelineTask import ExpertsBlockPipelineTask
@@ -85,8 +86,9 @@ class DistExpertsBlock(nn.Module):
                 self.expert_layers[e] = layer
             gate, up, down = stack_expert_weights(expert_layers, self.device, self.dtype)
         else:
-            # Weights already stacked on the device ([E_b, I, d], [E_b, I, d], [E_b, d, I]).
-            gate, up, down = stacked_weights
+            # Weights already stacked on the device ([E_b, I, d], [E_b, I, d], [E_b, d, I]); 8-bit codes
+            # (Fp8BlockExperts) are for the device-driven plane, where the host's side computes.
+            gate, up, down = (None,) * 3 if isinstance(stacked_weights, N.Fp8BlockExperts) else stacked_weights
         position = {e: i for i, e in enumerate(experts)}
         self.experts_combine_layer = (position, gate, up, down)
 

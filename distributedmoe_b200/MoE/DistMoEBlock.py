@@ -578,14 +578,20 @@ class DistMoEBlock(nn.Module):
         the reference's benchmark offers "fp8" as a whole-layer 8-bit cast,
         src/python/MoE/benchmarks/bench.py:184-185); or "fp8_block": e4m3 with one scale for each
         128 x 128 block of all three projections and for each 128 values of a token row, the form
-        in which 8-bit checkpoints are published (bf16 layers, hidden and inner % 16 == 0)."""
+        in which 8-bit checkpoints are published (bf16 layers, hidden and inner % 16 == 0);
+        local_stack may then be such a checkpoint's codes and scales themselves, an
+        Fp8BlockExperts of this rank's S instances."""
         tte = self.tensor_transfer_engine
         if not getattr(tte, "direct", False):
             raise RuntimeError("the device-driven data plane needs the NVLinkDirect backend")
         E, k, d = self.number_of_experts, self.top_k, self.hidden_features
         inst = InstanceTable.from_blocks(self.expert_blocks, block_ranks, world, E)
         n_local = inst.local_count(rank)
-        g, u, dn = local_stack
+        codes = local_stack if isinstance(local_stack, N.Fp8BlockExperts) else None
+        if codes is not None and (expert_precision != "fp8_block" or codes.device != self.device):
+            raise ValueError(f"a stack of 8-bit codes runs on its own GPU with expert_precision 'fp8_block', not "
+                             f"{expert_precision!r} on {self.device}")
+        g, u, dn = local_stack if codes is None else (codes.wg_q, codes.wu_q, codes.wd_q)
         if g.dim() != 3 or g.shape[0] != n_local or g.shape[2] != d or u.shape != g.shape \
                 or dn.shape != (n_local, d, g.shape[1]):
             raise ValueError(f"rank {rank} holds {n_local} expert instances: its stack must be gate/up "
@@ -612,9 +618,9 @@ class DistMoEBlock(nn.Module):
             timeout_ms = wait_timeout_ms if wait_timeout_ms is not None else min(self.forward_timeout, 5000)
             self._ep = {
                 "world": world, "rank": rank, "inst": inst, "win": win, "cap": capacity, "policy": policy,
-                "n_local": n_local, "stack": (g, u, dn), "max_tokens": max_tokens,
+                "n_local": n_local, "stack": None if blocks else (g, u, dn), "max_tokens": max_tokens,
                 "fp8": N.Fp8Experts(g, u, dn) if fp8 and n_local > 0 else None, "is_fp8": fp8,
-                "blocks": N.Fp8BlockExperts(g, u, dn) if blocks and n_local > 0 else None,
+                "blocks": None if not blocks or n_local == 0 else N.Fp8BlockExperts(g, u, dn) if codes is None else codes,
                 "is_blocks": blocks,
                 "blocks_ws": torch.empty(N.ep_fp8_blocks_workspace(capacity, g.shape[1]), dtype=torch.uint8, device=dev)
                 if blocks and n_local > 0 else None,
@@ -736,7 +742,6 @@ class DistMoEBlock(nn.Module):
         N.ep_wait(win, N.EP_FLAG_DATA, tmo, dev)
         if ep["n_local"] > 0:
             # The down-projection stores every row straight into its host's return rows.
-            g, u, dn = ep["stack"]
             rows = T * k if ep["world"] == 1 else None
             segs = (ep["seg_expert"][:ep["n_local"]], ep["seg_end"][:ep["n_local"]])
             act = ACTIVATIONS[self.config.activation]
@@ -747,7 +752,7 @@ class DistMoEBlock(nn.Module):
                 hint = max(1, -(-ep["world"] * T * k // max(1, inst.n_inst)))
                 N.ep_expert_mlp_fp8_blocks(win, ep["blocks"], *segs, cap, act, ep["blocks_ws"], hint, work_rows=rows)
             else:
-                N.ep_expert_mlp(win, g, u, dn, *segs, cap, act, self._direct_tile_policy(T), work_rows=rows)
+                N.ep_expert_mlp(win, *ep["stack"], *segs, cap, act, self._direct_tile_policy(T), work_rows=rows)
         N.ep_signal(win, N.EP_FLAG_RESULTS, dev)
         N.ep_wait(win, N.EP_FLAG_RESULTS, tmo, dev)
         if T > 0:

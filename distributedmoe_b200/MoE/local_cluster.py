@@ -17,6 +17,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
+from distributedmoe_b200 import _native as N
 from distributedmoe_b200.MoE.DistExpertsBlock import DistExpertsBlock
 from distributedmoe_b200.MoE.DistMoEBlock import DistMoEBlock, DistMoEBlockConfig
 from distributedmoe_b200.TensorTransferEngine.TensorTransferEngine import (
@@ -76,7 +77,8 @@ class LocalCluster:
     """``with LocalCluster(...) as moe: y = moe(x)``.
 
     expert_layers: one list per block of modules with gate_proj/up_proj/down_proj, or
-    ``stacked`` = one (gate, up, down) tuple per block of already stacked device tensors."""
+    ``stacked`` = one (gate, up, down) tuple per block of already stacked device tensors, or one
+    Fp8BlockExperts per block (expert_precision "fp8_block")."""
 
     def __init__(self, number_of_experts: int, expert_blocks: List[List[int]], top_k: int, hidden_features: int,
                  dtype: torch.dtype, moe_device: torch.device, eb_devices: Sequence[torch.device],
@@ -102,6 +104,10 @@ class LocalCluster:
         direct = backend == TensorTransferEngineBackend.NVLinkDirect
         if direct and any(torch.device(d) != torch.device(moe_device) for d in eb_devices):
             raise ValueError("the single-process device-driven plane needs every block on the host's GPU")
+        coded = [isinstance(st, N.Fp8BlockExperts) for st in stacked or []]
+        if any(coded) and not (all(coded) and direct and expert_precision == "fp8_block"):
+            raise ValueError("stacks of 8-bit codes run on the device-driven plane with expert_precision 'fp8_block', all "
+                             "blocks alike")
         self.config = DistMoEBlockConfig(
             backend=backend, number_of_experts=number_of_experts,
             expert_blocks=expert_blocks, number_of_io_buffers=number_of_io_buffers, io_buffer_size=io_buffer_size,
@@ -145,8 +151,11 @@ class LocalCluster:
                 else:
                     from distributedmoe_b200.MoE.DistExpertsBlock import stack_expert_weights
                     stacks = [stack_expert_weights(expert_layers[b], self.config.moe_device, dtype) for b in range(nb)]
-                local = stacks[0] if nb == 1 else tuple(torch.cat([st[i] for st in stacks]).contiguous()
-                                                        for i in range(3))
+                if any(coded):
+                    local = N.Fp8BlockExperts.cat(stacks)
+                else:
+                    local = stacks[0] if nb == 1 else tuple(torch.cat([st[i] for st in stacks]).contiguous()
+                                                            for i in range(3))
                 mt = max_tokens if max_tokens is not None else max(1, io_buffer_size * number_of_io_buffers // top_k)
                 self.moe.setup_direct_plane(1, 0, [0] * nb, local, mt * top_k, lambda mine: [mine], mt,
                                             cuda_graphs=cuda_graphs, expert_precision=expert_precision)

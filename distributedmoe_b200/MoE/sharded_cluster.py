@@ -93,7 +93,8 @@ def experts_of_rank(number_of_experts: int, world: int, rank: int) -> List[int]:
 class ShardedCluster:
     """``with ShardedCluster(...) as moe: y = moe(x_local)`` on every rank.
 
-    stacked: this rank's (gate [E_g, I, d], up [E_g, I, d], down [E_g, d, I]) on its GPU.
+    stacked: this rank's (gate [E_g, I, d], up [E_g, I, d], down [E_g, d, I]) on its GPU, or an
+    Fp8BlockExperts of them (expert_precision "fp8_block").
     gemm_sm_reserve: SMs the grouped-MLP launches of this process leave free (process-wide)."""
 
     def __init__(self, number_of_experts: int, top_k: int, hidden_features: int, dtype: torch.dtype,
@@ -114,6 +115,9 @@ class ShardedCluster:
         cores, "fp8_block" all three projections with a scale for each block of 128
         (DistMoEBlock.setup_direct_plane)."""
         direct = backend == TensorTransferEngineBackend.NVLinkDirect
+        coded = isinstance(stacked, N.Fp8BlockExperts)
+        if coded and not (direct and expert_precision == "fp8_block"):
+            raise ValueError("a stack of 8-bit codes runs on the device-driven plane with expert_precision 'fp8_block'")
         if direct:
             # The task buffers only serve the metadata hand-shake: keep them small.
             io_buffer_size = io_buffer_size or 256
@@ -188,9 +192,11 @@ class ShardedCluster:
             self.moe = DistMoEBlock(config_of_host(r), host_tte)
             # Load the grouped-MLP kernels once here rather than inside a block's first task,
             # where the first launches would delay its health-check replies.
-            g, u, dn = stacked
             rows = torch.zeros(256, hidden_features, dtype=dtype, device=device)
-            N.grouped_gated_mlp(rows, g, u, dn, [0], [256], N.ACT_SILU, torch.empty_like(rows))
+            if coded:
+                N.grouped_gated_mlp_fp8_blocks(*N.quantize_blocks_e4m3(rows), stacked, [0], [256], N.ACT_SILU)
+            else:
+                N.grouped_gated_mlp(rows, *stacked, [0], [256], N.ACT_SILU, torch.empty_like(rows))
             torch.cuda.synchronize(device)
             if direct:
                 self.moe.setup_direct_plane(G, r, list(range(G)), stacked, G * max_tokens * top_k,

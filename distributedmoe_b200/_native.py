@@ -835,6 +835,21 @@ class Fp8BlockExperts:
         self._set(wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale)
         return self
 
+    @classmethod
+    def cat(cls, stacks: Sequence["Fp8BlockExperts"]) -> "Fp8BlockExperts":
+        """One stack of the experts of several, in order (their own tensors where there is one)."""
+        if len(stacks) == 1:
+            return stacks[0]
+
+        def codes(name):
+            return torch.cat([getattr(s, name).view(torch.uint8) for s in stacks]).view(torch.float8_e4m3fn)
+
+        def scales(name):
+            return torch.cat([getattr(s, name) for s in stacks])
+
+        return cls.from_quantized(codes("wg_q"), scales("wg_scale"), codes("wu_q"), scales("wu_scale"), codes("wd_q"),
+                                  scales("wd_scale"))
+
     def _set(self, wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale) -> None:
         _one_device(wg_q, wg_scale, wu_q, wu_scale, wd_q, wd_scale)
         shape = wg_q.shape
@@ -858,6 +873,10 @@ class Fp8BlockExperts:
     @property
     def shape(self):
         return self.wg_q.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.wg_q.device
 
 
 def grouped_gated_mlp_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, experts: Fp8BlockExperts, seg_expert,

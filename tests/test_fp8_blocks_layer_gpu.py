@@ -121,3 +121,91 @@ def test_direct_layer_refusals():
         with pytest.raises(ValueError):
             LocalCluster(2, [[0, 1]], 1, d, dtype, dev, [dev], stacked=[stack], io_buffer_size=64, number_of_io_buffers=1,
                          backend=B.NVLinkDirect, max_tokens=16, expert_precision=precision)
+
+
+def _codes(E, n, k, g):
+    """A stack as another program may have quantised it: scales that this framework's quantiser would not
+    choose (a block's largest code is not 448), values that bf16 does not hold."""
+    q = (torch.randn(E, n, k, generator=g, device=DEV) * 40).clamp(-300, 300).to(torch.float8_e4m3fn)
+    s = 1e-3 * (1 + torch.rand(E, -(-n // 128), -(-k // 128), generator=g, device=DEV))
+    return q, s
+
+
+def _expected_of(x, idx, w, values):
+    """_expected for weights given as the values [E, ., .] that their codes stand for."""
+    y = torch.zeros(x.shape, dtype=torch.float64, device=DEV)
+    slack, size = torch.zeros_like(y), torch.zeros_like(y)
+    xv = _values(*_quantize64(x), 1)
+    for e in range(values[0].shape[0]):
+        t, slot = torch.where(idx == e)
+        if t.numel() == 0:
+            continue
+        rows, err = _mlp_reference(xv[t], *(m[e] for m in values), True)
+        share = w[t, slot].double()[:, None]
+        y.index_add_(0, t, share * rows)
+        slack.index_add_(0, t, share * err)
+        size.index_add_(0, t, share * (rows.abs() + err))
+    slack = slack + (2.0 ** -8 + idx.shape[1] * 2.0 ** -23) * size
+    return y, slack + 2.0 ** -8 * (y.abs() + slack)
+
+
+def _cluster(E, blocks, k, d, stacked, **kw):
+    from distributedmoe_b200.MoE.local_cluster import LocalCluster
+    from distributedmoe_b200.TensorTransferEngine import TensorTransferEngineBackend as B
+    dev = torch.device(DEV)
+    kw = dict(dict(backend=B.NVLinkDirect, expert_precision="fp8_block"), **kw)
+    return LocalCluster(E, blocks, k, d, torch.bfloat16, dev, [dev] * len(blocks), stacked=stacked, io_buffer_size=256,
+                        number_of_io_buffers=1, max_tokens=512, activation="silu", renormalize=True, **kw)
+
+
+@gpu
+@pytest.mark.parametrize("blocks", [[[0, 1, 2, 3, 4, 5]], [[0, 1, 2], [3, 4, 5], [1, 4]]], ids=["one", "replicas"])
+@pytest.mark.parametrize("graphs", [False, True])
+def test_direct_layer_from_a_checkpoints_codes(blocks, graphs):
+    """The layer computes on the codes it is given, without copies of them where there is one block, and
+    keeps no 16-bit weights."""
+    N = _nat()
+    E, k, d, I = 6, 2, 272, 400
+    g = torch.Generator(device=DEV).manual_seed(31)
+    (gq, gs), (uq, us), (dq, ds) = _codes(E, I, d, g), _codes(E, I, d, g), _codes(E, d, I, g)
+    values = [_values(q, s, 128) for q, s in ((gq, gs), (uq, us), (dq, ds))]
+    w_r = (torch.randn(E, d, generator=g, device=DEV) * 0.05).to(torch.bfloat16)
+    stacked = [N.Fp8BlockExperts.from_quantized(*(t.view(torch.uint8)[b].view(t.dtype) if t.dtype == gq.dtype else t[b]
+                                                  for t in (gq, gs, uq, us, dq, ds))) for b in blocks]
+    cl = _cluster(E, blocks, k, d, stacked, cuda_graphs=graphs)
+    outs = []
+    try:
+        with torch.no_grad():
+            cl.moe.gate.weight.copy_(w_r)
+        assert cl.moe._ep["stack"] is None
+        if len(blocks) == 1:
+            assert cl.moe._ep["blocks"] is stacked[0]
+        for T in (1, 300, 512, 300):
+            x = torch.randn(T, d, generator=g, device=DEV).to(torch.bfloat16)
+            outs.append((x, cl.moe(x)))
+        torch.cuda.synchronize()
+        N.check_device_status(torch.device(DEV))
+    finally:
+        cl.close()
+    for x, y in outs:
+        idx, w, _ = N.router(x, w_r, k, renormalize=True, w_dtype=torch.float32)
+        want, slack = _expected_of(x, idx, w, values)
+        assert ((y.double() - want).abs() - slack).max().item() <= 0
+
+
+@gpu
+def test_codes_where_they_do_not_belong():
+    from distributedmoe_b200.TensorTransferEngine import TensorTransferEngineBackend as B
+    N = _nat()
+    g = torch.Generator(device=DEV).manual_seed(1)
+    d, I = 256, 384
+    codes = N.Fp8BlockExperts.from_quantized(*_codes(2, I, d, g), *_codes(2, I, d, g), *_codes(2, d, I, g))
+    stack = tuple(torch.zeros(2, *s, dtype=torch.bfloat16, device=DEV) for s in ((I, d), (I, d), (d, I)))
+    for blocks, stacked, kw in (([[0, 1]], [codes], dict(expert_precision="model")),
+                                ([[0, 1]], [codes], dict(expert_precision="fp8")),
+                                ([[0, 1]], [codes], dict(backend=B.NVLinkIPC)),
+                                ([[0, 1], [0, 1]], [codes, stack], {})):
+        with pytest.raises(ValueError, match="codes"):
+            _cluster(2, blocks, 1, d, stacked, **kw)
+    with pytest.raises(ValueError, match="its stack must be"):
+        _cluster(3, [[0, 1, 2]], 1, d, [codes])
