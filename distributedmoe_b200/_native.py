@@ -631,11 +631,12 @@ def grouped_gated_mlp_fp8(Xq: torch.Tensor, x_scale: torch.Tensor, experts: Fp8E
 FP8_BLOCK = 128
 
 
-def _int32(*sizes: int) -> None:
-    """Refuse numbers that the library takes as 32-bit ones and ctypes would wrap."""
-    for n in sizes:
-        if not -0x80000000 <= n <= 0x7FFFFFFF:
-            raise DMoEError(f"{n} is past the 2^31 - 1 that the library takes")
+# The library takes sizes as 32-bit numbers, and ctypes would wrap others.
+_MOST = 0x7FFFFFFF
+
+
+def _too_large(*sizes: int) -> None:
+    raise DMoEError(f"{max(sizes, key=abs)} is past the 2^31 - 1 that the library takes")
 
 
 def _blocks(n: int) -> int:
@@ -657,7 +658,8 @@ def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Te
     cols = shape[-1] if shape else 0
     if cols == 0 or cols % 16:
         raise DMoEError("x must be [..., cols] ([..., rows, cols] for 128 x 128 blocks) with cols a multiple of 16")
-    _int32(cols)
+    if cols > _MOST:
+        _too_large(cols)
     nb = -(-cols // FP8_BLOCK)
     if block_rows == 1:
         batch, rows = 1, x.numel() // cols
@@ -679,7 +681,8 @@ def quantize_blocks_e4m3(x: torch.Tensor, block_rows: int = 1) -> Tuple[torch.Te
 
 def _check_weight_blocks(q: torch.Tensor, scale: torch.Tensor, E: Optional[int], n: int, k: int, what: str) -> None:
     """A stack q [E, n, k] (E None: one matrix [n, k]) and its scales."""
-    _int32(E or 1, n, k)
+    if n > _MOST or k > _MOST or (E is not None and E > _MOST):
+        _too_large(E or 1, n, k)
     if q.dtype is not torch.float8_e4m3fn or scale.dtype is not torch.float32:
         raise DMoEError(f"{what} must be float8_e4m3fn with fp32 scales")
     nb, kb = -(-n // FP8_BLOCK), -(-k // FP8_BLOCK)
@@ -696,7 +699,8 @@ def _check_row_blocks(xq: torch.Tensor, x_scale: torch.Tensor, K: int) -> Tuple[
     shape, nb = xq.shape, -(-K // FP8_BLOCK)
     if len(shape) != 2 or shape[1] != K or x_scale.shape != (shape[0], nb):
         raise DMoEError(f"xq must be [rows, {K}] with scales [rows, {nb}]")
-    _int32(shape[0])
+    if shape[0] > _MOST:
+        _too_large(shape[0])
     a, b = xq.stride(), x_scale.stride()
     if (K > 1 and a[1] != 1) or (nb > 1 and b[1] != 1):
         raise DMoEError("the columns of xq and of its scales must be contiguous")
@@ -711,14 +715,18 @@ def _segments(seg_expert, seg_end, dev: int):
             raise DMoEError("a segment table on the device is two contiguous int32 tensors of one length")
         if seg_expert.get_device() != dev or seg_end.get_device() != dev:
             raise DMoEError(f"the segment table must be on cuda:{dev}")
-        _int32(seg_expert.numel())
-        return seg_expert.data_ptr(), seg_end.data_ptr(), seg_expert.numel(), 1, None
+        n = seg_expert.numel()
+        if n > _MOST:
+            _too_large(n)
+        return seg_expert.data_ptr(), seg_end.data_ptr(), n, 1, None
     if isinstance(seg_expert, torch.Tensor) or isinstance(seg_end, torch.Tensor):
         raise DMoEError("a segment table is two int32 CUDA tensors or two sequences of numbers")
     n = len(seg_expert)
     if n != len(seg_end):
         raise DMoEError("seg_expert and seg_end differ in length")
-    _int32(n, *map(int, seg_expert), *map(int, seg_end))
+    for v in (seg_expert, seg_end):
+        if n and (max(v) > _MOST or min(v) < -_MOST):
+            _too_large(*map(int, v))
     a1, a2 = _i32_array(seg_expert), _i32_array(seg_end)
     return ctypes.addressof(a1), ctypes.addressof(a2), n, 0, (a1, a2)
 
@@ -730,7 +738,8 @@ _FIRST_EXPERT = _Int32(0)
 def _product(xq, x_scale, w_q, w_scale, E, Nn, K, table, out, out_dtype, rows_hint) -> torch.Tensor:
     """table: (seg_expert, seg_end), or None for one segment of all rows and one matrix w_q (E None)."""
     dev = _one_device(xq, x_scale, w_q, w_scale, out)
-    _int32(rows_hint)
+    if abs(rows_hint) > _MOST:
+        _too_large(rows_hint)
     _check_weight_blocks(w_q, w_scale, E, Nn, K, "w_q")
     m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, K)
     if out is None:
@@ -789,7 +798,8 @@ def quantize_block_records(x: torch.Tensor, out: Optional[torch.Tensor] = None) 
     T, d = x.shape
     if d == 0 or d % 16 or not x.is_contiguous():
         raise DMoEError(f"8-bit records need a contiguous x with d % 16 == 0 (d={d})")
-    _int32(d)
+    if d > _MOST:
+        _too_large(d)
     rec = fp8_block_record_bytes(d)
     if out is None:
         out = torch.empty(T, rec, dtype=torch.uint8, device=x.device)
@@ -886,8 +896,9 @@ def grouped_gated_mlp_fp8_blocks(xq: torch.Tensor, x_scale: torch.Tensor, expert
     1 x 128 in the epilogue, Y = h Wd^T in bf16.  xq [rows, d] with x_scale [rows, ceil(d / 128)]
     (rows may be strided); segments and rows_hint as :func:`grouped_matmul_fp8_blocks`; rows outside
     the segments are not written.  Returns Y [rows, d] (a new tensor if not given)."""
-    dev = _one_device(xq, x_scale, experts.wg_q, Y)
-    _int32(rows_hint, act)
+    dev = _one_device(xq, x_scale, experts._wg_q, Y)
+    if abs(rows_hint) > _MOST or abs(act) > _MOST:
+        _too_large(rows_hint, act)
     stacks = experts._args()
     d, I = stacks[-2:]
     m, x_ld, xs_ld = _check_row_blocks(xq, x_scale, d)
@@ -913,14 +924,15 @@ class _BalanceLoss(torch.autograd.Function):
         k = idx.shape[1]
         S = 1 if seq_end is None else seq_end.numel()
         code = dtype_code(logits.dtype)
-        counts = torch.empty(S * (E + 1) + 1, dtype=torch.int32, device=device)
+        nbytes = lib().dmoe_balance_loss_workspace_size()
+        # counts, then the workspace from an 8-byte boundary on
+        at = (S * (E + 1) + 2) & ~1
+        counts = torch.empty(at + nbytes // 4, dtype=torch.int32, device=device)
         per_expert = torch.empty(S, E, dtype=torch.int32, device=device)  # the caller's own, who may add other ranks' to it
         loss = torch.empty(2, dtype=torch.float32, device=device)
-        nbytes = lib().dmoe_balance_loss_workspace_size()
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         _call(dev, "balance_loss", lib().dmoe_balance_loss, logits.data_ptr(), code, idx.data_ptr(), T, E, k, mode,
-              _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), per_expert.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes,
-              scratch.status(device).data_ptr())
+              _ptr(seq_end), S, _ptr(mask), counts.data_ptr(), per_expert.data_ptr(), loss.data_ptr(),
+              counts.data_ptr() + 4 * at, nbytes, scratch.status(device).data_ptr())
         ctx.save_for_backward(logits, seq_end, mask, counts)
         ctx.args = (dev, code, T, E, k, mode, S)
         ctx.set_materialize_grads(False)
@@ -974,7 +986,9 @@ def balance_loss(logits: torch.Tensor, idx: torch.Tensor, *, mode: int = ROUTER_
         raise DMoEError("seq_end must be an int32 vector")
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != logits.shape[:1]):
         raise DMoEError("mask must be bool [T]")
-    _int32(*logits.shape, idx.shape[1], int(mode), 0 if seq_end is None else seq_end.numel())
+    T, E = logits.shape
+    if T > _MOST or E > _MOST or idx.shape[1] > _MOST or abs(mode) > _MOST or (seq_end is not None and seq_end.numel() > _MOST):
+        _too_large(T, E, idx.shape[1], int(mode), 0 if seq_end is None else seq_end.numel())
     return _BalanceLoss.apply(logits, idx, int(mode), seq_end, mask, dev)
 
 
@@ -1183,7 +1197,8 @@ def ep_expert_mlp_fp8_blocks(win: EpWindow, experts: Fp8BlockExperts, seg_expert
     e4m3 stacks, down projection included; the return rows are bf16.  workspace: uint8, at least
     ``ep_fp8_blocks_workspace(cap, I)`` bytes; rows_hint: rows an instance is expected to have."""
     dev = _one_device(experts.wd_q, seg_expert, seg_end, workspace)
-    _int32(rows_hint, act, seg_expert.numel())
+    if abs(rows_hint) > _MOST or abs(act) > _MOST or seg_expert.numel() > _MOST:
+        _too_large(rows_hint, act, seg_expert.numel())
     device = seg_expert.device
     stacks = experts._args()
     E, d, I = stacks[-3:]
