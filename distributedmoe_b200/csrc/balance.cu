@@ -385,7 +385,11 @@ __global__ void __launch_bounds__(kBalThreads)
 // distributed shared memory and goes on to the losses.
 constexpr int kSmallRanks = 8;
 constexpr int kSmallCounts = 1024;        // n_seq * (E + 1) at most
-constexpr int64_t kSmallLogits = 1 << 15;  // T * E at most: 4096 x 8 takes 12 us against 11 in three launches
+// T * E at most.  One launch saves the host 4 us (24.5 against 28.5 a call at every size here), and the GPU
+// 3-6 us where tokens are few: 64 x 64 takes 4.3 us against 10.4 in three launches, 512 x 64 7.4 against
+// 11.0, 256 x 128 6.1 against 11.3.  The more tokens, the less: 4096 x 8 10.7 against 10.4, and past the limit
+// 8192 x 8 17.6 against 10.4 (16384 x 8 then also costs the call: 32.9 against 28.5).
+constexpr int64_t kSmallLogits = 1 << 15;
 
 __device__ __forceinline__ uint32_t in_rank(const void* p, int rank) {
   uint32_t r;

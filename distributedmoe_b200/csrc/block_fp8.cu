@@ -25,9 +25,10 @@
 // TMEM holds two: a step's MMAs (512 cycles) and its way through the epilogue (about 1,000: commit, wake,
 // 128 columns a warp read and added, hand-back) overlap with the next step's and no further.
 //
-// What bounds them, measured on a B200: many rows, a step takes about 720 cycles of 512 (4096 x 14336
-// x 4096 in 216-224 us, 2.2 PFLOP/s, against 174 us for the same loop without scales, one read-back a
-// tile) and the power cap holds the clock at 1.3-1.6 GHz meanwhile; few rows, HBM (512 rows over 32
+// What bounds them, measured on a B200: many rows, the way of an accumulator from its first MMA to its
+// hand-back, about 1,400 cycles, which two accumulators share: a step takes 700-720 cycles where its MMAs
+// take 512 (4096 x 14336 x 4096 in 216-230 us, 2.1-2.2 PFLOP/s, against 174 us for the same loop without
+// scales, one read-back a tile; long runs meet the power cap besides); few rows, HBM (512 rows over 32
 // experts of 7168/2048: gate/up 939 MB in 160 us, down 470 MB in 85 us, 5.5-5.9 TB/s); one token
 // through 14336 x 4096, 59 MB in 16 us: 1.3 us to set up, 11 us of memory, 2.7 us to join and leave.
 #include <cuda_fp8.h>
@@ -1308,9 +1309,12 @@ int run_product(Product& p, const BlkSegs& segs, int hint, cudaStream_t stream) 
   const int64_t by_pair = segs.dev_end ? (int64_t)(rows + kPM / 2) * used : (int64_t)row_tiles(segs, kPM) * kPM;
   const int64_t by_single = segs.dev_end ? (int64_t)(rows + 64) * used : (int64_t)row_tiles(segs, 128) * 128;
   if (tile_m == 128 && by_pair * 93 < by_single * 100) return launch_pair<GATED>(p, segs, row_tiles(segs, kPM), stream);
-  // Long reductions: the tiles of a last, partly empty wave are split over two SMs each (1002 rows over
-  // 8 experts at 4096 x 14336: 125 -> 112 us; 8192 over 32 at 2048 x 7168: 172 -> 168).  Short ones lose
-  // more by the cluster launch (500 rows over 8 at 4096 x 4096: 29.8 -> 30.5 us).
+  // Long reductions: the tiles of a last, partly empty wave are split over two SMs each.  The kernel's rule
+  // lets 128-row tiles go to two from 44 blocks of K on (k_blk / 2 + 24 <= k_blk + 2); below, the cluster
+  // launch alone is left (1002 rows over 8 experts, N = 4096, whole -> split: 32 blocks 41.0 -> 41.7 us, 40
+  // 49.3 -> 49.9, 44 53.9 -> 51.5, 48 57.6 -> 53.8, 56 65.9 -> 60.9; 8192 rows over 32, N = 2048: 32 103.4 ->
+  // 104.6, 48 164.6 -> 156.7, 56 174.1 -> 169.3; 500 rows over 8, whose last wave is too full for it: 32
+  // 28.6 -> 29.0, 56 46.3 -> 46.6).
   if (p.args.k_blk >= 48) return launch_single<GATED, true>(p, segs, tile_m, m_tiles, 2, stream);
   return launch_single<GATED, false>(p, segs, tile_m, m_tiles, 1, stream);
 }
