@@ -358,15 +358,19 @@ __device__ __forceinline__ float2 two_factors(float x, float w) {
   return make_float2(m * power_of_two(e1), power_of_two(min(max(e - e1, -126), 127)));
 }
 
+// A scale.  Not by the read-only path: this kernel may have started before the one ahead of it in the stream,
+// which may be writing these, had ended, and that path takes only what no one writes while a kernel runs.
+__device__ __forceinline__ float scale_at(const float* p) { return *p; }
+
 // add_step where the product of two scales is no normal number in some lane: sums times the normal products
 // as there, then the others as (sum * c1) * c2.  x, w0, w1: the step's scales, read once more.
 template <bool GATED, class F>
 __device__ __forceinline__ void add_step_any(uint64_t (&sum)[64], uint32_t tbase, int half, const float* x, const float* w0,
                                              const float* w1, F&& release) {
-  const float xs = __ldg(x);
+  const float xs = scale_at(x);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float w = __ldg(!GATED || j < 4 ? w0 : w1), s = normal(xs * w) ? xs * w : 0.f;
+    const float w = scale_at(!GATED || j < 4 ? w0 : w1), s = normal(xs * w) ? xs * w : 0.f;
     const float2 c = two_factors(xs, w);
     const uint64_t sp = pack_f2(s, s), p1 = pack_f2(c.x, c.x), p2 = pack_f2(c.y, c.y);
     uint32_t v[16];
@@ -497,18 +501,18 @@ struct StepScales {
     const int64_t at = ((int64_t)t.expert * a.n_blk + nb) * a.k_blk;
     w0 = a.ws0 + at;
     w1 = GATED ? a.ws1 + at : w0;
-    xn = __ldg(x + kb);
-    an = __ldg(w0 + kb);
-    bn = GATED ? __ldg(w1 + kb) : an;
+    xn = scale_at(x + kb);
+    an = scale_at(w0 + kb);
+    bn = GATED ? scale_at(w1 + kb) : an;
   }
   template <bool GATED>
   __device__ __forceinline__ void take(int kb, int end, float& s0, float& s1) {
     s0 = xn * an;
     s1 = xn * bn;
     if (kb + 1 < end) {
-      xn = __ldg(x + kb + 1);
-      an = __ldg(w0 + kb + 1);
-      bn = GATED ? __ldg(w1 + kb + 1) : an;
+      xn = scale_at(x + kb + 1);
+      an = scale_at(w0 + kb + 1);
+      bn = GATED ? scale_at(w1 + kb + 1) : an;
     }
   }
 };
