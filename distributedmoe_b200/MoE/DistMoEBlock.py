@@ -580,7 +580,7 @@ class DistMoEBlock(nn.Module):
         128 x 128 block of all three projections and for each 128 values of a token row, the form
         in which 8-bit checkpoints are published (bf16 layers, hidden and inner % 16 == 0);
         local_stack may then be such a checkpoint's codes and scales themselves, an
-        Fp8BlockExperts of this rank's S instances."""
+        Fp8BlockExperts of this rank's S instances, whose present tensors it keeps."""
         tte = self.tensor_transfer_engine
         if not getattr(tte, "direct", False):
             raise RuntimeError("the device-driven data plane needs the NVLinkDirect backend")
@@ -591,6 +591,9 @@ class DistMoEBlock(nn.Module):
         if codes is not None and (expert_precision != "fp8_block" or codes.device != self.device):
             raise ValueError(f"a stack of 8-bit codes runs on its own GPU with expert_precision 'fp8_block', not "
                              f"{expert_precision!r} on {self.device}")
+        if codes is not None:
+            # A stack of the plane's own: captured graphs hold its tensors' addresses, the caller may exchange theirs.
+            codes = N.Fp8BlockExperts.cat([codes])
         g, u, dn = local_stack if codes is None else (codes.wg_q, codes.wu_q, codes.wd_q)
         if g.dim() != 3 or g.shape[0] != n_local or g.shape[2] != d or u.shape != g.shape \
                 or dn.shape != (n_local, d, g.shape[1]):

@@ -847,9 +847,10 @@ class Fp8BlockExperts:
 
     @classmethod
     def cat(cls, stacks: Sequence["Fp8BlockExperts"]) -> "Fp8BlockExperts":
-        """One stack of the experts of several, in order (their own tensors where there is one)."""
+        """One stack of the experts of several, in order; of one, a stack of the same tensors."""
         if len(stacks) == 1:
-            return stacks[0]
+            s, = stacks
+            return cls.from_quantized(s.wg_q, s.wg_scale, s.wu_q, s.wu_scale, s.wd_q, s.wd_scale)
 
         def codes(name):
             return torch.cat([getattr(s, name).view(torch.uint8) for s in stacks]).view(torch.float8_e4m3fn)

@@ -179,7 +179,7 @@ def test_direct_layer_from_a_checkpoints_codes(blocks, graphs):
             cl.moe.gate.weight.copy_(w_r)
         assert cl.moe._ep["stack"] is None
         if len(blocks) == 1:
-            assert cl.moe._ep["blocks"] is stacked[0]
+            assert cl.moe._ep["blocks"]._args() == stacked[0]._args()
         for T in (1, 300, 512, 300):
             x = torch.randn(T, d, generator=g, device=DEV).to(torch.bfloat16)
             outs.append((x, cl.moe(x)))
@@ -209,3 +209,70 @@ def test_codes_where_they_do_not_belong():
             _cluster(2, blocks, 1, d, stacked, **kw)
     with pytest.raises(ValueError, match="its stack must be"):
         _cluster(3, [[0, 1, 2]], 1, d, [codes])
+
+
+@gpu
+@pytest.mark.parametrize("graphs", [False, True])
+def test_the_layer_keeps_the_codes_it_was_given(graphs):
+    """A tensor that replaces another in the caller's stack is not the layer's: a captured graph would go on
+    with the old one, which might be freed by then."""
+    N = _nat()
+    E, k, d, I = 4, 2, 256, 272
+    g = torch.Generator(device=DEV).manual_seed(2)
+    parts = [*_codes(E, I, d, g), *_codes(E, I, d, g), *_codes(E, d, I, g)]
+    codes = N.Fp8BlockExperts.from_quantized(*parts)
+    cl = _cluster(E, [list(range(E))], k, d, [codes], cuda_graphs=graphs)
+    try:
+        x = torch.randn(64, d, generator=g, device=DEV).to(torch.bfloat16)
+        first = [cl.moe(x) for _ in range(3)][-1]
+        codes.wd_scale = parts[5] * 2
+        assert torch.equal(cl.moe(x), first)
+        parts[5].mul_(2)  # values changed in place are seen
+        assert torch.equal(cl.moe(x), first * 2)
+        N.check_device_status(torch.device(DEV))
+    finally:
+        cl.close()
+
+
+@gpu
+def test_one_rank_of_the_sharded_cluster_from_codes():
+    """The launch that puts one rank on each GPU, with one rank."""
+    import socket
+    from datetime import timedelta
+
+    import torch.distributed as dist
+
+    from distributedmoe_b200.MoE.sharded_cluster import ShardedCluster
+    from distributedmoe_b200.TensorTransferEngine import TensorTransferEngineBackend as B
+    N = _nat()
+    E, k, d, I = 4, 2, 256, 272
+    g = torch.Generator(device=DEV).manual_seed(3)
+    (gq, gs), (uq, us), (dq, ds) = _codes(E, I, d, g), _codes(E, I, d, g), _codes(E, d, I, g)
+    codes = N.Fp8BlockExperts.from_quantized(gq, gs, uq, us, dq, ds)
+    w_r = (torch.randn(E, d, generator=g, device=DEV) * 0.05).to(torch.bfloat16)
+    dev = torch.device(DEV)
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=0, world_size=1,
+                            timeout=timedelta(seconds=60))
+    try:
+        for bad in (dict(expert_precision="model"), dict(expert_precision="fp8_block", backend=B.NVLinkIPC)):
+            with pytest.raises(ValueError, match="codes"):
+                ShardedCluster(E, k, d, torch.bfloat16, dev, codes, max_tokens=256, **bad)
+        cl = ShardedCluster(E, k, d, torch.bfloat16, dev, codes, activation="silu", renormalize=True, max_tokens=256,
+                            expert_precision="fp8_block")
+        try:
+            with torch.no_grad():
+                cl.moe.gate.weight.copy_(w_r)
+            x = torch.randn(200, d, generator=g, device=DEV).to(torch.bfloat16)
+            y = cl.moe(x)
+            torch.cuda.synchronize()
+            N.check_device_status(dev)
+        finally:
+            cl.close()
+    finally:
+        dist.destroy_process_group()
+    idx, w, _ = N.router(x, w_r, k, renormalize=True, w_dtype=torch.float32)
+    want, slack = _expected_of(x, idx, w, [_values(q, s, 128) for q, s in ((gq, gs), (uq, us), (dq, ds))])
+    assert ((y.double() - want).abs() - slack).max().item() <= 0
