@@ -795,6 +795,8 @@ def fp8_block_record_bytes(d: int) -> int:
 def quantize_block_records(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [T, d] -> uint8 records [T, fp8_block_record_bytes(d)]: row t's codes, then its scales."""
     dev = _one_device(x, out)
+    if x.dim() != 2:
+        raise DMoEError("8-bit records need x [T, d]")
     T, d = x.shape
     if d == 0 or d % 16 or not x.is_contiguous():
         raise DMoEError(f"8-bit records need a contiguous x with d % 16 == 0 (d={d})")

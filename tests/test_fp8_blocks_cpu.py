@@ -234,3 +234,10 @@ def test_replaced_weights_are_checked(monkeypatch):
             setattr(ex, name, t)
     ex.wd_scale = ds * 2
     assert torch.equal(ex.wd_scale, ds * 2) and ex._args()[5] == ex.wd_scale.data_ptr()
+
+
+def test_records_of_rows_only(monkeypatch):
+    monkeypatch.setattr(N, "_one_device", lambda *t: 0)
+    for shape in ((256,), (2, 3, 256)):
+        with pytest.raises(N.DMoEError):
+            N.quantize_block_records(torch.zeros(shape))
